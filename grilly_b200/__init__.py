@@ -13,11 +13,12 @@ from . import _lib
 from .compute import Compute
 from .device import Device, DeviceTensor
 from .encoder import SentenceEncoder, EncoderWeights
+from .rows8 import NormQ8, Rows8
 
 __version__ = "0.2.0"
 VULKAN_AVAILABLE = False  # nothing here goes through Vulkan
 
-__all__ = ["Compute", "Device", "DeviceTensor", "SentenceEncoder", "EncoderWeights", "CUDA_AVAILABLE", "VULKAN_AVAILABLE"]
+__all__ = ["Compute", "Device", "DeviceTensor", "SentenceEncoder", "EncoderWeights", "Rows8", "NormQ8", "CUDA_AVAILABLE", "VULKAN_AVAILABLE"]
 
 
 def _probe() -> bool:

@@ -21,7 +21,7 @@ ELT_GELU, ELT_SILU, ELT_RELU, ELT_ADD, ELT_SWIGLU, ELT_GCU, ELT_ROSWISH = 1, 2, 
 ROPE_NONE, ROPE_INTERLEAVED, ROPE_ROTATE_HALF = 0, 1, 2
 DIST_L2, DIST_COSINE, DIST_DOT = 1, 2, 3
 ARCH_POST_LN, ARCH_MODERNBERT = 0, 1
-FLAG_OUT_BF16, FLAG_ROUND_TF32, FLAG_SWIGLU_PAIRS = 1, 2, 4
+FLAG_OUT_BF16, FLAG_ROUND_TF32, FLAG_SWIGLU_PAIRS, FLAG_IN_BF16 = 1, 2, 4, 8
 
 
 class EncoderConfig(C.Structure):
@@ -89,6 +89,12 @@ SIGNATURES = {
     "grilly_attention_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _f],
     "grilly_adam_update": [_vp, _vp, _vp, _vp, _vp, _ll, _f, _f, _f, _f, _f, _f, _i],
     "grilly_transpose_2d": [_vp, _vp, _vp, _i, _i],
+    "grilly_quantize_rows": [_vp, _vp, _vp, _vp, _ll, _i, _ll, _i],
+    "grilly_dequantize_rows": [_vp, _vp, _vp, _vp, _ll, _i, _ll, _i],
+    "grilly_rmsnorm_residual_q8": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _i, _ll, _f, _i],
+    "grilly_linear_q8": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _i, _i, _ll, _ll, _i, _i],
+    "grilly_linear_backward_q8": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _i, _i, _ll, _i],
+    "grilly_rmsnorm_backward_q8": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _i, _ll, _i],
     "grilly_encoder_create": [_vp, C.POINTER(EncoderConfig), _pp],
     "grilly_encoder_set_weight": [_vp, C.c_char_p, _i, _vp, _sz],
     "grilly_encoder_forward": [_vp, _vp, _vp, _i, _i, _vp],

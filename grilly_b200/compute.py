@@ -18,6 +18,7 @@ import numpy as np
 
 from . import _lib as L
 from .device import Device, DeviceTensor
+from .rows8 import Rows8Ops
 
 _PREC = {"tf32": L.PREC_TF32, "bf16": L.PREC_BF16, "tf32x3": L.PREC_TF32X3}
 _ACT = {None: L.ACT_NONE, "none": L.ACT_NONE, "gelu": L.ACT_GELU, "silu": L.ACT_SILU, "relu": L.ACT_RELU}
@@ -70,8 +71,9 @@ class _Namespace:
         return t.numpy() if to_host else t
 
 
-class FNN(_Namespace):
-    """backend/fnn.py ``VulkanFNN``: the GEMM family, normalisation and activations."""
+class FNN(Rows8Ops, _Namespace):
+    """backend/fnn.py ``VulkanFNN``: the GEMM family, normalisation and activations; the 8-bit row methods come from
+    :class:`~grilly_b200.rows8.Rows8Ops`."""
 
     def __init__(self, backend):
         super().__init__(backend)

@@ -1,0 +1,59 @@
+// Shared by the 8-bit row kernels (rows8.cu) and their matrix products (gemm8.cu).
+#pragma once
+#include "internal.h"
+#include <new>
+
+namespace gb {
+
+// Smallest scale of a row: 2^-126, the smallest normal fp32 number, so that 1 / scale is finite for every row.
+constexpr float ROWS8_TINY = 1.17549435e-38f;
+
+// Runs the body of an entry point under the context's lock, on the context's device (the caller's current device is
+// put back), and turns what C++ would throw into a status: nothing may unwind into a C caller.
+template <class F>
+int rows8_entry(grilly_ctx* ctx, F&& body) noexcept {
+  if (!ctx) return GRILLY_ERR_INVALID_ARG;
+  int before = -1;
+  int rc = GRILLY_ERR_CUDA;
+  try {
+    std::lock_guard<std::mutex> lock(ctx->mu);
+    if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+    if (before != ctx->device && cudaSetDevice(ctx->device) != cudaSuccess) return set_error(ctx, GRILLY_ERR_CUDA, "cudaSetDevice failed");
+    rc = body();
+  } catch (const std::bad_alloc&) {
+    rc = GRILLY_ERR_OOM;
+  } catch (...) {
+    rc = GRILLY_ERR_CUDA;
+  }
+  if (before >= 0 && before != ctx->device) cudaSetDevice(before);
+  return rc;
+}
+
+// Scratch of one call from the stream-ordered pool: taken and given back on the context's stream, so calls on other
+// streams and captured graphs never share it.
+struct Rows8Scratch {
+  grilly_ctx* ctx;
+  void* p = nullptr;
+  explicit Rows8Scratch(grilly_ctx* c) : ctx(c) {}
+  Rows8Scratch(const Rows8Scratch&) = delete;
+  int take(size_t bytes) {
+    const cudaError_t e = cudaMallocAsync(&p, bytes ? bytes : 16, ctx->stream);
+    if (e == cudaSuccess) return GRILLY_OK;
+    cudaGetLastError();
+    p = nullptr;
+    return set_error(ctx, e == cudaErrorMemoryAllocation ? GRILLY_ERR_OOM : GRILLY_ERR_CUDA,
+                     std::string("8-bit rows: scratch: ") + cudaGetErrorString(e));
+  }
+  ~Rows8Scratch() { if (p) cudaFreeAsync(p, ctx->stream); }
+};
+
+// Checks the geometry of an 8-bit row tensor.
+inline int rows8_check(grilly_ctx* ctx, const char* who, const void* q, const void* scale, long long rows, int features, long long ld) {
+  if (rows < 0 || features < 1) return set_error(ctx, GRILLY_ERR_INVALID_ARG, std::string(who) + ": rows must not be negative and features must be positive");
+  if (ld < features || ld % 16 != 0) return set_error(ctx, GRILLY_ERR_INVALID_ARG, std::string(who) + ": the rows' pitch must be a multiple of 16 and at least the features");
+  if (rows > 0 && (!q || !scale)) return set_error(ctx, GRILLY_ERR_INVALID_ARG, std::string(who) + ": null 8-bit rows");
+  if (reinterpret_cast<uintptr_t>(q) & 15) return set_error(ctx, GRILLY_ERR_INVALID_ARG, std::string(who) + ": 8-bit rows must be 16-byte aligned");
+  return GRILLY_OK;
+}
+
+}  // namespace gb

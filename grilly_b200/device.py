@@ -17,10 +17,10 @@ from . import _lib as L
 
 
 class DeviceTensor:
-    """A contiguous array in device memory. dtype is 'f32', 'bf16' or 'i32'."""
+    """A contiguous array in device memory. dtype is 'f32', 'bf16', 'i32' or 'i8'."""
 
     __slots__ = ("dev", "ptr", "shape", "dtype", "_owned", "__weakref__")
-    _ITEMSIZE = {"f32": 4, "bf16": 2, "i32": 4}
+    _ITEMSIZE = {"f32": 4, "bf16": 2, "i32": 4, "i8": 1}
 
     def __init__(self, dev: "Device", ptr: int, shape, dtype: str, owned: bool = True):
         self.dev, self.ptr, self.shape, self.dtype, self._owned = dev, ptr, tuple(int(s) for s in shape), dtype, owned
@@ -124,10 +124,10 @@ class Device:
         return t
 
     def upload(self, arr: np.ndarray, dtype: str = "f32", round_tf32: bool = False) -> DeviceTensor:
-        """Copy a NumPy array to the device as fp32 (optionally rounded to tf32), bf16 or int32."""
-        if dtype == "i32":
-            host = np.ascontiguousarray(arr, dtype=np.int32)
-            t = self.empty(host.shape, "i32")
+        """Copy a NumPy array to the device as fp32 (optionally rounded to tf32), bf16, int32 or int8."""
+        if dtype in ("i32", "i8"):
+            host = np.ascontiguousarray(arr, dtype=np.int32 if dtype == "i32" else np.int8)
+            t = self.empty(host.shape, dtype)
             self.check(self.lib.grilly_upload(self.ctx, t.ptr, host.ctypes.data, host.nbytes))
             self.sync()
             return t
@@ -152,7 +152,7 @@ class Device:
             out = self.download(tf)
             tf.free()
             return out
-        out = np.empty(t.shape, dtype=np.int32 if t.dtype == "i32" else np.float32)
+        out = np.empty(t.shape, dtype={"i32": np.int32, "i8": np.int8}.get(t.dtype, np.float32))
         self.check(self.lib.grilly_download(self.ctx, out.ctypes.data, t.ptr, out.nbytes))
         return out
 

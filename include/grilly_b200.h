@@ -53,6 +53,8 @@ enum {
   GRILLY_FLAG_SWIGLU_PAIRS = 4  /* weight rows interleaved (gate_j, up_j): y[:, j] = gate_j * silu(up_j), N/2 columns out;
                                    with act = GRILLY_ACT_GELU the gate is gate_j * gelu(up_j) (GeGLU) */
 };
+/* further flag of the 8-bit row operators: the floating input tensors are bf16 instead of fp32 */
+enum { GRILLY_FLAG_IN_BF16 = 8 };
 
 /* ---- context, replaces VulkanCore (backend/core.py:14-439) ------------------------------- */
 int grilly_device_count(int* count);
@@ -273,6 +275,53 @@ int grilly_adam_update(grilly_ctx* ctx, float* weights_dev, float* gradients_dev
 /* out[c][r] = in[r][c] on the device: the grad_output^T operand of VulkanFNN.linear_backward's weight gradient
  * (backend/fnn.py:1548-1573 transposes on the host). */
 int grilly_transpose_2d(grilly_ctx* ctx, const float* in_dev, float* out_dev, int rows, int cols);
+
+/* ---- rows in 8 bits: written, multiplied and kept for the backward pass ---------------------------------------
+ * A tensor in 8-bit rows is an int8 matrix q [rows][ld] (ld >= features, a multiple of 16; the base 16-byte aligned;
+ * the buffer holds rows * ld bytes) and one fp32 scale per row; element (r, c) stands for q[r][c] * scale[r].
+ * Written here: scale = max(max|row| / 127, 2^-126), q = x / scale rounded to the nearest integer (ties to even), so
+ * |q| <= 127 and a value is off by at most scale / 2; a zero row is exact. A row that holds a NaN or an infinity gets
+ * scale NaN and q = 0: every value read back from it is NaN. Bytes between features and ld are written as 0 and never
+ * change a result when read. The reference has no 8-bit type (its layers store fp32, backend/fnn.py:1437-1489); these
+ * stand beside its linear, RMSNorm and backward entry points. All are asynchronous on the context's stream, keep no
+ * state between calls and can be captured into a CUDA graph; scratch comes from the pool in stream order. rows = 0 is
+ * allowed (gradients summed over rows are then zero). Sums over rows have a fixed order: results repeat bit for bit. */
+/* x [rows][features] fp32, or bf16 with GRILLY_FLAG_IN_BF16, -> q, scale. A weight matrix (out, in) quantised this way
+ * carries one scale per output channel. */
+int grilly_quantize_rows(grilly_ctx* ctx, const void* x_dev, void* q_dev, float* scale_dev, long long rows, int features,
+                         long long ld, int flags);
+/* q, scale -> y [rows][features] fp32, or bf16 with GRILLY_FLAG_OUT_BF16 (the product, rounded once). */
+int grilly_dequantize_rows(grilly_ctx* ctx, const void* q_dev, const float* scale_dev, void* y_dev, long long rows, int features,
+                           long long ld, int flags);
+/* h = x + residual (residual NULL: h = x); rstd = 1 / sqrt(mean(h^2) + eps); y = h * rstd * gamma (gamma NULL: 1), written
+ * as 8-bit rows y_q, y_scale. snn-rmsnorm.glsl:34-75 after fnn-residual.glsl, with the sums in fp32 and from the unrounded
+ * h. Optional outputs (NULL: not written): h_dev [rows][features] in the inputs' type; h_q with h_scale, h in 8-bit rows
+ * (the checkpoint that grilly_rmsnorm_backward_q8 reads), and rstd_dev [rows]. h_dev may be x_dev or residual_dev (in
+ * place). x, residual and h are fp32, or bf16 with GRILLY_FLAG_IN_BF16. eps > 0. A row whose sum of squares is not a
+ * finite fp32 number counts as a row with an infinity. */
+int grilly_rmsnorm_residual_q8(grilly_ctx* ctx, const void* x_dev, const void* residual_dev, const float* gamma_dev, void* h_dev,
+                               void* y_q_dev, float* y_scale_dev, void* h_q_dev, float* h_scale_dev, float* rstd_dev,
+                               long long rows, int features, long long ld, float eps, int flags);
+/* y[m][n] = act(x_scale[m] * w_scale[n] * sum_k x_q[m][k] * w_q[n][k] + bias[n]), y [M][N] fp32 or bf16
+ * (GRILLY_FLAG_OUT_BF16): fnn-linear.glsl:33-58 and its fused activations on 8-bit rows. The sum is exact (int32):
+ * K <= 131071. bias fp32 or NULL; act in GRILLY_ACT_*. */
+int grilly_linear_q8(grilly_ctx* ctx, const void* x_q_dev, const float* x_scale_dev, const void* w_q_dev, const float* w_scale_dev,
+                     const float* bias_dev, void* y_dev, long long M, int N, int K, long long ld_x, long long ld_w, int act, int flags);
+/* Backward pass of y = x W^T + b (backend/fnn.py:1501-1573) from the 8-bit checkpoint of x [M][K]:
+ *   grad_x [M][K] = grad_out W;  grad_w [N][K] = grad_out^T x;  grad_b [N] = column sums of grad_out.
+ * grad_out [M][N] and W [N][K] are bf16; grad_x and grad_w fp32, or bf16 with GRILLY_FLAG_OUT_BF16; grad_b fp32. A NULL
+ * output is not computed. bf16 products with fp32 sums; x enters them as q * scale rounded to bf16. */
+int grilly_linear_backward_q8(grilly_ctx* ctx, const void* grad_out_dev, const void* x_q_dev, const float* x_scale_dev,
+                              const void* w_dev, void* grad_x_dev, void* grad_w_dev, float* grad_b_dev, long long M, int N, int K,
+                              long long ld_x, int flags);
+/* Backward pass of the norm above from the 8-bit checkpoint of h and its rstd: with n = h * rstd and g = grad_out * gamma,
+ *   grad_h = rstd * (g - n * mean(g * n)) (+ grad_residual, the gradient that reaches h past the norm);
+ *   grad_gamma [features] = sum over rows of grad_out * n.
+ * grad_out, grad_residual (or NULL) and grad_h are fp32, or bf16 with GRILLY_FLAG_IN_BF16; gamma fp32 or NULL (= 1);
+ * grad_gamma fp32, NULL: not computed. grad_h may be grad_out or grad_residual (in place). */
+int grilly_rmsnorm_backward_q8(grilly_ctx* ctx, const void* grad_out_dev, const void* h_q_dev, const float* h_scale_dev,
+                               const float* rstd_dev, const float* gamma_dev, const void* grad_residual_dev, void* grad_h_dev,
+                               float* grad_gamma_dev, long long rows, int features, long long ld, int flags);
 
 /* ---- resident sentence encoder ---------------------------------------------------------------- */
 /* VulkanSentenceTransformer.encode utils/vulkan_sentence_transformer.py:1109-1219; weights live on the device between
