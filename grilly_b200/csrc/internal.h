@@ -93,7 +93,7 @@ enum { PROF_GEMM = 0, PROF_ATTN = 1, PROF_NORM = 2, PROF_EMBED = 3, PROF_POOL = 
 int prof_begin(grilly_ctx* ctx, int cls, double flops, double bytes);
 void prof_end(grilly_ctx* ctx, int idx);
 
-enum { TM_F32 = 0, TM_BF16 = 1 };
+enum { TM_F32 = 0, TM_BF16 = 1, TM_U8 = 2 };
 enum { TM_SW128 = 0, TM_SW128_ATOM32 = 1, TM_SWNONE = 2, TM_SW64 = 3 };  // 128-byte swizzle of 16-byte chunks, or of 32-byte chunks (tf32 MN-major), none, or the 64-byte swizzle
 // 2-D row-major tensor [outer][inner] with a row pitch, 128-byte swizzle, zero fill out of bounds.
 int get_tmap_2d(grilly_ctx* ctx, int dtype, const void* ptr, uint64_t inner, uint64_t outer, uint64_t stride_bytes,
