@@ -216,31 +216,40 @@ int launch_gemm8(grilly_ctx* ctx, Operand oa, Operand ob, long long M, int N, lo
   g.k_blocks = static_cast<int>((k + BK - 1) / BK);
   g.err = ctx->err_dev;
   const int elt = g.out_bf16 ? 2 : 4;
-  g.wide_store = g.ld_out % 4 == 0 && reinterpret_cast<uintptr_t>(g.out) % (4 * elt) == 0;
   // parts along k until every pair has a tile
   const int tiles = g.tiles_m * g.tiles_n;
   const int want = std::max(1, std::min(pairs / tiles, g.k_blocks / 4));
   g.k_per_split = (g.k_blocks + want - 1) / want;
   g.splits = (g.k_blocks + g.k_per_split - 1) / g.k_per_split;
+  if (static_cast<long long>(tiles) * g.splits > 0x3fffffffll) return set_error(ctx, GRILLY_ERR_UNSUPPORTED, "8-bit rows: too many tiles");
+  g.by_tiles = Divisor(tiles);
+  g.by_group_tiles = Divisor(g.tile_group * g.tiles_n);
+  g.by_group = Divisor(g.tile_group);
+  g.by_last_group = Divisor(std::max(1, g.tiles_m % g.tile_group));
   const double bytes = (kInt8 ? 1.0 : 2.0) * (static_cast<double>(M) * k + static_cast<double>(N) * k) + static_cast<double>(M) * N * elt;
   const int pi = prof_begin(ctx, PROF_GEMM, 2.0 * M * static_cast<double>(N) * k, bytes);
   cfg.gridDim = dim3(2 * std::min(pairs, tiles * g.splits), 1, 1);
+  CUtensorMap to = ta;
+  g.wide_store = g.ld_out * elt % 16 == 0 && reinterpret_cast<uintptr_t>(g.out) % 16 == 0;
   if (g.splits == 1) {
-    GB_CUDA_CHECK(ctx, cudaLaunchKernelEx(&cfg, kern, ta, tb, g));
+    // 64 bytes of 32 rows per store, cut off at the edges
+    if (g.wide_store && (rc = get_tmap_2d(ctx, g.out_bf16 ? TM_BF16 : TM_F32, g.out, N, M, g.ld_out * elt, 64 / elt, 32, &to, TM_SW64))) return rc;
+    GB_CUDA_CHECK(ctx, cudaLaunchKernelEx(&cfg, kern, ta, tb, to, g));
     ctx->launches++;
   } else {
+    // planes of whole tiles, so that a store at the lower edge of one does not reach into the next
     Rows8Scratch ws(ctx);
-    const long long ld_ws = (N + 3) / 4 * 4ll;
-    if ((rc = ws.take(static_cast<size_t>(g.splits) * M * ld_ws * 4))) return rc;
+    const long long ld_ws = (N + 3) / 4 * 4ll, plane_rows = tiles_m * Cfg::TILE;
+    if ((rc = ws.take(static_cast<size_t>(g.splits) * plane_rows * ld_ws * 4))) return rc;
     Gemm8Args part = g;
     part.out = ws.p;
     part.ld_out = ld_ws;
-    part.raw = 1;
-    part.wide_store = 1;
-    GB_CUDA_CHECK(ctx, cudaLaunchKernelEx(&cfg, kern, ta, tb, part));
+    part.raw = part.wide_store = 1;
+    if ((rc = get_tmap_2d(ctx, TM_F32, ws.p, N, g.splits * plane_rows, ld_ws * 4, 16, 32, &to, TM_SW64))) return rc;
+    GB_CUDA_CHECK(ctx, cudaLaunchKernelEx(&cfg, kern, ta, tb, to, part));
     const long long pieces = M * ((N + 3) / 4);
     gemm8_join_kernel<KIND><<<static_cast<unsigned>(std::min<long long>((pieces + 255) / 256, ctx->num_sms * 8ll)), 256, 0, ctx->stream>>>(
-        g, static_cast<const uint32_t*>(ws.p), ld_ws);
+        g, static_cast<const uint32_t*>(ws.p), ld_ws, plane_rows * ld_ws);
     ctx->launches += 2;
     GB_CUDA_CHECK(ctx, cudaGetLastError());
   }

@@ -7,29 +7,44 @@
 // A pair of CTAs shares one tcgen05.mma (cta_group::2): a 256 x 256 tile of C, of which each CTA loads 128 rows of A and
 // 128 of B per k-block of 128 bytes and keeps 128 rows of the accumulator in its own tensor memory, twice, so that one
 // tile is written while the next is computed. Roles per CTA: warp 0 TMA producer (own halves, bytes counted on the
-// leader's barrier), warp 1 MMA issuer (leader) and TMEM allocation, the rest epilogue. Every wait is bounded and reports
-// through the device status word. Nothing is broadcast by TMA.
+// leader's barrier), warp 1 MMA issuer (leader) and TMEM allocation, 16 epilogue warps, and for Q8 one warp that brings
+// the next tile's column scales and bias into shared memory (left to the epilogue warps, each tile waited twice for L2).
+// Every wait is bounded and reports through the device status word. Nothing is broadcast by TMA.
 //
 // Few tiles of a long product are split along k: every part stores its raw 32-bit sums to its own plane of a workspace and
 // a second kernel adds the planes in order (no atomics: results repeat bit for bit).
 #pragma once
 #include "ptx.cuh"
+#include "../../include/grilly_b200.h"
 #include <cuda_bf16.h>
 
 namespace gb {
 
 enum class Gemm8Kind { Q8, DGRAD, WGRAD };
 
+// Division of 0 <= n < 2^31 by a number the host knows: n * m >> s with s = 31 + ceil(log2 d), m = floor(2^s / d) + 1. The
+// error of m is at most 2^-31 of a quotient step for every such n, so the quotient is exact (Granlund and Montgomery).
+struct Divisor {
+  uint32_t d, m, s;
+  Divisor() = default;
+  __host__ explicit Divisor(uint32_t n) : d(n), s(31) {
+    while ((1ull << (s - 31)) < n) ++s;
+    m = static_cast<uint32_t>((1ull << s) / n + 1);
+  }
+  __device__ __forceinline__ int quotient(int n) const { return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * m) >> s); }
+};
+
 struct Gemm8Args {
   long long M;
   int N;
   int tiles_m, tiles_n, tile_group, k_blocks;
   int splits, k_per_split;    // k-blocks per part
+  Divisor by_tiles, by_group_tiles, by_group, by_last_group;   // tiles, group * tiles_n, group, tiles_m % group (or 1)
   // epilogue
   void* out;                  // C [M][N] fp32 or bf16, or the workspace [splits][M][ld_out] of raw sums
   long long ld_out;
   int out_bf16, raw;
-  int wide_store;             // rows of C start on 4-element boundaries
+  int wide_store;             // rows of C lie on 16-byte boundaries: TMA stores them
   const float* row_scale;     // Q8: per row and per column, and the bias
   const float* col_scale;
   const float* bias;
@@ -37,111 +52,153 @@ struct Gemm8Args {
   int* err;
 };
 
-constexpr int GEMM8_EPI_WARPS = 8;
-constexpr int GEMM8_THREADS = 64 + 32 * GEMM8_EPI_WARPS;
+constexpr int GEMM8_EPI_WARPS = 16;
+constexpr int GEMM8_PARAM_WARP = 2 + GEMM8_EPI_WARPS;
+constexpr int GEMM8_THREADS = 32 * (GEMM8_PARAM_WARP + 1);
 
 struct Gemm8Cfg {
   static constexpr int TILE = 256;
   static constexpr int HALF_BYTES = 128 * 128;               // 128 rows (or columns) x 128 bytes
   static constexpr int STAGE_BYTES = 2 * HALF_BYTES;
-  static constexpr int STAGES = 6;
-  static constexpr int EPI_BYTES = 32 * 128;                 // per epilogue warp: 32 rows x 32 columns of 32 bits
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + GEMM8_EPI_WARPS * EPI_BYTES + 1024 /*align slack*/ + 256 /*barriers*/;
+  static constexpr int STAGES = 5;
+  static constexpr int EPI_BYTES = 32 * 64;                  // per epilogue warp: 32 rows x 64 bytes of C on their way out
+  static constexpr int PARAM_FLOATS = 2 * TILE;              // column scales and bias of a tile, double-buffered
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + GEMM8_EPI_WARPS * EPI_BYTES + 2 * PARAM_FLOATS * 4 + 1024 /*align slack*/ + 256 /*barriers*/;
   static constexpr int TMEM_COLS = 512;
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of one CTA");
 };
 
-// ---- epilogue arithmetic
+// ---- epilogue arithmetic: two neighbouring columns at a time (one instruction for two fp32 products or sums)
+struct F2 {
+  uint64_t v;
+  __device__ __forceinline__ F2() {}
+  __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { F2 d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return d; }
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) { F2 d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v)); return d; }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) { F2 d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v)); return d; }
+__device__ __forceinline__ float fast_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// v * sigmoid(z) with z = v for SiLU and z = 2 sqrt(2/pi) (v + 0.044715 v^3) for GELU (its tanh form: 0.5 v (1 + tanh(z / 2))).
+// One exponential and one reciprocal, each within 2 ulp, keep the relative accuracy far below zero too, where 1 + tanh
+// would cancel. Where 2^(-z log2 e) overflows, the reciprocal is 0 and so is the result.
+template <int ACT>
+__device__ __forceinline__ F2 gemm8_act2(F2 v) {
+  constexpr float L2E = 1.4426950408889634f, S = 2.f * 0.7978845608028654f;
+  if constexpr (ACT == GRILLY_ACT_RELU) {
+    float a, b;
+    v.get(a, b);
+    return F2(a < 0.f ? 0.f : a, b < 0.f ? 0.f : b);
+  } else if constexpr (ACT == GRILLY_ACT_GELU || ACT == GRILLY_ACT_SILU) {
+    F2 z;
+    if constexpr (ACT == GRILLY_ACT_GELU) z = mul2(v, fma2(mul2(v, v), F2(-S * L2E * 0.044715f, -S * L2E * 0.044715f), F2(-S * L2E, -S * L2E)));
+    else z = mul2(v, F2(-L2E, -L2E));
+    float a, b;
+    z.get(a, b);
+    add2(F2(fast_exp2(a), fast_exp2(b)), F2(1.f, 1.f)).get(a, b);
+    return mul2(v, F2(fast_rcp(a), fast_rcp(b)));
+  } else {
+    return v;
+  }
+}
 __device__ __forceinline__ float gemm8_act(float v, int act) {
-  // GELU (tanh form) as v * sigmoid(2 u): one exponential and one division, accurate for v far below zero too
+  float a, b;
   switch (act) {
-    case 1: return __fdividef(v, 1.f + __expf(-2.f * 0.7978845608028654f * v * fmaf(0.044715f, v * v, 1.f)));
-    case 2: return __fdividef(v, 1.f + __expf(-v));
-    case 3: return v < 0.f ? 0.f : v;
+    case GRILLY_ACT_GELU: gemm8_act2<GRILLY_ACT_GELU>(F2(v, v)).get(a, b); return a;
+    case GRILLY_ACT_SILU: gemm8_act2<GRILLY_ACT_SILU>(F2(v, v)).get(a, b); return a;
+    case GRILLY_ACT_RELU: return v < 0.f ? 0.f : v;
     default: return v;
   }
 }
 
-// Tile of the persistent loop: `fast` blocks are walked in groups so that the tiles of one moment share rows of A and B.
-static __device__ __noinline__ uint64_t gemm8_tile(int tile, int num_fast, int num_slow, int group) {
-  const int per_group = group * num_slow;
-  const int g = tile / per_group, first = g * group;
-  const int size = min(num_fast - first, group), r = tile - g * per_group, slow = r / size;
-  return static_cast<uint64_t>(static_cast<uint32_t>(first + r - slow * size)) | (static_cast<uint64_t>(static_cast<uint32_t>(slow)) << 32);
+// Tile of the persistent loop: row blocks are walked in groups so that the tiles of one moment share rows of A and B.
+__device__ __forceinline__ void gemm8_tile(const Gemm8Args& a, int tile, int& m, int& n) {
+  const int g = a.by_group_tiles.quotient(tile), first = g * a.tile_group;
+  const int r = tile - g * static_cast<int>(a.by_group_tiles.d);
+  const bool whole = first + a.tile_group <= a.tiles_m;
+  n = whole ? a.by_group.quotient(r) : a.by_last_group.quotient(r);
+  m = first + r - n * static_cast<int>(whole ? a.by_group.d : a.by_last_group.d);
 }
 
-// Writes 32 rows x 32 columns. They lie in shared memory as raw 32-bit sums, row r at 128 r with its 16-byte pieces
-// exchanged by r % 8 (no bank conflicts on either side). W columns per lane: 4 where rows of C are aligned for it, else 1;
-// either way the lanes of one store cover whole pieces of rows.
-template <Gemm8Kind KIND, int W>
-__device__ __forceinline__ void gemm8_store_block(const Gemm8Args& a, const uint8_t* stage, long long row0, int col0, int lane, uint8_t* out_base) {
-  constexpr int PER_ROW = 32 / W;            // lanes per row
-  constexpr int ROWS = 32 / PER_ROW;         // rows per store
-  const int piece = (lane % PER_ROW) * W;    // first column of the lane
-  const int col = col0 + piece;
-  if (col >= a.N) return;
-  float cs[W], bias[W];
+// One warp writes 32 rows x 32 columns of C. r: the lane's row, 32 neighbouring columns, as raw sums (int32 for Q8).
+// Q8: times the row's scale, times the column's scale plus bias (shared memory, the same address in every lane), activation.
+// The values go to the warp's 2 KB of shared memory as rows of 64 bytes (32 columns of bf16, or 16 of fp32 twice) whose
+// 16-byte pieces are exchanged as TMA's 64-byte swizzle does, so neither side has bank conflicts, and one TMA store takes
+// them out, cut off at the edges of C. Where C's rows are not on 16-byte boundaries the lanes store them themselves.
+template <Gemm8Kind KIND, int ACT>
+__device__ __forceinline__ void gemm8_finish(uint32_t (&r)[32], float rs, const float* cs, const float* bias) {
   if constexpr (KIND == Gemm8Kind::Q8) {
-    if (!a.raw) {
+    const F2 rs2(rs, rs);
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        const bool in = col + j < a.N;
-        cs[j] = in ? __ldg(a.col_scale + col + j) : 0.f;
-        bias[j] = (in && a.bias) ? __ldg(a.bias + col + j) : 0.f;
+    for (int j = 0; j < 32; j += 4) {
+      const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(cs + j), d = *reinterpret_cast<const ulonglong2*>(bias + j);
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        F2 c2, d2;
+        c2.v = i ? c.y : c.x;
+        d2.v = i ? d.y : d.x;
+        const F2 v(static_cast<float>(static_cast<int>(r[j + i])), static_cast<float>(static_cast<int>(r[j + i + 1])));
+        float a, b;
+        gemm8_act2<ACT>(fma2(mul2(v, rs2), c2, d2)).get(a, b);
+        r[j + i] = __float_as_uint(a);
+        r[j + i + 1] = __float_as_uint(b);
       }
     }
   }
+}
+// 16 words of a lane's row into the warp's staging rows
+__device__ __forceinline__ void gemm8_stage(uint8_t* stage, int lane, const uint32_t (&w)[16]) {
+#pragma unroll
+  for (int p = 0; p < 4; ++p)
+    *reinterpret_cast<uint4*>(stage + lane * 64 + ((p ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]);
+}
+__device__ __forceinline__ void gemm8_write(const Gemm8Args& a, const CUtensorMap* tmap_out, const uint32_t (&r)[32], uint8_t* stage, long long row0,
+                                            int out_row, int col0, int lane) {
+  const bool half = a.out_bf16 && !a.raw;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (h == 1 && half && a.wide_store) break;               // 32 columns of bf16 went out at once
+    const int first = col0 + 16 * h;
+    if (first >= a.N) break;
+    uint32_t w[16];
+    if (half && a.wide_store) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+        w[j] = *reinterpret_cast<const uint32_t*>(&t);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) w[j] = r[16 * h + j];
+    }
+    if (a.wide_store) {
+      if (lane == 0) tma_store_wait_read<0>();               // the warp's last store has left the staging rows
+      __syncwarp();
+      gemm8_stage(stage, lane, w);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_2d(tmap_out, stage, first, out_row);
+        tma_store_commit();
+      }
+    } else {
+      __syncwarp();
+      gemm8_stage(stage, lane, w);
+      __syncwarp();
+      const int c = lane & 15, rows = static_cast<int>(a.M - row0 < 32 ? a.M - row0 : 32);
+      if (first + c < a.N) {
 #pragma unroll 8
-  for (int i = 0; i < 32 / ROWS; ++i) {
-    const int r = i * ROWS + lane / PER_ROW;
-    const long long row = row0 + r;
-    if (row >= a.M) break;
-    uint32_t w[W];
-    const uint8_t* src = stage + r * 128 + (((piece >> 2) ^ (r & 7)) << 4) + (piece & 3) * 4;
-    if constexpr (W == 4) {
-      const uint4 t = *reinterpret_cast<const uint4*>(src);
-      w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w;
-    } else {
-      w[0] = *reinterpret_cast<const uint32_t*>(src);
-    }
-    const long long at = row * a.ld_out + col;
-    if (a.raw) {                             // the workspace's rows are multiples of 4 long
-      if constexpr (W == 4) *reinterpret_cast<uint4*>(out_base + at * 4) = make_uint4(w[0], w[1], w[2], w[3]);
-      else *reinterpret_cast<uint32_t*>(out_base + at * 4) = w[0];
-      continue;
-    }
-    float v[W];
-    if constexpr (KIND == Gemm8Kind::Q8) {
-      const float rs = __ldg(a.row_scale + row);
-#pragma unroll
-      for (int j = 0; j < W; ++j) v[j] = gemm8_act(fmaf(static_cast<float>(static_cast<int>(w[j])) * rs, cs[j], bias[j]), a.act);
-    } else {
-#pragma unroll
-      for (int j = 0; j < W; ++j) v[j] = __uint_as_float(w[j]);
-    }
-    if (a.out_bf16) {
-      __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(out_base) + at;
-      if constexpr (W == 4) {
-        if (col + 4 <= a.N) {
-          const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
-          *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-          continue;
+        for (int q = lane >> 4; q < rows; q += 2) {
+          const float v = *reinterpret_cast<const float*>(stage + q * 64 + (((c >> 2) ^ ((q >> 1) & 3)) << 4) + (c & 3) * 4);
+          const long long at = (row0 + q) * a.ld_out + first + c;
+          if (half) static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16(v);
+          else static_cast<float*>(a.out)[at] = v;
         }
       }
-#pragma unroll
-      for (int j = 0; j < W; ++j)
-        if (col + j < a.N) p[j] = __float2bfloat16(v[j]);
-    } else {
-      float* p = reinterpret_cast<float*>(out_base) + at;
-      if constexpr (W == 4) {
-        if (col + 4 <= a.N) {
-          *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-          continue;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < W; ++j)
-        if (col + j < a.N) p[j] = v[j];
     }
   }
 }
@@ -165,7 +222,8 @@ __host__ __device__ constexpr uint32_t make_idesc_i8(int m, int n) {
 
 template <Gemm8Kind KIND>
 __global__ void __launch_bounds__(GEMM8_THREADS, 1)
-gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const Gemm8Args args) {
+gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                  const __grid_constant__ CUtensorMap tmap_out, const Gemm8Args args) {
   using Cfg = Gemm8Cfg;
   constexpr int STAGES = Cfg::STAGES;
   constexpr bool kInt8 = KIND == Gemm8Kind::Q8, kAMn = KIND == Gemm8Kind::WGRAD, kBMn = KIND != Gemm8Kind::Q8;
@@ -177,11 +235,14 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* epi = smem + STAGES * Cfg::STAGE_BYTES;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(epi + GEMM8_EPI_WARPS * Cfg::EPI_BYTES);
+  float* params = reinterpret_cast<float*>(epi + GEMM8_EPI_WARPS * Cfg::EPI_BYTES);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(params + 2 * Cfg::PARAM_FLOATS);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* tmem_full = empty_bar + STAGES;
   uint64_t* tmem_empty = tmem_full + 2;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tmem_empty + 2);
+  uint64_t* param_full = tmem_empty + 2;
+  uint64_t* param_empty = param_full + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(param_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -198,11 +259,14 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tmem_full[i], 1);
       mbar_init(&tmem_empty[i], 2 * GEMM8_EPI_WARPS);          // used in the leader only
+      mbar_init(&param_full[i], 1);
+      mbar_init(&param_empty[i], GEMM8_EPI_WARPS);
     }
     *abort_flag = 0;
     fence_mbar_init();
     prefetch_tmap(&tmap_a);
     prefetch_tmap(&tmap_b);
+    if (args.wide_store) prefetch_tmap(&tmap_out);
   }
   if (warp == 1) {
     tmem_alloc_pair(tmem_holder, Cfg::TMEM_COLS);
@@ -221,7 +285,7 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     st_cluster_u32(map_to_cta(const_cast<int*>(abort_flag), rank ^ 1u), 1u);
   };
   auto k_range = [&](int item, int& k0, int& k1) {
-    const int part = item / tiles;
+    const int part = args.by_tiles.quotient(item);
     k0 = part * args.k_per_split;
     k1 = min(args.k_blocks, k0 + args.k_per_split);
     return item - part * tiles;
@@ -235,9 +299,10 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
       bool ok = true;
       for (int item = pair; item < items && ok; item += num_pairs) {
         int k0, k1;
-        const uint64_t t = gemm8_tile(k_range(item, k0, k1), args.tiles_m, args.tiles_n, args.tile_group);
-        const int a_row = static_cast<int>(static_cast<uint32_t>(t)) * Cfg::TILE + static_cast<int>(rank) * 128;
-        const int b_row = static_cast<int>(t >> 32) * Cfg::TILE + static_cast<int>(rank) * 128;
+        int tm, tn;
+        gemm8_tile(args, k_range(item, k0, k1), tm, tn);
+        const int a_row = tm * Cfg::TILE + static_cast<int>(rank) * 128;
+        const int b_row = tn * Cfg::TILE + static_cast<int>(rank) * 128;
         for (int kb = k0; kb < k1; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) { fail(ERR_WAIT_EMPTY); ok = false; break; }
           uint8_t* sa = smem + stage * Cfg::STAGE_BYTES;
@@ -303,43 +368,96 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         }
       }
     }
+  } else if (warp == GEMM8_PARAM_WARP) {
+    // ------------------------------------------------------------ column scales and bias of the tiles, one tile ahead
+    if constexpr (KIND == Gemm8Kind::Q8) {
+      if (!args.raw) {
+        int it = 0;
+        for (int item = pair; item < items; item += num_pairs, ++it) {
+          const int buf = it & 1;
+          int tm, tn;
+          gemm8_tile(args, item, tm, tn);
+          float c[Cfg::TILE / 32], d[Cfg::TILE / 32];
+#pragma unroll
+          for (int j = 0; j < Cfg::TILE / 32; ++j) {
+            const int col = tn * Cfg::TILE + j * 32 + lane;
+            c[j] = col < args.N ? __ldg(args.col_scale + col) : 0.f;
+            d[j] = (col < args.N && args.bias) ? __ldg(args.bias + col) : 0.f;
+          }
+          if (!mbar_wait(&param_empty[buf], ((it >> 1) & 1u) ^ 1u, abort_flag)) { fail(ERR_WAIT_EMPTY); break; }
+          float* p = params + buf * Cfg::PARAM_FLOATS;
+#pragma unroll
+          for (int j = 0; j < Cfg::TILE / 32; ++j) {
+            p[j * 32 + lane] = c[j];
+            p[Cfg::TILE + j * 32 + lane] = d[j];
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&param_full[buf]);
+        }
+      }
+    }
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs, own 128 rows of the tile)
-    constexpr int NCHUNK = Cfg::TILE / 32, G = GEMM8_EPI_WARPS / 4;
+    constexpr int NCHUNK = Cfg::TILE / 32, G = GEMM8_EPI_WARPS / 4, PER_WARP = NCHUNK / G;
     const int quad = warp & 3, group = (warp - 2) >> 2;
     uint8_t* stage = epi + (warp - 2) * Cfg::EPI_BYTES;
     const uint32_t leader_tempty0 = map_to_cta(&tmem_empty[0], 0);
+    const bool scaled = KIND == Gemm8Kind::Q8 && !args.raw;
+    // the rows' scales are read one tile ahead
+    auto row_of = [&](int tm) { return static_cast<long long>(tm) * Cfg::TILE + static_cast<int>(rank) * 128 + quad * 32; };
+    auto row_scale = [&](int item) {
+      int tm, tn;
+      if (!scaled || item >= items) return 0.f;
+      gemm8_tile(args, item, tm, tn);
+      const long long row = row_of(tm) + lane;
+      return row < args.M ? __ldg(args.row_scale + row) : 0.f;
+    };
+    float rs = row_scale(pair);
     int it = 0;
     for (int item = pair; item < items; item += num_pairs, ++it) {
-      int k0, k1;
-      const int tile = k_range(item, k0, k1);
-      const uint64_t t = gemm8_tile(tile, args.tiles_m, args.tiles_n, args.tile_group);
-      const long long row0 = static_cast<long long>(static_cast<uint32_t>(t)) * Cfg::TILE + static_cast<int>(rank) * 128 + quad * 32;
-      const int first_col = static_cast<int>(t >> 32) * Cfg::TILE;
-      uint8_t* out = static_cast<uint8_t*>(args.out);
-      if (args.raw) out += static_cast<long long>(item / tiles) * args.M * args.ld_out * 4;
+      const int part = args.by_tiles.quotient(item);
+      int tm, tn;
+      gemm8_tile(args, item - part * tiles, tm, tn);
+      const long long row0 = row_of(tm);
+      const int first_col = tn * Cfg::TILE;
+      const int out_row = static_cast<int>(row0) + (args.raw ? part * args.tiles_m * Cfg::TILE : 0);
+      const int chunks = row0 >= args.M ? 0 : min(NCHUNK, (args.N - first_col + 31) / 32);   // warp-uniform
+      const float rs_next = row_scale(item + num_pairs);
       const int acc = it & 1;
+      const float* p = params + acc * Cfg::PARAM_FLOATS;
+      if (scaled && !mbar_wait(&param_full[acc], (it >> 1) & 1u, abort_flag)) { fail(ERR_WAIT_FULL); break; }
       if (!mbar_wait(&tmem_full[acc], (it >> 1) & 1u, abort_flag)) { fail(ERR_WAIT_TMEM_FULL); break; }
       tc_fence_after();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * Cfg::TILE;
-      for (int c = group; c < NCHUNK; c += G) {
-        const int col0 = first_col + c * 32;
-        if (col0 >= args.N || row0 >= args.M) break;           // warp-uniform
-        uint32_t r[32];
-        __syncwarp();
-        tmem_ld_32x32(taddr + c * 32, r);
-        tmem_ld_wait();
 #pragma unroll
-        for (int p = 0; p < 8; ++p)
-          *reinterpret_cast<uint4*>(stage + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_uint4(r[4 * p], r[4 * p + 1], r[4 * p + 2], r[4 * p + 3]);
+      for (int i = 0; i < PER_WARP; ++i) {
+        const int c = group + i * G;
         __syncwarp();
-        if (args.wide_store) gemm8_store_block<KIND, 4>(args, stage, row0, col0, lane, out);
-        else gemm8_store_block<KIND, 1>(args, stage, row0, col0, lane, out);
+        if (c < chunks) {
+          uint32_t r[32];
+          tmem_ld_32x32(taddr + c * 32, r);
+          tmem_ld_wait();
+          if (scaled) {
+            const float* cs = p + c * 32;
+            switch (args.act) {
+              case GRILLY_ACT_GELU: gemm8_finish<KIND, GRILLY_ACT_GELU>(r, rs, cs, cs + Cfg::TILE); break;
+              case GRILLY_ACT_SILU: gemm8_finish<KIND, GRILLY_ACT_SILU>(r, rs, cs, cs + Cfg::TILE); break;
+              case GRILLY_ACT_RELU: gemm8_finish<KIND, GRILLY_ACT_RELU>(r, rs, cs, cs + Cfg::TILE); break;
+              default: gemm8_finish<KIND, GRILLY_ACT_NONE>(r, rs, cs, cs + Cfg::TILE);
+            }
+          }
+          gemm8_write(args, &tmap_out, r, stage, row0, out_row, first_col + c * 32, lane);
+        }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(leader_tempty0 + acc * 8);
+      if (lane == 0) {
+        mbar_arrive_cluster(leader_tempty0 + acc * 8);
+        if (scaled) mbar_arrive(&param_empty[acc]);
+      }
+      rs = rs_next;
     }
+    if (lane == 0) tma_store_wait_all<0>();
   }
 
   // ---------------------------------------------------------------- teardown
@@ -355,9 +473,9 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
 
 // Adds the parts of a product split along k, in order, and applies the epilogue. Four columns per thread.
 template <Gemm8Kind KIND>
-__global__ void __launch_bounds__(256) gemm8_join_kernel(const Gemm8Args a, const uint32_t* __restrict__ ws, long long ld_ws) {
+__global__ void __launch_bounds__(256) gemm8_join_kernel(const Gemm8Args a, const uint32_t* __restrict__ ws, long long ld_ws, long long plane) {
   const int per_row = (a.N + 3) / 4;
-  const long long total = a.M * per_row, plane = a.M * ld_ws;
+  const long long total = a.M * per_row;
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
     const long long row = i / per_row;
     const int col = static_cast<int>(i - row * per_row) * 4;

@@ -9,6 +9,7 @@ on every call).
 from __future__ import annotations
 
 import ctypes as C
+import math
 import weakref
 
 import numpy as np
@@ -23,14 +24,16 @@ class DeviceTensor:
     _ITEMSIZE = {"f32": 4, "bf16": 2, "i32": 4, "i8": 1}
 
     def __init__(self, dev: "Device", ptr: int, shape, dtype: str, owned: bool = True):
-        self.dev, self.ptr, self.shape, self.dtype, self._owned = dev, ptr, tuple(int(s) for s in shape), dtype, owned
+        # a view is made for every operand of a call: this and __del__ are kept short
+        self.dev = dev
+        self.ptr = ptr
+        self.shape = tuple(map(int, shape))
+        self.dtype = dtype
+        self._owned = owned
 
     @property
     def size(self) -> int:
-        n = 1
-        for s in self.shape:
-            n *= s
-        return n
+        return math.prod(self.shape)
 
     @property
     def nbytes(self) -> int:
@@ -63,7 +66,8 @@ class DeviceTensor:
 
     def __del__(self):
         try:
-            self.free()
+            if self._owned is True:
+                self.free()
         except Exception:
             pass
 

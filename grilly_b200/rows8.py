@@ -8,6 +8,7 @@ backward methods (backend/fnn.py:1394-1573, snn-rmsnorm.glsl:34-75).
 """
 from __future__ import annotations
 
+import math
 from collections import namedtuple
 
 import numpy as np
@@ -23,57 +24,48 @@ NormQ8.__doc__ = """What ``rmsnorm_residual_q8`` gives: the norm's output in 8-b
 ``keep``, that sum in 8-bit rows and 1 / root-mean-square of every row (else None) for ``rmsnorm_backward_q8``."""
 
 
+def _check_shape(shape):
+    if len(shape) < 1 or shape[-1] < 1 or min(shape) < 0:
+        raise ValueError(f"8-bit rows need a shape (..., features) with at least one feature, not {shape}")
+
+
 class Rows8:
     """A tensor of ``shape`` (..., features) in 8-bit rows on the device: element (r, c) stands for ``q[r, c] * scale[r]``.
 
     ``q`` is an 'i8' :class:`DeviceTensor` (rows, ld) with ld a multiple of 16 of at least ``features`` (what lies between
     is never used), ``scale`` an 'f32' one with one entry per row. A row whose scale is NaN stands for NaN."""
 
-    __slots__ = ("q", "scale", "shape")
+    __slots__ = ("q", "scale", "shape", "dev", "rows", "features", "ld")
 
     def __init__(self, q: DeviceTensor, scale: DeviceTensor, shape):
-        shape = tuple(int(s) for s in shape)
-        if len(shape) < 1 or shape[-1] < 1 or min(shape) < 0:
-            raise ValueError(f"8-bit rows need a shape (..., features) with at least one feature, not {shape}")
-        rows = 1
-        for s in shape[:-1]:
-            rows *= s
+        shape = tuple(map(int, shape))
+        _check_shape(shape)
+        rows = math.prod(shape[:-1])
+        features = shape[-1]
         if q.dtype != "i8" or len(q.shape) != 2 or scale.dtype != "f32":
             raise ValueError("q must be an 'i8' tensor (rows, ld), scale an 'f32' tensor")
-        if q.shape[0] != rows or scale.size != rows:
-            raise ValueError(f"q has {q.shape[0]} rows and scale {scale.size} entries, shape {shape} needs {rows}")
-        if q.shape[1] % 16 or q.shape[1] < shape[-1]:
-            raise ValueError(f"q's row length {q.shape[1]} must be a multiple of 16 and at least {shape[-1]}")
+        held, ld = q.shape
+        if held != rows or (scale.shape != (rows,) and scale.size != rows):
+            raise ValueError(f"q has {held} rows and scale {scale.size} entries, shape {shape} needs {rows}")
+        if ld % 16 or ld < features:
+            raise ValueError(f"q's row length {ld} must be a multiple of 16 and at least {features}")
         if q.dev is not scale.dev:
             raise ValueError("q and scale belong to different contexts")
-        self.q, self.scale, self.shape = q, scale, shape
+        self.q = q
+        self.scale = scale
+        self.shape = shape
+        self.dev = q.dev
+        self.rows = rows
+        self.features = features
+        self.ld = ld
 
     @classmethod
     def empty(cls, dev, shape) -> "Rows8":
         """Uninitialised 8-bit rows in the pool of ``dev``, to be written by an operator."""
-        shape = tuple(int(s) for s in shape)
-        if len(shape) < 1 or shape[-1] < 1 or min(shape) < 0:
-            raise ValueError(f"8-bit rows need a shape (..., features) with at least one feature, not {shape}")
-        rows = 1
-        for s in shape[:-1]:
-            rows *= s
+        shape = tuple(map(int, shape))
+        _check_shape(shape)
+        rows = math.prod(shape[:-1])
         return cls(dev.empty((rows, (shape[-1] + 15) // 16 * 16), "i8"), dev.empty((rows,)), shape)
-
-    @property
-    def dev(self):
-        return self.q.dev
-
-    @property
-    def rows(self) -> int:
-        return self.q.shape[0]
-
-    @property
-    def features(self) -> int:
-        return self.shape[-1]
-
-    @property
-    def ld(self) -> int:
-        return self.q.shape[1]
 
     @property
     def nbytes(self) -> int:
@@ -100,18 +92,15 @@ class Rows8Ops:
     DeviceTensors of this backend's context; with a NumPy operand the floating results are NumPy arrays. ``out`` takes
     the result's tensors, so that a call allocates nothing; a call that is captured into a CUDA graph needs it."""
 
-    # ---- operands ---------------------------------------------------------------------------
-    def _mine(self, t, name):
-        if t.dev is not self.dev:
-            raise ValueError(f"{name} belongs to another context")
-        return t
-
+    # ---- operands (checked in every call: kept short) -----------------------------------------
     def _float_in(self, x, name, host_dtype="f32"):
         """-> (DeviceTensor, came from the host)."""
         if isinstance(x, DeviceTensor):
             if x.dtype not in _FLOAT:
                 raise ValueError(f"{name} must be f32 or bf16, not {x.dtype}")
-            return self._mine(x, name), False
+            if x.dev is not self.dev:
+                raise ValueError(f"{name} belongs to another context")
+            return x, False
         return self.dev.upload(np.asarray(x, dtype=np.float32), host_dtype), True
 
     def _f32_vector(self, v, n, name):
@@ -121,44 +110,47 @@ class Rows8Ops:
         if isinstance(v, DeviceTensor):
             if v.dtype != "f32":
                 raise ValueError(f"{name} must be f32, not {v.dtype}")
-            self._mine(v, name)
-            size = v.size
-        else:
-            v = np.asarray(v, dtype=np.float32)
-            size = v.size
-        if size != n:
-            raise ValueError(f"{name} has {size} entries, expected {n}")
-        return v if isinstance(v, DeviceTensor) else self.dev.upload(v.reshape(-1))
+            if v.dev is not self.dev:
+                raise ValueError(f"{name} belongs to another context")
+            if v.shape != (n,) and v.size != n:
+                raise ValueError(f"{name} has {v.size} entries, expected {n}")
+            return v
+        v = np.asarray(v, dtype=np.float32)
+        if v.size != n:
+            raise ValueError(f"{name} has {v.size} entries, expected {n}")
+        return self.dev.upload(v.reshape(-1))
 
     def _rows8_in(self, x, name):
         if not isinstance(x, Rows8):
             raise TypeError(f"{name} must be 8-bit rows (Rows8), see quantize_rows")
-        self._mine(x, name)
+        if x.dev is not self.dev:
+            raise ValueError(f"{name} belongs to another context")
         return x
 
     def _rows8_out(self, out, shape, name="out"):
         if out is None:
             return Rows8.empty(self.dev, shape)
-        self._rows8_in(out, name)
-        if out.shape != tuple(shape):
-            raise ValueError(f"{name} has shape {out.shape}, expected {tuple(shape)}")
+        if not isinstance(out, Rows8) or out.dev is not self.dev or out.shape != shape:
+            self._rows8_in(out, name)
+            raise ValueError(f"{name} has shape {out.shape}, expected {shape}")
         return out
 
     def _float_out(self, out, shape, dtype, name="out"):
-        """``dtype``: the type of a new tensor, or the types allowed where the caller brings one."""
+        """``dtype``: the type of a new tensor, or of one that the caller brings (a tuple: the types it may have)."""
         if out is None:
-            return self.dev.empty(shape, dtype if isinstance(dtype, str) else dtype[0])
-        if not isinstance(out, DeviceTensor) or out.dtype not in ((dtype,) if isinstance(dtype, str) else dtype):
+            return self.dev.empty(shape, dtype)
+        if not isinstance(out, DeviceTensor) or out.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
             raise ValueError(f"{name} must be a DeviceTensor of type {dtype}")
-        self._mine(out, name)
-        if tuple(out.shape) != tuple(shape):
-            raise ValueError(f"{name} has shape {out.shape}, expected {tuple(shape)}")
+        if out.dev is not self.dev:
+            raise ValueError(f"{name} belongs to another context")
+        if out.shape != shape:
+            raise ValueError(f"{name} has shape {out.shape}, expected {shape}")
         return out
 
     @staticmethod
     def _shape(x, name):
-        shape = tuple(int(s) for s in np.shape(x)) if not isinstance(x, DeviceTensor) else x.shape
-        if len(shape) < 1 or shape[-1] < 1:
+        shape = x.shape if isinstance(x, DeviceTensor) else tuple(map(int, np.shape(x)))
+        if not shape or shape[-1] < 1:
             raise ValueError(f"{name} must be (..., features) with at least one feature, not {shape}")
         return shape
 
@@ -195,7 +187,7 @@ class Rows8Ops:
         F = shape[-1]
         if residual is not None and self._shape(residual, "residual") != shape:
             raise ValueError(f"residual must have shape {shape}")
-        if not (eps > 0 and np.isfinite(eps)):
+        if not 0.0 < eps < math.inf:
             raise ValueError("eps must be positive and finite")
         if isinstance(residual, DeviceTensor) and isinstance(x, DeviceTensor) and residual.dtype != x.dtype:
             raise ValueError(f"x is {x.dtype} and residual {residual.dtype}: they must have one type")
@@ -230,11 +222,8 @@ class Rows8Ops:
             raise ValueError("act must be None, 'gelu', 'silu' or 'relu'")
         if dtype not in _FLOAT:
             raise ValueError("dtype must be 'f32' or 'bf16'")
-        for t, name in ((x, "x"), (weights, "weights")):
-            if isinstance(t, Rows8):
-                self._mine(t, name)
-        x_shape = x.shape if isinstance(x, Rows8) else self._shape(x, "x")
-        w_shape = weights.shape if isinstance(weights, Rows8) else self._shape(weights, "weights")
+        x_shape = self._rows8_in(x, "x").shape if isinstance(x, Rows8) else self._shape(x, "x")
+        w_shape = self._rows8_in(weights, "weights").shape if isinstance(weights, Rows8) else self._shape(weights, "weights")
         if len(w_shape) != 2 or w_shape[0] < 1:
             raise ValueError("weights must be 2-D (out_features, in_features)")
         N, K = w_shape
