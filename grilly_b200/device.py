@@ -17,6 +17,26 @@ import numpy as np
 from . import _lib as L
 
 
+class _Block:
+    """Memory of a device's pool; given back when the last tensor that holds it goes away."""
+
+    __slots__ = ("dev", "ptr")
+
+    def __init__(self, dev: "Device", ptr: int):
+        self.dev, self.ptr = dev, ptr
+
+    def free(self) -> None:
+        ptr, self.ptr = self.ptr, 0
+        if ptr:
+            self.dev.free_ptr(ptr)
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
 class DeviceTensor:
     """A contiguous array in device memory. dtype is 'f32', 'bf16', 'i32' or 'i8'."""
 
@@ -24,12 +44,12 @@ class DeviceTensor:
     _ITEMSIZE = {"f32": 4, "bf16": 2, "i32": 4, "i8": 1}
 
     def __init__(self, dev: "Device", ptr: int, shape, dtype: str, owned: bool = True):
-        # a view is made for every operand of a call: this and __del__ are kept short
+        # a view is made for every operand of a call: this is kept short, and only memory of its own has a finaliser
         self.dev = dev
         self.ptr = ptr
         self.shape = tuple(map(int, shape))
         self.dtype = dtype
-        self._owned = owned
+        self._owned = _Block(dev, ptr) if owned is True else owned
 
     @property
     def size(self) -> int:
@@ -52,24 +72,16 @@ class DeviceTensor:
         t = DeviceTensor(self.dev, self.ptr, shape, self.dtype, owned=False)
         if t.size != self.size:
             raise ValueError(f"cannot reshape {self.shape} to {tuple(shape)}")
-        # a view keeps its base alive
-        object.__setattr__(t, "_owned", self)
+        t._owned = self   # a view keeps its base alive
         return t
 
     def numpy(self) -> np.ndarray:
         return self.dev.download(self)
 
     def free(self) -> None:
-        if self._owned is True and self.ptr:
-            self.dev.free_ptr(self.ptr)
+        if type(self._owned) is _Block:
+            self._owned.free()
             self.ptr = 0
-
-    def __del__(self):
-        try:
-            if self._owned is True:
-                self.free()
-        except Exception:
-            pass
 
 
 class Device:
@@ -123,9 +135,8 @@ class Device:
             self.lib.grilly_free(self.ctx, C.c_void_p(ptr))
 
     def empty(self, shape, dtype: str = "f32") -> DeviceTensor:
-        t = DeviceTensor(self, 0, shape, dtype)
-        t.ptr = self.alloc_ptr(max(t.nbytes, 16))
-        return t
+        shape = tuple(map(int, shape))
+        return DeviceTensor(self, self.alloc_ptr(max(math.prod(shape) * DeviceTensor._ITEMSIZE[dtype], 16)), shape, dtype)
 
     def upload(self, arr: np.ndarray, dtype: str = "f32", round_tf32: bool = False) -> DeviceTensor:
         """Copy a NumPy array to the device as fp32 (optionally rounded to tf32), bf16, int32 or int8."""
