@@ -15,6 +15,7 @@
 // a second kernel adds the planes in order (no atomics: results repeat bit for bit).
 #pragma once
 #include "ptx.cuh"
+#include "f32x2.cuh"
 #include "../../include/grilly_b200.h"
 #include <cuda_bf16.h>
 
@@ -68,16 +69,7 @@ struct Gemm8Cfg {
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of one CTA");
 };
 
-// ---- epilogue arithmetic: two neighbouring columns at a time (one instruction for two fp32 products or sums)
-struct F2 {
-  uint64_t v;
-  __device__ __forceinline__ F2() {}
-  __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
-  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-};
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { F2 d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return d; }
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) { F2 d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v)); return d; }
-__device__ __forceinline__ F2 add2(F2 a, F2 b) { F2 d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v)); return d; }
+// ---- epilogue arithmetic, two neighbouring columns at a time
 __device__ __forceinline__ float fast_rcp(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

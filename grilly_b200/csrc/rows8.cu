@@ -9,6 +9,7 @@
 #include "rows8.h"
 #include "rows8_sum.cuh"
 #include "ptx.cuh"
+#include "f32x2.cuh"
 #include <cuda_bf16.h>
 #include <algorithm>
 #include <initializer_list>
@@ -29,91 +30,100 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
   return v;
 }
-__device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(FULL, v); }
+// of magnitudes: non-negative floats order like their bits, an infinity is above every finite number and a NaN above that
+__device__ __forceinline__ float warp_max(float v) { return __uint_as_float(__reduce_max_sync(FULL, __float_as_uint(v))); }
+__device__ __forceinline__ bool not_finite(float magnitude) { return __float_as_uint(magnitude) >= INF_BITS; }
 
-// ---- VEC values of type T at p (16 bytes, or one value)
-__device__ __forceinline__ void load_vec(const float* p, float (&v)[4]) {
-  const float4 t = *reinterpret_cast<const float4*>(p);
-  v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+// A piece: VEC neighbouring values of a row (16 bytes of T, or one value), held as pairs (one value: the pair's second is 0).
+template <int VEC>
+struct Piece {
+  static constexpr int PAIRS = (VEC + 1) / 2;
+  F2 v[PAIRS];
+};
+__device__ __forceinline__ void load_piece(const float* p, Piece<4>& x) {
+  const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(p);
+  x.v[0].v = t.x;
+  x.v[1].v = t.y;
 }
-__device__ __forceinline__ void load_vec(const __nv_bfloat16* p, float (&v)[8]) {
+__device__ __forceinline__ void load_piece(const __nv_bfloat16* p, Piece<8>& x) {
   const uint4 t = *reinterpret_cast<const uint4*>(p);
   const uint32_t w[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
+  for (int i = 0; i < 4; ++i) x.v[i] = F2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
 }
-__device__ __forceinline__ void load_vec(const float* p, float (&v)[1]) { v[0] = *p; }
-__device__ __forceinline__ void load_vec(const __nv_bfloat16* p, float (&v)[1]) { v[0] = __bfloat162float(*p); }
-__device__ __forceinline__ void store_vec(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
-__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
-  const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&t);
+__device__ __forceinline__ void load_piece(const float* p, Piece<1>& x) { x.v[0] = F2(*p, 0.f); }
+__device__ __forceinline__ void load_piece(const __nv_bfloat16* p, Piece<1>& x) { x.v[0] = F2(__bfloat162float(*p), 0.f); }
+__device__ __forceinline__ void store_piece(float* p, const Piece<4>& x) { *reinterpret_cast<ulonglong2*>(p) = make_ulonglong2(x.v[0].v, x.v[1].v); }
+__device__ __forceinline__ void store_piece(__nv_bfloat16* p, const Piece<8>& x) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(x.v[0].bf16(), x.v[1].bf16(), x.v[2].bf16(), x.v[3].bf16());
 }
-__device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float (&v)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7]));
+__device__ __forceinline__ float only(const Piece<1>& x) {
+  float a, b;
+  x.v[0].get(a, b);
+  return a;
 }
-__device__ __forceinline__ void store_vec(float* p, const float (&v)[1]) { *p = v[0]; }
-__device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float (&v)[1]) { *p = __float2bfloat16(v[0]); }
+__device__ __forceinline__ void store_piece(float* p, const Piece<1>& x) { *p = only(x); }
+__device__ __forceinline__ void store_piece(__nv_bfloat16* p, const Piece<1>& x) { *p = __float2bfloat16(only(x)); }
 // VEC fp32 parameters of the columns (1 where there are none)
 template <int VEC>
-__device__ __forceinline__ void load_gamma(const float* gamma, int col, float (&g)[VEC]) {
+__device__ __forceinline__ void load_gamma(const float* gamma, int col, Piece<VEC>& g) {
   if (!gamma) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) g[j] = 1.f;
+    for (int j = 0; j < Piece<VEC>::PAIRS; ++j) g.v[j] = F2(1.f, 1.f);
   } else if constexpr (VEC == 1) {
-    g[0] = gamma[col];
+    g.v[0] = F2(gamma[col], 0.f);
   } else {
 #pragma unroll
     for (int j = 0; j < VEC; j += 4) {
-      const float4 t = *reinterpret_cast<const float4*>(gamma + col + j);
-      g[j] = t.x; g[j + 1] = t.y; g[j + 2] = t.z; g[j + 3] = t.w;
+      const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(gamma + col + j);
+      g.v[j / 2].v = t.x;
+      g.v[j / 2 + 1].v = t.y;
     }
   }
 }
 
-// |x| as bits: non-negative floats order like their bits, an infinity is above every finite number and a NaN above that,
-// so one integer maximum finds the largest magnitude and whether the row has a value that is not finite.
-__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 // max(amax / 127, 2^-126) or NaN. The quotient is the product with the rounded 1 / 127 and one correction by its remainder
 // (Markstein), the correctly rounded one for every finite amax that is not clamped (checked over all significands).
-__device__ __forceinline__ float row_scale(uint32_t amax_bits) {
-  const float a = __uint_as_float(amax_bits), r = 1.f / 127.f, q = a * r;
-  return amax_bits >= INF_BITS ? ROWS8_NAN : fmaxf(fmaf(fmaf(-127.f, q, a), r, q), ROWS8_TINY);
+__device__ __forceinline__ float row_scale(float a) {
+  const float r = 1.f / 127.f, q = a * r;
+  return not_finite(a) ? ROWS8_NAN : fmaxf(fmaf(fmaf(-127.f, q, a), r, q), ROWS8_TINY);
 }
 // 1 / scale to 1 ulp: it only decides values next to a tie. Scales lie in [2^-126, 2^121], where the approximation holds.
 __device__ __forceinline__ float row_inverse(float scale) { return __fdividef(1.f, scale); }
 // x * inv rounded to the nearest integer (ties to even), in the low byte: adding 1.5 * 2^23 leaves no fraction bits, and
 // one fused multiply-add rounds once. Four bytes come out of three byte permutes; conversions would run at a quarter rate.
-__device__ __forceinline__ uint32_t round_byte(float x, float inv) { return __float_as_uint(fmaf(x, inv, 12582912.f)); }
-__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+// keep: all ones, or zero for a row that is not finite.
+__device__ __forceinline__ uint32_t round4(F2 a, F2 b, F2 inv) {
+  const F2 magic(12582912.f, 12582912.f);
+  float f[4];
+  fma2(a, inv, magic).get(f[0], f[1]);
+  fma2(b, inv, magic).get(f[2], f[3]);
+  return __byte_perm(__byte_perm(__float_as_uint(f[0]), __float_as_uint(f[1]), 0x0040),
+                     __byte_perm(__float_as_uint(f[2]), __float_as_uint(f[3]), 0x0040), 0x5410);
 }
-// keep: all ones, or zero for a row that is not finite
-__device__ __forceinline__ void store_q(int8_t* p, const float (&v)[8], float inv, uint32_t keep) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(
-      pack4(round_byte(v[0], inv), round_byte(v[1], inv), round_byte(v[2], inv), round_byte(v[3], inv)) & keep,
-      pack4(round_byte(v[4], inv), round_byte(v[5], inv), round_byte(v[6], inv), round_byte(v[7], inv)) & keep);
+__device__ __forceinline__ void store_q(int8_t* p, const Piece<8>& x, F2 inv, uint32_t keep) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(round4(x.v[0], x.v[1], inv) & keep, round4(x.v[2], x.v[3], inv) & keep);
 }
-__device__ __forceinline__ void store_q(int8_t* p, const float (&v)[4], float inv, uint32_t keep) {
-  *reinterpret_cast<uint32_t*>(p) = pack4(round_byte(v[0], inv), round_byte(v[1], inv), round_byte(v[2], inv), round_byte(v[3], inv)) & keep;
+__device__ __forceinline__ void store_q(int8_t* p, const Piece<4>& x, F2 inv, uint32_t keep) {
+  *reinterpret_cast<uint32_t*>(p) = round4(x.v[0], x.v[1], inv) & keep;
 }
-__device__ __forceinline__ void store_q(int8_t* p, const float (&v)[1], float inv, uint32_t keep) { *p = static_cast<int8_t>(round_byte(v[0], inv) & keep); }
+__device__ __forceinline__ void store_q(int8_t* p, const Piece<1>& x, F2 inv, uint32_t keep) {
+  *p = static_cast<int8_t>(round4(x.v[0], x.v[0], inv) & keep);
+}
 // four signed bytes as floats: byte + 128 below the bits of 2^23, then the offset taken off; exact
-__device__ __forceinline__ void unpack4(uint32_t w, float* v) {
+__device__ __forceinline__ void unpack4(uint32_t w, F2& lo, F2& hi) {
   w ^= 0x80808080u;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + j)) - 8388736.f;
+  const F2 offset(-8388736.f, -8388736.f);
+  lo = add2(F2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440)), __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7441))), offset);
+  hi = add2(F2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7442)), __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7443))), offset);
 }
-__device__ __forceinline__ void load_q(const int8_t* p, float (&v)[8]) {
+__device__ __forceinline__ void load_q(const int8_t* p, Piece<8>& x) {
   const uint2 t = *reinterpret_cast<const uint2*>(p);
-  unpack4(t.x, v);
-  unpack4(t.y, v + 4);
+  unpack4(t.x, x.v[0], x.v[1]);
+  unpack4(t.y, x.v[2], x.v[3]);
 }
-__device__ __forceinline__ void load_q(const int8_t* p, float (&v)[4]) { unpack4(*reinterpret_cast<const uint32_t*>(p), v); }
-__device__ __forceinline__ void load_q(const int8_t* p, float (&v)[1]) { v[0] = static_cast<float>(*p); }
+__device__ __forceinline__ void load_q(const int8_t* p, Piece<4>& x) { unpack4(*reinterpret_cast<const uint32_t*>(p), x.v[0], x.v[1]); }
+__device__ __forceinline__ void load_q(const int8_t* p, Piece<1>& x) { x.v[0] = F2(static_cast<float>(*p), 0.f); }
 
 // ---- the ring
 // Up to three row tensors (all 16-byte aligned) and the geometry that the host chose.
@@ -124,7 +134,8 @@ struct Ring {
   int bytes[3];              // bytes of one row
   int at[3];                 // where a tensor's row lies in a slot
   int tensors, slot;         // slot: bytes, a multiple of 16
-  int team, teams, depth;    // threads per team, teams per CTA, slots per team
+  int aligned;               // every row starts on a 16-byte boundary and holds a multiple of 16 bytes
+  int depth;                 // slots per team
   int gamma_at, slots_at;    // offsets in shared memory: barriers first, then reductions, gamma, slots
   long long rows;
   long long first_tail;      // from this row on, bytes past the tensors' last 16-byte boundary are needed
@@ -132,8 +143,7 @@ struct Ring {
   int* err;
 };
 struct RowStats {
-  float sq;
-  uint32_t my, mh;
+  float sq, my, mh;            // sum of squares, max |h gamma|, max |h|
 };
 constexpr int RED_AT = MAX_TEAMS * MAX_DEPTH * 8;              // RowStats [2][CTA / 32]
 constexpr int ABORT_AT = RED_AT + 2 * (CTA / 32) * 12;
@@ -145,8 +155,10 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-// A team's view of the ring. All of a team's threads call next() and done() together.
+// A team's view of the ring (TEAM threads). All of a team's threads call next() and done() together.
+template <int TEAM>
 struct Team {
+  static constexpr int TEAMS = CTA / TEAM;
   const Ring& g;
   uint8_t* smem;
   uint64_t* bars;
@@ -155,20 +167,20 @@ struct Team {
   uint32_t flip;                 // which half of the reduction scratch
   long long row, step;
 
-  __device__ Team(const Ring& ring, uint8_t* shared) : g(ring), smem(shared), flip(0) {
-    team = threadIdx.x / g.team;
-    tid = threadIdx.x - team * g.team;
+  __device__ __forceinline__ Team(const Ring& ring, uint8_t* shared) : g(ring), smem(shared), flip(0) {
+    team = threadIdx.x / TEAM;
+    tid = threadIdx.x % TEAM;
     bars = reinterpret_cast<uint64_t*>(smem) + team * g.depth;
     abort_flag = reinterpret_cast<volatile int*>(smem + ABORT_AT);
-    row = team < g.teams ? static_cast<long long>(team) * gridDim.x + blockIdx.x : g.rows;   // long rows leave threads idle
-    step = static_cast<long long>(g.teams) * gridDim.x;
+    row = static_cast<long long>(team) * gridDim.x + blockIdx.x;
+    step = static_cast<long long>(TEAMS) * gridDim.x;
     slot = 0;
     parity = 0;
   }
   // whole CTA: barriers, gamma, the first rows on their way
   __device__ void start(const float* gamma) {
     if (threadIdx.x == 0) {
-      for (int i = 0; i < g.teams * g.depth; ++i) mbar_init(reinterpret_cast<uint64_t*>(smem) + i, 1);
+      for (int i = 0; i < TEAMS * g.depth; ++i) mbar_init(reinterpret_cast<uint64_t*>(smem) + i, 1);
       *abort_flag = 0;
       fence_mbar_init();
     }
@@ -190,6 +202,14 @@ struct Team {
   __device__ uint8_t* slot_of(int d) const { return smem + g.slots_at + (team * g.depth + d) * g.slot; }
   __device__ void fetch(long long r, int d) const {
     if (r >= g.rows) return;
+    if (g.aligned) {
+      uint8_t* to = slot_of(d);
+      mbar_expect_tx(&bars[d], g.slot);
+      bulk_load(to, static_cast<const uint8_t*>(g.src[0]) + r * g.pitch[0], g.bytes[0], &bars[d]);
+      if (g.tensors > 1) bulk_load(to + g.at[1], static_cast<const uint8_t*>(g.src[1]) + r * g.pitch[1], g.bytes[1], &bars[d]);
+      if (g.tensors > 2) bulk_load(to + g.at[2], static_cast<const uint8_t*>(g.src[2]) + r * g.pitch[2], g.bytes[2], &bars[d]);
+      return;
+    }
     uint32_t sum = 0;
     long long from[3], to[3];
 #pragma unroll
@@ -206,8 +226,8 @@ struct Team {
         bulk_load(slot_of(d) + g.at[i], static_cast<const uint8_t*>(g.src[i]) + from[i], static_cast<uint32_t>(to[i] - from[i]), &bars[d]);
   }
   __device__ void sync() const {
-    if (g.team == 32) __syncwarp();
-    else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(g.team) : "memory");
+    if constexpr (TEAM == 32) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(TEAM) : "memory");
   }
   // waits for the current row; false: the wait ran out (reported) and the team stops
   __device__ bool next() {
@@ -228,7 +248,7 @@ struct Team {
         }
       }
     }
-    if (g.team == 32) {
+    if constexpr (TEAM == 32) {
       ok = __all_sync(FULL, ok);
     } else {
       asm volatile(
@@ -238,7 +258,7 @@ struct Team {
           "bar.red.and.pred q, %2, %3, p;\n\t"
           "selp.s32 %0, 1, 0, q;\n\t"
           "}\n"
-          : "=r"(ok) : "r"(ok), "r"(team + 1), "r"(g.team) : "memory");
+          : "=r"(ok) : "r"(ok), "r"(team + 1), "n"(TEAM) : "memory");
     }
     return ok != 0;
   }
@@ -269,13 +289,14 @@ struct Team {
     if constexpr (kSum) s.sq = warp_sum(s.sq);
     if constexpr (kMax) s.mh = warp_max(s.mh);
     if constexpr (kTwo) s.my = warp_max(s.my);
-    if (g.team > 32) {
-      const int lane = threadIdx.x & 31, warps = g.team >> 5;
+    if constexpr (TEAM > 32) {
+      constexpr int WARPS = TEAM / 32;
+      const int lane = threadIdx.x & 31;
       RowStats* red = reinterpret_cast<RowStats*>(smem + RED_AT) + flip * (CTA / 32);
       flip ^= 1;             // the other half is free again once every thread has passed this row's barriers
       if (lane == 0) red[threadIdx.x >> 5] = s;
       sync();
-      s = lane < warps ? red[team * warps + lane] : RowStats{0.f, 0u, 0u};
+      s = lane < WARPS ? red[team * WARPS + lane] : RowStats{0.f, 0.f, 0.f};
       if constexpr (kSum) s.sq = warp_sum(s.sq);
       if constexpr (kMax) s.mh = warp_max(s.mh);
       if constexpr (kTwo) s.my = warp_max(s.my);
@@ -283,7 +304,12 @@ struct Team {
     return s;
   }
 };
-#define FOR_PIECES(i, c) _Pragma("unroll") for (int i = 0, c = t.tid * VEC; i < NV; ++i, c += t.g.team * VEC) if (c < F)
+// The pieces of a row that a thread has: i counts them, c is the first column. Rows shorter than a team's full width leave
+// the loop for all threads at once.
+#define FOR_PIECES(i, c)                                                                       \
+  _Pragma("unroll") for (int i = 0, c = t.tid * VEC; i < NV; ++i, c += TEAM * VEC)              \
+    if (i * TEAM * VEC >= F) break;                                                            \
+    else if (c < F)
 
 // ---- a row per block of 1024 threads, for what the ring does not take
 __device__ __forceinline__ RowStats block_reduce(RowStats s, RowStats* red) {
@@ -301,29 +327,30 @@ __device__ __forceinline__ RowStats block_reduce(RowStats s, RowStats* red) {
 }
 
 // ---------------------------------------------------------------- quantise
-template <class T, int VEC>
+template <class T, int VEC, int TEAM>
 __global__ void __launch_bounds__(CTA, 1) quantize_rows_kernel(const __grid_constant__ Ring ring, int8_t* q, float* scale, long long ld) {
-  constexpr int NV = PER_THREAD / VEC;
+  constexpr int NV = PER_THREAD / VEC, PAIRS = Piece<VEC>::PAIRS;
   extern __shared__ __align__(16) uint8_t smem[];
-  Team t(ring, smem);
+  Team<TEAM> t(ring, smem);
   t.start(nullptr);
   const int F = ring.F;
   for (; t.row < ring.rows; t.done()) {
     if (!t.next()) break;
-    const T* xp = t.values<T>(0);
-    float v[NV][VEC];
-    RowStats s{0.f, 0u, 0u};
+    const T* xp = t.template values<T>(0);
+    Piece<VEC> x[NV];
+    float m = 0.f;
     FOR_PIECES(i, c) {
-      load_vec(xp + c, v[i]);
+      load_piece(xp + c, x[i]);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) s.mh = max(s.mh, abs_bits(v[i][j]));
+      for (int j = 0; j < PAIRS; ++j) m = max_abs(m, x[i].v[j]);
     }
-    s = t.reduce<false, true, false>(s);
-    const float sc = row_scale(s.mh), inv = row_inverse(sc);
-    const uint32_t keep = s.mh >= INF_BITS ? 0u : FULL;
+    m = t.template reduce<false, true, false>(RowStats{0.f, 0.f, m}).mh;
+    const float sc = row_scale(m), inv = row_inverse(sc);
+    const F2 inv2(inv, inv);
+    const uint32_t keep = not_finite(m) ? 0u : FULL;
     int8_t* qp = q + t.row * ld;
-    FOR_PIECES(i, c) store_q(qp + c, v[i], inv, keep);
-    for (long long c = F + t.tid; c < ld; c += ring.team) qp[c] = 0;
+    FOR_PIECES(i, c) store_q(qp + c, x[i], inv2, keep);
+    for (long long c = F + t.tid; c < ld; c += TEAM) qp[c] = 0;
     if (t.tid == 0) scale[t.row] = sc;
   }
   t.end();
@@ -334,19 +361,19 @@ __global__ void __launch_bounds__(1024) quantize_long_rows_kernel(const T* x, in
   __shared__ RowStats red[32];
   for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* xp = x + row * F;
-    RowStats s{0.f, 0u, 0u};
-    float v[1];
+    RowStats s{0.f, 0.f, 0.f};
+    Piece<1> v;
     for (int c = threadIdx.x; c < F; c += blockDim.x) {
-      load_vec(xp + c, v);
-      s.mh = max(s.mh, abs_bits(v[0]));
+      load_piece(xp + c, v);
+      s.mh = max_abs(s.mh, v.v[0]);
     }
     s = block_reduce(s, red);
     const float sc = row_scale(s.mh), inv = row_inverse(sc);
-    const uint32_t keep = s.mh >= INF_BITS ? 0u : FULL;
+    const uint32_t keep = not_finite(s.mh) ? 0u : FULL;
     for (long long c = threadIdx.x; c < ld; c += blockDim.x) {
-      v[0] = 0.f;
-      if (c < F) load_vec(xp + c, v);
-      store_q(q + row * ld + c, v, inv, keep);
+      v.v[0] = F2(0.f, 0.f);
+      if (c < F) load_piece(xp + c, v);
+      store_q(q + row * ld + c, v, F2(inv, inv), keep);
     }
     if (threadIdx.x == 0) scale[row] = sc;
     __syncthreads();
@@ -363,15 +390,16 @@ __global__ void __launch_bounds__(256) dequantize_vec_kernel(const int8_t* __res
     const uint32_t row = i / per_row, c = (i - row * per_row) * 16;
     const uint4 w = *reinterpret_cast<const uint4*>(q + row * ld + c);
     const float s = __ldg(scale + row);
-    float v[16];
-    unpack4(w.x, v); unpack4(w.y, v + 4); unpack4(w.z, v + 8); unpack4(w.w, v + 12);
+    const F2 s2(s, s);
+    F2 v[8];
+    unpack4(w.x, v[0], v[1]); unpack4(w.y, v[2], v[3]); unpack4(w.z, v[4], v[5]); unpack4(w.w, v[6], v[7]);
     T* yp = y + (static_cast<long long>(row) * per_row * 16 + c);
 #pragma unroll
     for (int k = 0; k < 16; k += VEC) {
-      float o[VEC];
+      Piece<VEC> o;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) o[j] = v[k + j] * s;
-      store_vec(yp + k, o);
+      for (int j = 0; j < VEC / 2; ++j) o.v[j] = mul2(v[k / 2 + j], s2);
+      store_piece(yp + k, o);
     }
   }
 }
@@ -384,8 +412,9 @@ __global__ void __launch_bounds__(256) dequantize_any_kernel(const int8_t* __res
     const float s = __ldg(scale + row);
 #pragma unroll 8
     for (int c = lane; c < F; c += 32) {
-      const float v[1] = {static_cast<float>(q[row * ld + c]) * s};
-      store_vec(y + row * F + c, v);
+      Piece<1> v;
+      v.v[0] = F2(static_cast<float>(q[row * ld + c]) * s, 0.f);
+      store_piece(y + row * F + c, v);
     }
   }
 }
@@ -411,13 +440,13 @@ struct NormScales {
 };
 __device__ __forceinline__ NormScales norm_scales(const RowStats& s, float inv_f, float eps) {
   NormScales r;
-  const bool bad = abs_bits(s.sq) >= INF_BITS || s.my >= INF_BITS;
+  const bool bad = not_finite(s.sq) || not_finite(s.my);   // a sum of squares: never negative
   r.keep = bad ? 0u : FULL;
   const float var = s.sq * inv_f + eps;
   float t = rsqrtf(var);                       // within 2 ulp; one Newton step brings it to the rounding of 1 / sqrt
   t = fmaf(t, fmaf(-0.5f * var * t, t, 0.5f), t);
   r.rstd = bad ? ROWS8_NAN : t;
-  r.ys = bad ? ROWS8_NAN : row_scale(abs_bits(__uint_as_float(s.my) * r.rstd));
+  r.ys = bad ? ROWS8_NAN : row_scale(s.my * r.rstd);
   r.hs = bad ? ROWS8_NAN : row_scale(s.mh);
   r.yi = row_inverse(r.ys);
   r.hi = row_inverse(r.hs);
@@ -431,55 +460,59 @@ __device__ __forceinline__ void norm_row_done(const NormQ8Args& a, const NormSca
 
 // One reduction serves both outputs: the largest |h gamma| times rstd is the largest |y|, so sum h^2, max |h gamma| and
 // max |h| are taken together and nothing waits for rstd. A row has been read whole before h is written (in place).
-template <class T, int VEC>
+template <class T, int VEC, int TEAM>
 __global__ void __launch_bounds__(CTA, 1) rmsnorm_q8_kernel(const __grid_constant__ Ring ring, const NormQ8Args a) {
-  constexpr int NV = PER_THREAD / VEC;
+  constexpr int NV = PER_THREAD / VEC, PAIRS = Piece<VEC>::PAIRS;
   extern __shared__ __align__(16) uint8_t smem[];
-  Team t(ring, smem);
+  Team<TEAM> t(ring, smem);
   t.start(a.gamma);
   const float* gamma = a.gamma ? reinterpret_cast<const float*>(smem + ring.gamma_at) : nullptr;
   const int F = ring.F;
   const float inv_f = 1.f / static_cast<float>(F);
   for (; t.row < ring.rows; t.done()) {
     if (!t.next()) break;
-    const T* xp = t.values<T>(0);
-    const T* rp = ring.tensors > 1 ? t.values<T>(1) : nullptr;
-    float h[NV][VEC], sum[4] = {0.f, 0.f, 0.f, 0.f};
-    RowStats s{0.f, 0u, 0u};
+    const T* xp = t.template values<T>(0);
+    const T* rp = ring.tensors > 1 ? t.template values<T>(1) : nullptr;
+    Piece<VEC> h[NV];
+    F2 sum[2] = {F2(0.f, 0.f), F2(0.f, 0.f)};
+    RowStats s{0.f, 0.f, 0.f};
     FOR_PIECES(i, c) {
-      load_vec(xp + c, h[i]);
+      load_piece(xp + c, h[i]);
       if (rp) {
-        float r[VEC];
-        load_vec(rp + c, r);
+        Piece<VEC> r;
+        load_piece(rp + c, r);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) h[i][j] += r[j];
+        for (int j = 0; j < PAIRS; ++j) h[i].v[j] = add2(h[i].v[j], r.v[j]);
       }
-      float gm[VEC];
+      Piece<VEC> gm;
       load_gamma(gamma, c, gm);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        float& acc = sum[(i * VEC + j) & 3];
-        acc = fmaf(h[i][j], h[i][j], acc);
-        s.my = max(s.my, abs_bits(h[i][j] * gm[j]));
-        s.mh = max(s.mh, abs_bits(h[i][j]));
+      for (int j = 0; j < PAIRS; ++j) {
+        F2& acc = sum[(i * PAIRS + j) & 1];
+        acc = fma2(h[i].v[j], h[i].v[j], acc);
+        s.my = max_abs(s.my, mul2(h[i].v[j], gm.v[j]));
+        s.mh = max_abs(s.mh, h[i].v[j]);
       }
     }
-    s.sq = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    s = t.reduce<true, true, true>(s);
+    float even, odd;
+    add2(sum[0], sum[1]).get(even, odd);
+    s.sq = even + odd;
+    s = t.template reduce<true, true, true>(s);
     const NormScales r = norm_scales(s, inv_f, a.eps);
+    const F2 rstd(r.rstd, r.rstd), yi(r.yi, r.yi), hi(r.hi, r.hi);
     T* hp = a.h ? static_cast<T*>(a.h) + t.row * F : nullptr;
     int8_t* yq = a.yq + t.row * a.ld;
     int8_t* hq = a.hq ? a.hq + t.row * a.ld : nullptr;
     FOR_PIECES(i, c) {
-      if (hp) store_vec(hp + c, h[i]);
-      if (hq) store_q(hq + c, h[i], r.hi, r.keep);
-      float gm[VEC];
-      load_gamma(gamma, c, gm);
+      if (hp) store_piece(hp + c, h[i]);
+      if (hq) store_q(hq + c, h[i], hi, r.keep);
+      Piece<VEC> y;
+      load_gamma(gamma, c, y);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) gm[j] *= h[i][j] * r.rstd;
-      store_q(yq + c, gm, r.yi, r.keep);
+      for (int j = 0; j < PAIRS; ++j) y.v[j] = mul2(mul2(h[i].v[j], rstd), y.v[j]);
+      store_q(yq + c, y, yi, r.keep);
     }
-    for (long long c = F + t.tid; c < a.ld; c += ring.team) {
+    for (long long c = F + t.tid; c < a.ld; c += TEAM) {
       yq[c] = 0;
       if (hq) hq[c] = 0;
     }
@@ -494,33 +527,33 @@ __global__ void __launch_bounds__(1024) rmsnorm_q8_long_kernel(const NormQ8Args 
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* xp = static_cast<const T*>(a.x) + row * a.F;
     const T* rp = a.residual ? static_cast<const T*>(a.residual) + row * a.F : nullptr;
-    RowStats s{0.f, 0u, 0u};
-    float h[1], r[1], gm[1];
+    RowStats s{0.f, 0.f, 0.f};
+    Piece<1> h, r, gm;
     auto in = [&](int c) {
-      load_vec(xp + c, h);
+      load_piece(xp + c, h);
       if (rp) {
-        load_vec(rp + c, r);
-        h[0] += r[0];
+        load_piece(rp + c, r);
+        h.v[0] = add2(h.v[0], r.v[0]);
       }
       load_gamma(a.gamma, c, gm);
     };
     for (int c = threadIdx.x; c < a.F; c += blockDim.x) {
       in(c);
-      s.sq = fmaf(h[0], h[0], s.sq);
-      s.my = max(s.my, abs_bits(h[0] * gm[0]));
-      s.mh = max(s.mh, abs_bits(h[0]));
+      s.sq = fmaf(only(h), only(h), s.sq);
+      s.my = max_abs(s.my, mul2(h.v[0], gm.v[0]));
+      s.mh = max_abs(s.mh, h.v[0]);
     }
     s = block_reduce(s, red);
     const NormScales n = norm_scales(s, 1.f / static_cast<float>(a.F), a.eps);
     for (long long c = threadIdx.x; c < a.ld; c += blockDim.x) {
-      h[0] = gm[0] = 0.f;
+      h.v[0] = gm.v[0] = F2(0.f, 0.f);
       if (c < a.F) {
         in(static_cast<int>(c));
-        if (a.h) store_vec(static_cast<T*>(a.h) + row * a.F + c, h);
+        if (a.h) store_piece(static_cast<T*>(a.h) + row * a.F + c, h);
       }
-      if (a.hq) store_q(a.hq + row * a.ld + c, h, n.hi, n.keep);
-      gm[0] *= h[0] * n.rstd;
-      store_q(a.yq + row * a.ld + c, gm, n.yi, n.keep);
+      if (a.hq) store_q(a.hq + row * a.ld + c, h, F2(n.hi, n.hi), n.keep);
+      gm.v[0] = mul2(mul2(h.v[0], F2(n.rstd, n.rstd)), gm.v[0]);
+      store_q(a.yq + row * a.ld + c, gm, F2(n.yi, n.yi), n.keep);
     }
     if (threadIdx.x == 0) norm_row_done(a, n, row);
     __syncthreads();
@@ -544,72 +577,86 @@ struct NormBwdQ8Args {
 // A thread keeps the same columns of every row that its team meets, so the gradient of gamma is summed in registers and
 // leaves once per CTA; the CTAs' sums are added by sum_partials_kernel in a fixed order. The row is read from the ring
 // twice (before and after its one sum) instead of being held next to those sums.
-template <class T, int VEC>
+template <class T, int VEC, int TEAM>
 __global__ void __launch_bounds__(CTA, 1) rmsnorm_bwd_kernel(const __grid_constant__ Ring ring, const NormBwdQ8Args a) {
-  constexpr int NV = PER_THREAD / VEC;
+  constexpr int NV = PER_THREAD / VEC, PAIRS = Piece<VEC>::PAIRS;
   extern __shared__ __align__(16) uint8_t smem[];
-  Team t(ring, smem);
+  Team<TEAM> t(ring, smem);
   t.start(a.gamma);
   const float* gamma = a.gamma ? reinterpret_cast<const float*>(smem + ring.gamma_at) : nullptr;
   const int F = ring.F;
   const float inv_f = 1.f / static_cast<float>(F);
-  float acc[NV][VEC];
+  Piece<VEC> acc[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) acc[i][j] = 0.f;
+    for (int j = 0; j < PAIRS; ++j) acc[i].v[j] = F2(0.f, 0.f);
   for (; t.row < ring.rows; t.done()) {
     const float rstd = __ldg(a.rstd + t.row), s = __ldg(a.hs + t.row) * rstd;
+    const F2 s2(s, s), rstd2(rstd, rstd);
     if (!t.next()) break;
-    const int8_t* qp = t.values<int8_t>(0);
-    const T* gp = t.values<T>(1);
-    const T* rp = ring.tensors > 2 ? t.values<T>(2) : nullptr;
-    float dots[4] = {0.f, 0.f, 0.f, 0.f};
+    const int8_t* qp = t.template values<int8_t>(0);
+    const T* gp = t.template values<T>(1);
+    const T* rp = ring.tensors > 2 ? t.template values<T>(2) : nullptr;
+    F2 dots[2] = {F2(0.f, 0.f), F2(0.f, 0.f)};
     FOR_PIECES(i, c) {
-      float g[VEC], n[VEC], gm[VEC];
-      load_vec(gp + c, g);
+      Piece<VEC> g, n, gm;
+      load_piece(gp + c, g);
       load_q(qp + c, n);
       load_gamma(gamma, c, gm);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        n[j] *= s;
-        acc[i][j] = fmaf(g[j], n[j], acc[i][j]);
-        float& dot = dots[(i * VEC + j) & 3];
-        dot = fmaf(g[j] * gm[j], n[j], dot);
+      for (int j = 0; j < PAIRS; ++j) {
+        n.v[j] = mul2(n.v[j], s2);
+        acc[i].v[j] = fma2(g.v[j], n.v[j], acc[i].v[j]);
+        F2& dot = dots[(i * PAIRS + j) & 1];
+        dot = fma2(mul2(g.v[j], gm.v[j]), n.v[j], dot);
       }
     }
-    const float dot = t.reduce<true, false, false>(RowStats{(dots[0] + dots[1]) + (dots[2] + dots[3]), 0u, 0u}).sq * inv_f;
+    float even, odd;
+    add2(dots[0], dots[1]).get(even, odd);
+    const float dot = t.template reduce<true, false, false>(RowStats{even + odd, 0.f, 0.f}).sq * inv_f;
+    const F2 back(-s * dot, -s * dot);       // the row's part along n, for the bytes of n
     T* op = static_cast<T*>(a.gh) + t.row * F;
     FOR_PIECES(i, c) {
-      float g[VEC], n[VEC], gm[VEC];
-      load_vec(gp + c, g);
+      Piece<VEC> g, n, r;
+      load_piece(gp + c, g);
       load_q(qp + c, n);
-      load_gamma(gamma, c, gm);
+      load_gamma(gamma, c, r);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) g[j] = rstd * (g[j] * gm[j] - n[j] * s * dot);
+      for (int j = 0; j < PAIRS; ++j) g.v[j] = fma2(n.v[j], back, mul2(g.v[j], r.v[j]));
       if (rp) {
-        float r[VEC];
-        load_vec(rp + c, r);
+        load_piece(rp + c, r);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) g[j] += r[j];
+        for (int j = 0; j < PAIRS; ++j) g.v[j] = fma2(g.v[j], rstd2, r.v[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < PAIRS; ++j) g.v[j] = mul2(g.v[j], rstd2);
       }
-      store_vec(op + c, g);
+      store_piece(op + c, g);
     }
   }
   t.end();
   if (!a.partial) return;
-  // the teams' sums, one after the other, through the ring's memory: every row that was fetched has been waited for
+  // the teams' sums side by side in the ring's memory (teams * F <= 512 * 32: every row that was fetched has been waited
+  // for), then added in the teams' order
   float* columns = reinterpret_cast<float*>(smem + ring.slots_at);
-  for (int w = 0; w < ring.teams; ++w) {
-    if (t.team == w) {
-      FOR_PIECES(i, c) {
+  float* mine = columns + t.team * F;
+  FOR_PIECES(i, c) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) columns[c + j] = w == 0 ? acc[i][j] : columns[c + j] + acc[i][j];
-      }
+    for (int j = 0; j < PAIRS; ++j) {
+      float lo, hi;
+      acc[i].v[j].get(lo, hi);
+      mine[c + 2 * j] = lo;
+      if constexpr (VEC > 1) mine[c + 2 * j + 1] = hi;
     }
-    __syncthreads();
   }
-  for (int c = threadIdx.x; c < F; c += CTA) a.partial[static_cast<long long>(blockIdx.x) * F + c] = columns[c];
+  __syncthreads();
+  for (int c = threadIdx.x; c < F; c += CTA) {
+    float sum = columns[c];
+#pragma unroll
+    for (int w = 1; w < CTA / TEAM; ++w) sum += columns[w * F + c];
+    a.partial[static_cast<long long>(blockIdx.x) * F + c] = sum;
+  }
 }
 // What the ring does not take: the rows in two passes, the columns by themselves before them (grad_h may be
 // grad_out).
@@ -622,20 +669,21 @@ __global__ void __launch_bounds__(1024) rmsnorm_bwd_long_rows_kernel(const NormB
     T* op = static_cast<T*>(a.gh) + row * a.F;
     const int8_t* qp = a.hq + row * a.ld;
     const float rstd = a.rstd[row], s = a.hs[row] * rstd;
-    RowStats st{0.f, 0u, 0u};
-    float g[1], gm[1], r[1] = {0.f};
+    RowStats st{0.f, 0.f, 0.f};
+    Piece<1> g, gm, r;
     for (int c = threadIdx.x; c < a.F; c += blockDim.x) {
-      load_vec(gp + c, g);
+      load_piece(gp + c, g);
       load_gamma(a.gamma, c, gm);
-      st.sq = fmaf(g[0] * gm[0], static_cast<float>(qp[c]) * s, st.sq);
+      st.sq = fmaf(only(g) * only(gm), static_cast<float>(qp[c]) * s, st.sq);
     }
     const float dot = block_reduce(st, red).sq / static_cast<float>(a.F);
     for (int c = threadIdx.x; c < a.F; c += blockDim.x) {
-      load_vec(gp + c, g);
+      load_piece(gp + c, g);
       load_gamma(a.gamma, c, gm);
-      if (rp) load_vec(rp + c, r);
-      g[0] = rstd * (g[0] * gm[0] - static_cast<float>(qp[c]) * s * dot) + r[0];
-      store_vec(op + c, g);
+      r.v[0] = F2(0.f, 0.f);
+      if (rp) load_piece(rp + c, r);
+      g.v[0] = F2(rstd * (only(g) * only(gm) - static_cast<float>(qp[c]) * s * dot) + only(r), 0.f);
+      store_piece(op + c, g);
     }
     __syncthreads();
   }
@@ -645,10 +693,11 @@ __global__ void __launch_bounds__(256) rmsnorm_bwd_long_columns_kernel(const Nor
   const long long r0 = static_cast<long long>(blockIdx.x) * rows_per_block;
   const long long r1 = min(a.rows, r0 + rows_per_block);
   for (int f = threadIdx.x; f < a.F; f += blockDim.x) {
-    float acc = 0.f, g[1];
+    float acc = 0.f;
+    Piece<1> g;
     for (long long r = r0; r < r1; ++r) {
-      load_vec(static_cast<const T*>(a.go) + r * a.F + f, g);
-      acc = fmaf(g[0], static_cast<float>(a.hq[r * a.ld + f]) * (a.hs[r] * a.rstd[r]), acc);
+      load_piece(static_cast<const T*>(a.go) + r * a.F + f, g);
+      acc = fmaf(only(g), static_cast<float>(a.hq[r * a.ld + f]) * (a.hs[r] * a.rstd[r]), acc);
     }
     a.partial[static_cast<long long>(blockIdx.x) * a.F + f] = acc;
   }
@@ -661,24 +710,26 @@ bool aligned16(std::initializer_list<const void*> ps) {
 }
 constexpr int RING_BYTES = 216 * 1024;
 
-// The ring's geometry; false where the rows do not fit it (more than 512 * 32 values, fewer than two rows in shared memory,
-// pointers off 16-byte boundaries). It depends on the row's length alone, so a row's sums have the same order, and its
+// The ring's geometry, for rows of up to 512 * 32 values of which two per team fit shared memory, on tensors that start on
+// 16-byte boundaries. It depends on the row's length alone, so a row's sums have the same order, and its
 // result the same bits, in every batch.
 struct RowTensor {
   const void* p;
   long long pitch;   // bytes
   int bytes;
 };
-bool make_ring(grilly_ctx* ctx, Ring& g, long long rows, int F, const RowTensor* tensors, int count, bool gamma, size_t* smem, unsigned* grid) {
-  if (F > CTA * PER_THREAD) return false;
+// Returns the threads per row, or 0.
+int make_ring(grilly_ctx* ctx, Ring& g, long long rows, int F, const RowTensor* tensors, int count, bool gamma, size_t* smem, unsigned* grid) {
+  if (F > CTA * PER_THREAD) return 0;
   g = Ring{};
   g.rows = rows;
   g.F = F;
   g.err = ctx->err_dev;
   g.tensors = count;
+  g.aligned = 1;
   g.first_tail = rows;
   for (int i = 0; i < count; ++i) {
-    if (reinterpret_cast<uintptr_t>(tensors[i].p) & 15) return false;
+    if (reinterpret_cast<uintptr_t>(tensors[i].p) & 15) return 0;
     g.src[i] = tensors[i].p;
     g.pitch[i] = tensors[i].pitch;
     g.bytes[i] = tensors[i].bytes;
@@ -686,27 +737,33 @@ bool make_ring(grilly_ctx* ctx, Ring& g, long long rows, int F, const RowTensor*
     const long long whole = g.total[i] & ~15ll;
     g.first_tail = std::min(g.first_tail, whole < g.bytes[i] ? 0 : (whole - g.bytes[i]) / g.pitch[i] + 1);
     g.at[i] = g.slot;
+    if (g.pitch[i] % 16 || g.bytes[i] % 16) g.aligned = 0;
     g.slot += (tensors[i].bytes + 15) / 16 * 16 + (tensors[i].pitch % 16 ? 16 : 0);
   }
-  g.team = 32;
-  while (g.team * PER_THREAD < F) g.team *= 2;
-  g.teams = CTA / g.team;
   g.gamma_at = GAMMA_AT;
   g.slots_at = GAMMA_AT + (gamma ? (4 * F + 15) / 16 * 16 : 0);
+  // the smallest team that holds a row, but few enough of them that each has two rows in shared memory: the threads that
+  // long rows leave without a row of their own join the others
   const int room = RING_BYTES - g.slots_at;
-  g.depth = std::min(MAX_DEPTH, room / (g.slot * g.teams));
-  // long rows: fewer of them at a time rather than none ahead
-  while (g.depth < 2 && g.teams > 1) {
-    g.teams /= 2;
-    g.depth = std::min(MAX_DEPTH, room / (g.slot * g.teams));
-  }
-  if (g.depth < 2) return false;
+  int team = 32;
+  while (team < CTA && (team * PER_THREAD < F || CTA / team * 2 * g.slot > room)) team *= 2;
+  const int teams = CTA / team;
+  if (teams * 2 * g.slot > room) return 0;
   *grid = static_cast<unsigned>(std::min<long long>(rows, ctx->num_sms));
-  const long long per_team = (rows + static_cast<long long>(*grid) * g.teams - 1) / (static_cast<long long>(*grid) * g.teams);
-  g.depth = static_cast<int>(std::min<long long>(g.depth, per_team));
-  *smem = g.slots_at + std::max(static_cast<size_t>(g.slot) * g.teams * g.depth, sizeof(float) * static_cast<size_t>(F));
-  return true;
+  const long long per_team = (rows + static_cast<long long>(*grid) * teams - 1) / (static_cast<long long>(*grid) * teams);
+  g.depth = static_cast<int>(std::min<long long>(std::min(MAX_DEPTH, room / (g.slot * teams)), per_team));
+  *smem = g.slots_at + std::max(static_cast<size_t>(g.slot) * teams * g.depth, sizeof(float) * static_cast<size_t>(F) * teams);
+  return team;
 }
+// CALL(TEAM) for the team of a ring
+#define WITH_TEAM(team, CALL)      \
+  switch (team) {                  \
+    case 32: CALL(32); break;      \
+    case 64: CALL(64); break;      \
+    case 128: CALL(128); break;    \
+    case 256: CALL(256); break;    \
+    default: CALL(512);            \
+  }
 template <class K>
 int allow_ring(grilly_ctx* ctx, K kern) {
   const void* key = reinterpret_cast<const void*>(kern);
@@ -725,11 +782,15 @@ int launch_quantize(grilly_ctx* ctx, const T* x, int8_t* q, float* scale, long l
   size_t smem;
   unsigned grid;
   const RowTensor in[1] = {{x, static_cast<long long>(sizeof(T)) * F, static_cast<int>(sizeof(T)) * F}};
-  if (!make_ring(ctx, ring, rows, F, in, 1, false, &smem, &grid)) {
+  const int team = make_ring(ctx, ring, rows, F, in, 1, false, &smem, &grid);
+  if (!team) {
     quantize_long_rows_kernel<<<any_grid(rows), 1024, 0, ctx->stream>>>(x, q, scale, rows, F, ld);
     return GRILLY_OK;
   }
-  auto kern = F % VEC == 0 ? quantize_rows_kernel<T, VEC> : quantize_rows_kernel<T, 1>;
+  void (*kern)(const Ring, int8_t*, float*, long long) = nullptr;
+#define PICK(TEAM) kern = F % VEC == 0 ? quantize_rows_kernel<T, VEC, TEAM> : quantize_rows_kernel<T, 1, TEAM>
+  WITH_TEAM(team, PICK)
+#undef PICK
   if (int rc = allow_ring(ctx, kern)) return rc;
   kern<<<grid, CTA, smem, ctx->stream>>>(ring, q, scale, ld);
   return GRILLY_OK;
@@ -755,11 +816,15 @@ int launch_rmsnorm(grilly_ctx* ctx, const NormQ8Args& a) {
   unsigned grid;
   const long long pitch = static_cast<long long>(sizeof(T)) * a.F;
   const RowTensor in[2] = {{a.x, pitch, static_cast<int>(pitch)}, {a.residual, pitch, static_cast<int>(pitch)}};
-  if (!aligned16({a.h}) || !make_ring(ctx, ring, a.rows, a.F, in, a.residual ? 2 : 1, a.gamma != nullptr, &smem, &grid)) {
+  const int team = aligned16({a.h}) ? make_ring(ctx, ring, a.rows, a.F, in, a.residual ? 2 : 1, a.gamma != nullptr, &smem, &grid) : 0;
+  if (!team) {
     rmsnorm_q8_long_kernel<T><<<any_grid(a.rows), 1024, 0, ctx->stream>>>(a);
     return GRILLY_OK;
   }
-  auto kern = a.F % VEC == 0 ? rmsnorm_q8_kernel<T, VEC> : rmsnorm_q8_kernel<T, 1>;
+  void (*kern)(const Ring, const NormQ8Args) = nullptr;
+#define PICK(TEAM) kern = a.F % VEC == 0 ? rmsnorm_q8_kernel<T, VEC, TEAM> : rmsnorm_q8_kernel<T, 1, TEAM>
+  WITH_TEAM(team, PICK)
+#undef PICK
   if (int rc = allow_ring(ctx, kern)) return rc;
   kern<<<grid, CTA, smem, ctx->stream>>>(ring, a);
   return GRILLY_OK;
@@ -774,8 +839,12 @@ int launch_rmsnorm_bwd(grilly_ctx* ctx, NormBwdQ8Args& a, float* grad_gamma) {
   unsigned grid;
   const long long pitch = static_cast<long long>(sizeof(T)) * a.F;
   const RowTensor in[3] = {{a.hq, a.ld, (a.F + 15) / 16 * 16}, {a.go, pitch, static_cast<int>(pitch)}, {a.gr, pitch, static_cast<int>(pitch)}};
-  if (aligned16({a.gh}) && make_ring(ctx, ring, a.rows, a.F, in, a.gr ? 3 : 2, a.gamma != nullptr, &smem, &grid)) {
-    auto kern = a.F % VEC == 0 ? rmsnorm_bwd_kernel<T, VEC> : rmsnorm_bwd_kernel<T, 1>;
+  const int team = aligned16({a.gh}) ? make_ring(ctx, ring, a.rows, a.F, in, a.gr ? 3 : 2, a.gamma != nullptr, &smem, &grid) : 0;
+  if (team) {
+    void (*kern)(const Ring, const NormBwdQ8Args) = nullptr;
+#define PICK(TEAM) kern = a.F % VEC == 0 ? rmsnorm_bwd_kernel<T, VEC, TEAM> : rmsnorm_bwd_kernel<T, 1, TEAM>
+    WITH_TEAM(team, PICK)
+#undef PICK
     if (int rc = allow_ring(ctx, kern)) return rc;
     if (grad_gamma) {
       if (int rc = scratch.take(sizeof(float) * grid * static_cast<size_t>(a.F))) return rc;
