@@ -4,6 +4,7 @@
 #include "rows8_sum.cuh"
 #include "gemm8.cuh"
 #include <algorithm>
+#include <initializer_list>
 
 namespace gb {
 namespace {
@@ -99,27 +100,83 @@ __global__ void __launch_bounds__(256) linear_q8_few_kernel(const FewArgs a) {
 }
 
 // ---------------------------------------------------------------- operands of the backward pass
-// q * scale rounded to bf16, rows of ld values (what lies past the features is never read as a column)
-__global__ void __launch_bounds__(256) expand_rows_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale, __nv_bfloat16* __restrict__ y,
-                                                          long long pieces, int per_row) {
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < pieces; i += gridDim.x * 256ll) {
-    const float s = __ldg(scale + i / per_row);
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(q) + i);
-    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
-    uint32_t out[8];
+// q * scale rounded to bf16, rows of ld values (what lies past the features is never read as a column): piece i of 16 bytes
+__device__ __forceinline__ void expand_piece(const int8_t* q, float s, __nv_bfloat16* y, long long i) {
+  const uint4 w = __ldg(reinterpret_cast<const uint4*>(q) + i);
+  const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+  const F2 s2(s, s), offset(-8388736.f, -8388736.f);
+  uint32_t out[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t u = in[j] ^ 0x80808080u;
-      float v[4];
+  for (int j = 0; j < 4; ++j) {
+    // signed bytes as floats: byte + 128 below the bits of 2^23, then the offset taken off; exact
+    const uint32_t u = in[j] ^ 0x80808080u;
+    const F2 lo(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441)));
+    const F2 hi(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443)));
+    out[2 * j] = mul2(add2(lo, offset), s2).bf16();
+    out[2 * j + 1] = mul2(add2(hi, offset), s2).bf16();
+  }
+  uint4* yp = reinterpret_cast<uint4*>(y) + 2 * i;
+  yp[0] = make_uint4(out[0], out[1], out[2], out[3]);
+  yp[1] = make_uint4(out[4], out[5], out[6], out[7]);
+}
+// partial[block][n] = sum over the block's rows, V columns per thread, 256 threads across
+template <int V>
+__device__ __forceinline__ void sum_columns(const __nv_bfloat16* g, float* partial, long long M, int N, int across, int block, long long rows_per_block) {
+  const int n = (across * 256 + threadIdx.x) * V;
+  if (n >= N) return;
+  const long long r0 = block * rows_per_block, r1 = min(M, r0 + rows_per_block);
+  const __nv_bfloat16* p = g + r0 * N + n;
+  if constexpr (V == 8) {
+    F2 acc[4] = {F2(0.f, 0.f), F2(0.f, 0.f), F2(0.f, 0.f), F2(0.f, 0.f)};
+#pragma unroll 8
+    for (long long r = r0; r < r1; ++r, p += N) {
+      const uint4 t = __ldg(reinterpret_cast<const uint4*>(p));
+      const uint32_t w[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-      for (int b = 0; b < 4; ++b) v[b] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + b)) - 8388736.f) * s;
-      const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
-      out[2 * j] = *reinterpret_cast<const uint32_t*>(&lo);
-      out[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&hi);
+      for (int j = 0; j < 4; ++j) acc[j] = add2(acc[j], F2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u)));
     }
-    uint4* yp = reinterpret_cast<uint4*>(y) + 2 * i;
-    yp[0] = make_uint4(out[0], out[1], out[2], out[3]);
-    yp[1] = make_uint4(out[4], out[5], out[6], out[7]);
+    float* o = partial + static_cast<long long>(block) * N + n;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j].get(o[2 * j], o[2 * j + 1]);
+  } else {
+    float acc = 0.f;
+#pragma unroll 8
+    for (long long r = r0; r < r1; ++r, p += N) acc += __bfloat162float(*p);
+    partial[static_cast<long long>(block) * N + n] = acc;
+  }
+}
+// What the tensor-core launch reads, and the column sums beside it: the first sum_blocks * across blocks sum columns of
+// grad_out, the others expand the 8-bit rows.
+struct PrepareArgs {
+  const int8_t* q;
+  const float* scale;
+  __nv_bfloat16* x;
+  long long pieces;
+  Divisor per_row;
+  const __nv_bfloat16* g;
+  float* partial;
+  long long M, rows_per_block;
+  int N, across, sum_blocks, wide;
+};
+__global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ PrepareArgs a) {
+  const unsigned sums = a.sum_blocks * a.across;
+  if (blockIdx.x < sums) {
+    const int block = blockIdx.x / a.across, across = blockIdx.x - block * a.across;
+    if (a.wide) sum_columns<8>(a.g, a.partial, a.M, a.N, across, block, a.rows_per_block);
+    else sum_columns<1>(a.g, a.partial, a.M, a.N, across, block, a.rows_per_block);
+    return;
+  }
+  // 4 pieces per thread and turn, their loads together
+  const long long step = (gridDim.x - sums) * 1024ll;
+  for (long long base = (blockIdx.x - sums) * 1024ll + threadIdx.x; base < a.pieces; base += step) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const long long i = base + u * 256;
+      if (i < a.pieces) {
+        const long long row = a.pieces < (1ll << 31) ? a.per_row.quotient(static_cast<int>(i)) : i / a.per_row.d;
+        expand_piece(a.q, __ldg(a.scale + row), a.x, i);
+      }
+    }
   }
 }
 // rows of n bf16 values to rows of ld values, for TMA, which wants rows on 16-byte boundaries
@@ -130,32 +187,6 @@ __global__ void __launch_bounds__(256) pitch_rows_kernel(const __nv_bfloat16* __
     for (int c = lane; c < n; c += 32) y[row * ld + c] = x[row * n + c];
   }
 }
-// partial[block][n] = sum over the block's rows. V columns per thread.
-template <int V>
-__global__ void __launch_bounds__(256) column_sums_kernel(const __nv_bfloat16* __restrict__ g, float* __restrict__ partial, long long M, int N, long long rows_per_block) {
-  const int n = (blockIdx.x * 256 + threadIdx.x) * V;
-  if (n >= N) return;
-  const long long r0 = blockIdx.y * rows_per_block, r1 = min(M, r0 + rows_per_block);
-  float acc[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) acc[j] = 0.f;
-#pragma unroll 8
-  for (long long r = r0; r < r1; ++r) {
-    if constexpr (V == 8) {
-      const uint4 t = __ldg(reinterpret_cast<const uint4*>(g + r * N + n));
-      const uint32_t w[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        acc[2 * j] += __uint_as_float(w[j] << 16);
-        acc[2 * j + 1] += __uint_as_float(w[j] & 0xffff0000u);
-      }
-    } else {
-      acc[0] += __bfloat162float(g[r * N + n]);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < V; ++j) partial[static_cast<long long>(blockIdx.y) * N + n + j] = acc[j];
-}
 
 // ---------------------------------------------------------------- launches
 struct Operand {
@@ -163,38 +194,88 @@ struct Operand {
   long long ld;      // elements between rows
 };
 
-// C [M][N] of KIND over k; `a` and `b` as the kind reads them.
-template <Gemm8Kind KIND>
-int launch_gemm8(grilly_ctx* ctx, Operand oa, Operand ob, long long M, int N, long long k, Gemm8Args& g) {
+// The columns of a tile: as few of them past N as possible, then as wide as possible.
+int pick_tile_n(int N) {
+  int best = 256;
+  for (int w : {192, 128})
+    if ((N + w - 1) / w * w < (N + best - 1) / best * best) best = w;
+  return best;
+}
+
+// Geometry of C [M][N] over k. `pairs_for`: the pairs that this product may fill; parts along k until it does.
+int plan_gemm8(grilly_ctx* ctx, Gemm8Args& g, long long M, int N, long long k, int bk, int pairs_for) {
   using Cfg = Gemm8Cfg;
-  constexpr bool kInt8 = KIND == Gemm8Kind::Q8;
-  constexpr int BK = kInt8 ? 128 : 64;
   if (M > 0x7fffff00ll || k > 0x7fffff00ll || N > 0x7fffff00) return set_error(ctx, GRILLY_ERR_UNSUPPORTED, "8-bit rows: more than 2^31 - 256 rows");
-  CUtensorMap ta, tb;
+  g.M = M; g.N = N;
+  g.tile_n = pick_tile_n(N);
+  const long long tiles_m = (M + Cfg::TILE - 1) / Cfg::TILE, tiles_n = (N + g.tile_n - 1) / g.tile_n;
+  g.k_blocks = static_cast<int>((k + bk - 1) / bk);
+  const long long tiles = tiles_m * tiles_n;
+  const int want = static_cast<int>(std::max(1ll, std::min<long long>(pairs_for / tiles, g.k_blocks / 4)));
+  g.k_per_split = (g.k_blocks + want - 1) / want;
+  g.splits = (g.k_blocks + g.k_per_split - 1) / g.k_per_split;
+  if (tiles * g.splits > 0x1fffffffll) return set_error(ctx, GRILLY_ERR_UNSUPPORTED, "8-bit rows: too many tiles");
+  g.tiles_m = static_cast<int>(tiles_m);
+  g.tiles_n = static_cast<int>(tiles_n);
+  g.tile_group = 8;
+  g.by_tiles = Divisor(static_cast<uint32_t>(tiles));
+  g.by_group_tiles = Divisor(g.tile_group * g.tiles_n);
+  g.by_group = Divisor(g.tile_group);
+  g.by_last_group = Divisor(std::max(1, g.tiles_m % g.tile_group));
+  const int elt = g.out_bf16 ? 2 : 4;
+  g.wide_store = g.ld_out * elt % 16 == 0 && reinterpret_cast<uintptr_t>(g.out) % 16 == 0;
+  return GRILLY_OK;
+}
+
+// Tensor maps of one product, and where its parts go when it is split (the workspace is taken here).
+int map_gemm8(grilly_ctx* ctx, bool int8, Operand oa, Operand ob, long long k, Gemm8Args& g, Gemm8Maps& m, Rows8Scratch& ws, Gemm8Finish& f, int which) {
+  using Cfg = Gemm8Cfg;
   int rc;
-  if (kInt8) {
-    if ((rc = get_tmap_2d(ctx, TM_U8, oa.p, k, M, oa.ld, BK, 128, &ta))) return rc;
-    if ((rc = get_tmap_2d(ctx, TM_U8, ob.p, k, N, ob.ld, BK, 128, &tb))) return rc;
+  if (int8) {
+    if ((rc = get_tmap_2d(ctx, TM_U8, oa.p, k, g.M, oa.ld, 128, 128, &m.a))) return rc;
+    if ((rc = get_tmap_2d(ctx, TM_U8, ob.p, k, g.N, ob.ld, 128, g.tile_n / 2, &m.b))) return rc;
   } else {
-    if (KIND == Gemm8Kind::WGRAD) rc = get_tmap_2d(ctx, TM_BF16, oa.p, M, k, oa.ld * 2, 64, BK, &ta);
-    else rc = get_tmap_2d(ctx, TM_BF16, oa.p, k, M, oa.ld * 2, BK, 128, &ta);
+    if (g.a_across) rc = get_tmap_2d(ctx, TM_BF16, oa.p, g.M, k, oa.ld * 2, 64, 64, &m.a);
+    else rc = get_tmap_2d(ctx, TM_BF16, oa.p, k, g.M, oa.ld * 2, 64, 128, &m.a);
     if (rc) return rc;
-    if ((rc = get_tmap_2d(ctx, TM_BF16, ob.p, N, k, ob.ld * 2, 64, BK, &tb))) return rc;
+    if ((rc = get_tmap_2d(ctx, TM_BF16, ob.p, g.N, k, ob.ld * 2, 64, 64, &m.b))) return rc;
   }
-  auto kern = gemm8_pair_kernel<KIND>;
+  m.out = m.a;
+  const int elt = g.out_bf16 ? 2 : 4;
+  f.pieces[which] = 0;
+  if (g.splits == 1) {
+    // 64 bytes of 32 rows per store, cut off at the edges
+    return g.wide_store ? get_tmap_2d(ctx, g.out_bf16 ? TM_BF16 : TM_F32, g.out, g.N, g.M, g.ld_out * elt, 64 / elt, 32, &m.out, TM_SW64) : GRILLY_OK;
+  }
+  // planes of whole tiles, so that a store at the lower edge of one does not reach into the next
+  const long long ld_ws = (g.N + 3) / 4 * 4ll, plane_rows = static_cast<long long>(g.tiles_m) * Cfg::TILE;
+  if ((rc = ws.take(static_cast<size_t>(g.splits) * plane_rows * ld_ws * 4))) return rc;
+  f.job[which] = g;
+  f.ws[which] = static_cast<const uint32_t*>(ws.p);
+  f.ld_ws[which] = ld_ws;
+  f.plane[which] = plane_rows * ld_ws;
+  f.pieces[which] = g.M * (ld_ws / 4);
+  f.per_row[which] = Divisor(static_cast<uint32_t>(ld_ws / 4));
+  g.out = ws.p;
+  g.ld_out = ld_ws;
+  g.raw = g.wide_store = 1;
+  return get_tmap_2d(ctx, TM_F32, ws.p, g.N, g.splits * plane_rows, ld_ws * 4, 16, 32, &m.out, TM_SW64);
+}
+
+template <bool kInt8>
+int pairs_that_fit(grilly_ctx* ctx, cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, int* pairs) {
+  auto kern = gemm8_pair_kernel<kInt8>;
   const void* key = reinterpret_cast<const void*>(kern);
   if (!ctx->smem_attr_done.count(key)) {
-    GB_CUDA_CHECK(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES));
+    GB_CUDA_CHECK(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Gemm8Cfg::SMEM_BYTES));
     ctx->smem_attr_done.insert(key);
   }
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  attr->id = cudaLaunchAttributeClusterDimension;
+  attr->val.clusterDim.x = 2;
+  attr->val.clusterDim.y = 1;
+  attr->val.clusterDim.z = 1;
   cfg.blockDim = dim3(GEMM8_THREADS, 1, 1);
-  cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+  cfg.dynamicSmemBytes = Gemm8Cfg::SMEM_BYTES;
   cfg.stream = ctx->stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
@@ -206,54 +287,48 @@ int launch_gemm8(grilly_ctx* ctx, Operand oa, Operand ob, long long M, int N, lo
     if (n <= 0) return set_error(ctx, GRILLY_ERR_UNSUPPORTED, "8-bit rows: no CTA pair fits on this GPU");
     found = ctx->max_clusters.emplace(key, n).first;
   }
-  const int pairs = found->second;
-  const long long tiles_m = (M + Cfg::TILE - 1) / Cfg::TILE, tiles_n = (N + Cfg::TILE - 1) / Cfg::TILE;
-  if (tiles_m * tiles_n > 0x3fffffffll) return set_error(ctx, GRILLY_ERR_UNSUPPORTED, "8-bit rows: too many tiles");
-  g.M = M; g.N = N;
-  g.tiles_m = static_cast<int>(tiles_m);
-  g.tiles_n = static_cast<int>(tiles_n);
-  g.tile_group = 8;
-  g.k_blocks = static_cast<int>((k + BK - 1) / BK);
-  g.err = ctx->err_dev;
-  const int elt = g.out_bf16 ? 2 : 4;
-  // parts along k until every pair has a tile
-  const int tiles = g.tiles_m * g.tiles_n;
-  const int want = std::max(1, std::min(pairs / tiles, g.k_blocks / 4));
-  g.k_per_split = (g.k_blocks + want - 1) / want;
-  g.splits = (g.k_blocks + g.k_per_split - 1) / g.k_per_split;
-  if (static_cast<long long>(tiles) * g.splits > 0x3fffffffll) return set_error(ctx, GRILLY_ERR_UNSUPPORTED, "8-bit rows: too many tiles");
-  g.by_tiles = Divisor(tiles);
-  g.by_group_tiles = Divisor(g.tile_group * g.tiles_n);
-  g.by_group = Divisor(g.tile_group);
-  g.by_last_group = Divisor(std::max(1, g.tiles_m % g.tile_group));
-  const double bytes = (kInt8 ? 1.0 : 2.0) * (static_cast<double>(M) * k + static_cast<double>(N) * k) + static_cast<double>(M) * N * elt;
-  const int pi = prof_begin(ctx, PROF_GEMM, 2.0 * M * static_cast<double>(N) * k, bytes);
-  cfg.gridDim = dim3(2 * std::min(pairs, tiles * g.splits), 1, 1);
-  CUtensorMap to = ta;
-  g.wide_store = g.ld_out * elt % 16 == 0 && reinterpret_cast<uintptr_t>(g.out) % 16 == 0;
-  if (g.splits == 1) {
-    // 64 bytes of 32 rows per store, cut off at the edges
-    if (g.wide_store && (rc = get_tmap_2d(ctx, g.out_bf16 ? TM_BF16 : TM_F32, g.out, N, M, g.ld_out * elt, 64 / elt, 32, &to, TM_SW64))) return rc;
-    GB_CUDA_CHECK(ctx, cudaLaunchKernelEx(&cfg, kern, ta, tb, to, g));
-    ctx->launches++;
-  } else {
-    // planes of whole tiles, so that a store at the lower edge of one does not reach into the next
-    Rows8Scratch ws(ctx);
-    const long long ld_ws = (N + 3) / 4 * 4ll, plane_rows = tiles_m * Cfg::TILE;
-    if ((rc = ws.take(static_cast<size_t>(g.splits) * plane_rows * ld_ws * 4))) return rc;
-    Gemm8Args part = g;
-    part.out = ws.p;
-    part.ld_out = ld_ws;
-    part.raw = part.wide_store = 1;
-    if ((rc = get_tmap_2d(ctx, TM_F32, ws.p, N, g.splits * plane_rows, ld_ws * 4, 16, 32, &to, TM_SW64))) return rc;
-    GB_CUDA_CHECK(ctx, cudaLaunchKernelEx(&cfg, kern, ta, tb, to, part));
-    const long long pieces = M * ((N + 3) / 4);
-    gemm8_join_kernel<KIND><<<static_cast<unsigned>(std::min<long long>((pieces + 255) / 256, ctx->num_sms * 8ll)), 256, 0, ctx->stream>>>(
-        g, static_cast<const uint32_t*>(ws.p), ld_ws, plane_rows * ld_ws);
-    ctx->launches += 2;
-    GB_CUDA_CHECK(ctx, cudaGetLastError());
+  *pairs = found->second;
+  return GRILLY_OK;
+}
+
+template <bool kInt8>
+int launch_gemm8(grilly_ctx* ctx, cudaLaunchConfig_t& cfg, int pairs, const Gemm8Maps* maps, Gemm8Jobs& jobs) {
+  int items = 0;
+  double flops = 0, bytes = 0;
+  for (int j = 0; j < jobs.count; ++j) {
+    const Gemm8Args& g = jobs.job[j];
+    jobs.items[j] = g.tiles_m * g.tiles_n * g.splits;
+    items += jobs.items[j];
+    const double k = static_cast<double>(g.k_blocks) * (kInt8 ? 128 : 64);
+    flops += 2.0 * g.M * g.N * k;
+    bytes += (kInt8 ? 1.0 : 2.0) * (static_cast<double>(g.M) + g.N) * k + static_cast<double>(g.M) * g.N * (g.out_bf16 ? 2 : 4);
   }
+  const int P = std::min(pairs, items);
+  jobs.ahead_from = jobs.items[0] % P;
+  jobs.ahead = 0;
+  if (jobs.count > 1 && jobs.ahead_from) {
+    const int late = P - jobs.ahead_from;
+    jobs.ahead = std::min(jobs.job[0].k_per_split / jobs.job[1].k_per_split, jobs.items[1] / late);
+  }
+  jobs.err = ctx->err_dev;
+  cfg.gridDim = dim3(2 * P, 1, 1);
+  const int pi = prof_begin(ctx, PROF_GEMM, flops, bytes);
+  GB_CUDA_CHECK(ctx, cudaLaunchKernelEx(&cfg, gemm8_pair_kernel<kInt8>, maps[0], maps[jobs.count - 1], jobs));
   prof_end(ctx, pi);
+  ctx->launches++;
+  return GRILLY_OK;
+}
+
+// The second launch: parts joined, column sums totalled; nothing where neither is there.
+template <bool kInt8>
+int launch_finish(grilly_ctx* ctx, Gemm8Finish& f) {
+  const long long pieces = std::max(f.pieces[0], f.pieces[1]);
+  f.sum_at = static_cast<unsigned>(std::min<long long>((pieces + 511) / 512, ctx->num_sms * 4ll));
+  const unsigned grid = f.sum_at + (f.sums ? (f.F + 31) / 32 : 0);
+  if (!grid) return GRILLY_OK;
+  gemm8_finish_kernel<kInt8><<<grid, 512, 0, ctx->stream>>>(f);
+  ctx->launches++;
+  GB_CUDA_CHECK(ctx, cudaGetLastError());
   return GRILLY_OK;
 }
 
@@ -275,22 +350,6 @@ int tma_rows(grilly_ctx* ctx, const void* x, long long rows, int n, Rows8Scratch
   ctx->launches++;
   GB_CUDA_CHECK(ctx, cudaGetLastError());
   *out = {scratch.p, ld};
-  return GRILLY_OK;
-}
-
-int column_sums(grilly_ctx* ctx, const __nv_bfloat16* g, float* out, long long M, int N) {
-  const bool wide = N % 8 == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
-  const int across = wide ? (N / 8 + 255) / 256 : (N + 255) / 256;
-  const int blocks = static_cast<int>(std::max<long long>(1, std::min<long long>((M + 31) / 32, ctx->num_sms * 6ll / across)));
-  const long long per = (M + blocks - 1) / blocks;
-  Rows8Scratch ws(ctx);
-  if (int rc = ws.take(sizeof(float) * static_cast<size_t>(blocks) * N)) return rc;
-  float* partial = static_cast<float*>(ws.p);
-  if (wide) column_sums_kernel<8><<<dim3(across, blocks), 256, 0, ctx->stream>>>(g, partial, M, N, per);
-  else column_sums_kernel<1><<<dim3(across, blocks), 256, 0, ctx->stream>>>(g, partial, M, N, per);
-  sum_partials_kernel<<<(N + 31) / 32, 512, 0, ctx->stream>>>(partial, out, blocks, N);
-  ctx->launches += 2;
-  GB_CUDA_CHECK(ctx, cudaGetLastError());
   return GRILLY_OK;
 }
 
@@ -323,10 +382,22 @@ int grilly_linear_q8(grilly_ctx* ctx, const void* xq, const float* xs, const voi
       GB_CUDA_CHECK(ctx, cudaGetLastError());
       return GRILLY_OK;
     }
-    Gemm8Args g{};
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    int pairs = 0, rc;
+    if ((rc = pairs_that_fit<true>(ctx, cfg, &attr, &pairs))) return rc;
+    Gemm8Jobs jobs{};
+    Gemm8Maps maps;
+    Gemm8Finish finish{};
+    Rows8Scratch parts(ctx);
+    jobs.count = 1;
+    Gemm8Args& g = jobs.job[0];
     g.out = y; g.ld_out = N; g.out_bf16 = out_bf16;
     g.row_scale = xs; g.col_scale = ws; g.bias = bias; g.act = act;
-    return launch_gemm8<Gemm8Kind::Q8>(ctx, {xq, ldx}, {wq, ldw}, M, N, K, g);
+    if ((rc = plan_gemm8(ctx, g, M, N, K, 128, pairs))) return rc;
+    if ((rc = map_gemm8(ctx, true, {xq, ldx}, {wq, ldw}, K, g, maps, parts, finish, 0))) return rc;
+    if ((rc = launch_gemm8<true>(ctx, cfg, pairs, &maps, jobs))) return rc;
+    return launch_finish<true>(ctx, finish);
   });
 }
 
@@ -343,28 +414,72 @@ int grilly_linear_backward_q8(grilly_ctx* ctx, const void* go, const void* xq, c
       if (gbias) GB_CUDA_CHECK(ctx, cudaMemsetAsync(gbias, 0, sizeof(float) * N, ctx->stream));
       return GRILLY_OK;
     }
-    int rc;
-    Operand g{}, weights{};
-    Rows8Scratch g_rows(ctx), w_rows(ctx), x_rows(ctx);
-    if ((gx || gw) && (rc = tma_rows(ctx, go, M, N, g_rows, &g))) return rc;
-    if (gx) {
-      if ((rc = tma_rows(ctx, w, N, K, w_rows, &weights))) return rc;
-      Gemm8Args a{};
-      a.out = gx; a.ld_out = K; a.out_bf16 = bf16;
-      if ((rc = launch_gemm8<Gemm8Kind::DGRAD>(ctx, g, weights, M, K, N, a))) return rc;
+    int rc, pairs = 0;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    if ((rc = pairs_that_fit<false>(ctx, cfg, &attr, &pairs))) return rc;
+    Rows8Scratch g_rows(ctx), w_rows(ctx), x_rows(ctx), sums(ctx), parts_w(ctx), parts_x(ctx);
+    Gemm8Finish finish{};
+    // the checkpoint as bf16 rows, and the column sums of grad_out by blocks of rows
+    PrepareArgs p{};
+    p.per_row = Divisor(1);
+    unsigned blocks = 0;
+    if (gbias) {
+      p.g = static_cast<const __nv_bfloat16*>(go);
+      p.M = M;
+      p.N = N;
+      p.wide = N % 8 == 0 && (reinterpret_cast<uintptr_t>(go) & 15) == 0;
+      p.across = p.wide ? (N / 8 + 255) / 256 : (N + 255) / 256;
+      p.sum_blocks = static_cast<int>(std::max<long long>(1, std::min<long long>((M + 31) / 32, ctx->num_sms * 6ll / p.across)));
+      p.rows_per_block = (M + p.sum_blocks - 1) / p.sum_blocks;
+      if ((rc = sums.take(sizeof(float) * static_cast<size_t>(p.sum_blocks) * N))) return rc;
+      p.partial = static_cast<float*>(sums.p);
+      blocks = p.across * p.sum_blocks;
+      finish.partial = p.partial;
+      finish.sums = gbias;
+      finish.blocks = p.sum_blocks;
+      finish.F = N;
     }
     if (gw) {
       if ((rc = x_rows.take(static_cast<size_t>(M) * ldx * 2))) return rc;
-      const long long pieces = M * (ldx / 16);
-      expand_rows_kernel<<<static_cast<unsigned>(std::min<long long>((pieces + 255) / 256, ctx->num_sms * 32ll)), 256, 0, ctx->stream>>>(
-          static_cast<const int8_t*>(xq), xs, static_cast<__nv_bfloat16*>(x_rows.p), pieces, static_cast<int>(ldx / 16));
-      ctx->launches++;
-      Gemm8Args a{};
-      a.out = gw; a.ld_out = K; a.out_bf16 = bf16;
-      if ((rc = launch_gemm8<Gemm8Kind::WGRAD>(ctx, g, {x_rows.p, ldx}, N, K, M, a))) return rc;
+      p.q = static_cast<const int8_t*>(xq);
+      p.scale = xs;
+      p.x = static_cast<__nv_bfloat16*>(x_rows.p);
+      p.pieces = M * (ldx / 16);
+      p.per_row = Divisor(static_cast<uint32_t>(ldx / 16));
+      blocks += static_cast<unsigned>(std::min<long long>((p.pieces + 1023) / 1024, ctx->num_sms * 16ll));
     }
-    if (gbias && (rc = column_sums(ctx, static_cast<const __nv_bfloat16*>(go), gbias, M, N))) return rc;
-    return GRILLY_OK;
+    if (blocks) {
+      const int pi = prof_begin(ctx, PROF_OTHER, 0.0, (gw ? 3.0 * M * K : 0.0) + (gbias ? 2.0 * M * N : 0.0));
+      prepare_kernel<<<blocks, 256, 0, ctx->stream>>>(p);
+      prof_end(ctx, pi);
+      ctx->launches++;
+      GB_CUDA_CHECK(ctx, cudaGetLastError());
+    }
+    // both products in one launch, the one with the longer sums first
+    if (gx || gw) {
+      Operand g{}, weights{};
+      if ((rc = tma_rows(ctx, go, M, N, g_rows, &g))) return rc;
+      if (gx && (rc = tma_rows(ctx, w, N, K, w_rows, &weights))) return rc;
+      Gemm8Jobs jobs{};
+      Gemm8Maps maps[2];
+      const bool w_first = gw && (!gx || M >= N);
+      for (int j = 0; j < 2; ++j) {
+        const bool is_w = (j == 0) == w_first;
+        if (is_w ? !gw : !gx) continue;
+        const int at = jobs.count++;
+        Gemm8Args& a = jobs.job[at];
+        a.out = is_w ? gw : gx;
+        a.ld_out = K;
+        a.out_bf16 = bf16;
+        a.a_across = is_w;
+        const long long k = is_w ? M : N;
+        if ((rc = plan_gemm8(ctx, a, is_w ? N : M, K, k, 64, pairs))) return rc;
+        if ((rc = map_gemm8(ctx, false, g, is_w ? Operand{x_rows.p, ldx} : weights, k, a, maps[at], is_w ? parts_w : parts_x, finish, at))) return rc;
+      }
+      if ((rc = launch_gemm8<false>(ctx, cfg, pairs, maps, jobs))) return rc;
+    }
+    return launch_finish<false>(ctx, finish);
   });
 }
 

@@ -1,11 +1,12 @@
 // Matrix products of the 8-bit row operators on the tensor cores: C[M][N] = epilogue(sum over k of A(m, k) B(n, k)).
 //
-//   Gemm8Kind::Q8      A = x_q [M][K], B = W_q [N][K], int8 along k (kind::i8, exact int32 sums): linear_q8
-//   Gemm8Kind::DGRAD   A = grad_out [M][k] along k, B = W [k][N] across k (bf16, fp32 sums): grad_x = grad_out W
-//   Gemm8Kind::WGRAD   A = grad_out [k][M], B = x [k][N], both across k (bf16): grad_W = grad_out^T x
+//   linear_q8            A = x_q [M][K], B = W_q [N][K], int8 along k (kind::i8, exact int32 sums)
+//   linear_backward_q8   two products in one launch, bf16 with fp32 sums:
+//     grad_x = grad_out W       A = grad_out [M][k] along k, B = W [k][N] across k
+//     grad_W = grad_out^T x     A = grad_out [k][M], B = x [k][N], both across k
 //
-// A pair of CTAs shares one tcgen05.mma (cta_group::2): a 256 x 256 tile of C, of which each CTA loads 128 rows of A and
-// 128 of B per k-block of 128 bytes and keeps 128 rows of the accumulator in its own tensor memory, twice, so that one
+// A pair of CTAs shares one tcgen05.mma (cta_group::2): a 256 x 256 tile of C (256 x 192 or 256 x 128 where that leaves less
+// of the last column block empty), of which each CTA loads half the rows of A and half of B per k-block of 128 bytes and keeps 128 rows of the accumulator in its own tensor memory, twice, so that one
 // tile is written while the next is computed. Roles per CTA: warp 0 TMA producer (own halves, bytes counted on the
 // leader's barrier), warp 1 MMA issuer (leader) and TMEM allocation, 16 epilogue warps, and for Q8 one warp that brings
 // the next tile's column scales and bias into shared memory (left to the epilogue warps, each tile waited twice for L2).
@@ -16,12 +17,11 @@
 #pragma once
 #include "ptx.cuh"
 #include "f32x2.cuh"
+#include "rows8_sum.cuh"
 #include "../../include/grilly_b200.h"
 #include <cuda_bf16.h>
 
 namespace gb {
-
-enum class Gemm8Kind { Q8, DGRAD, WGRAD };
 
 // Division of 0 <= n < 2^31 by a number the host knows: n * m >> s with s = 31 + ceil(log2 d), m = floor(2^s / d) + 1. The
 // error of m is at most 2^-31 of a quotient step for every such n, so the quotient is exact (Granlund and Montgomery).
@@ -35,9 +35,12 @@ struct Divisor {
   __device__ __forceinline__ int quotient(int n) const { return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * m) >> s); }
 };
 
+// One product of a launch.
 struct Gemm8Args {
   long long M;
   int N;
+  int a_across;               // bf16: A lies across k
+  int tile_n;                 // columns of a tile
   int tiles_m, tiles_n, tile_group, k_blocks;
   int splits, k_per_split;    // k-blocks per part
   Divisor by_tiles, by_group_tiles, by_group, by_last_group;   // tiles, group * tiles_n, group, tiles_m % group (or 1)
@@ -50,7 +53,37 @@ struct Gemm8Args {
   const float* col_scale;
   const float* bias;
   int act;
+};
+struct Gemm8Maps {
+  CUtensorMap a, b, out;
+};
+// The products of a launch and how the pairs share them: pair p of P takes the items (tile and part of k) p, p + P, ... of
+// the first, then items of the second. Where the first does not divide evenly, the pairs from ahead_from on are one item
+// short and take `ahead` items more of the second (the first's items are the longer ones).
+struct Gemm8Jobs {
+  Gemm8Args job[2];
+  int count, items[2];
+  int ahead_from, ahead;
   int* err;
+};
+struct Gemm8Walk {
+  int p, P, first, j;
+  __device__ Gemm8Walk(int pair, int pairs) : p(pair), P(pairs), first(pair), j(0) {}
+  __device__ __forceinline__ bool next(const Gemm8Jobs& jobs, int& job, int& item) {
+    if (first < jobs.items[0]) {
+      job = 0;
+      item = first;
+      first += P;
+      return true;
+    }
+    if (jobs.count < 2) return false;
+    const int late = P - jobs.ahead_from, before = jobs.ahead * late;
+    job = 1;
+    if (p >= jobs.ahead_from) item = j < jobs.ahead ? j * late + p - jobs.ahead_from : before + (j - jobs.ahead) * P + p;
+    else item = before + j * P + p;
+    ++j;
+    return item < jobs.items[1];
+  }
 };
 
 constexpr int GEMM8_EPI_WARPS = 16;
@@ -117,28 +150,26 @@ __device__ __forceinline__ void gemm8_tile(const Gemm8Args& a, int tile, int& m,
 }
 
 // One warp writes 32 rows x 32 columns of C. r: the lane's row, 32 neighbouring columns, as raw sums (int32 for Q8).
-// Q8: times the row's scale, times the column's scale plus bias (shared memory, the same address in every lane), activation.
+// int8: times the row's scale, times the column's scale plus bias (shared memory, the same address in every lane), activation.
 // The values go to the warp's 2 KB of shared memory as rows of 64 bytes (32 columns of bf16, or 16 of fp32 twice) whose
 // 16-byte pieces are exchanged as TMA's 64-byte swizzle does, so neither side has bank conflicts, and one TMA store takes
 // them out, cut off at the edges of C. Where C's rows are not on 16-byte boundaries the lanes store them themselves.
-template <Gemm8Kind KIND, int ACT>
+template <int ACT>
 __device__ __forceinline__ void gemm8_finish(uint32_t (&r)[32], float rs, const float* cs, const float* bias) {
-  if constexpr (KIND == Gemm8Kind::Q8) {
-    const F2 rs2(rs, rs);
+  const F2 rs2(rs, rs);
 #pragma unroll
-    for (int j = 0; j < 32; j += 4) {
-      const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(cs + j), d = *reinterpret_cast<const ulonglong2*>(bias + j);
+  for (int j = 0; j < 32; j += 4) {
+    const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(cs + j), d = *reinterpret_cast<const ulonglong2*>(bias + j);
 #pragma unroll
-      for (int i = 0; i < 4; i += 2) {
-        F2 c2, d2;
-        c2.v = i ? c.y : c.x;
-        d2.v = i ? d.y : d.x;
-        const F2 v(static_cast<float>(static_cast<int>(r[j + i])), static_cast<float>(static_cast<int>(r[j + i + 1])));
-        float a, b;
-        gemm8_act2<ACT>(fma2(mul2(v, rs2), c2, d2)).get(a, b);
-        r[j + i] = __float_as_uint(a);
-        r[j + i + 1] = __float_as_uint(b);
-      }
+    for (int i = 0; i < 4; i += 2) {
+      F2 c2, d2;
+      c2.v = i ? c.y : c.x;
+      d2.v = i ? d.y : d.x;
+      const F2 v(static_cast<float>(static_cast<int>(r[j + i])), static_cast<float>(static_cast<int>(r[j + i + 1])));
+      float a, b;
+      gemm8_act2<ACT>(fma2(mul2(v, rs2), c2, d2)).get(a, b);
+      r[j + i] = __float_as_uint(a);
+      r[j + i + 1] = __float_as_uint(b);
     }
   }
 }
@@ -212,17 +243,14 @@ __host__ __device__ constexpr uint32_t make_idesc_i8(int m, int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-template <Gemm8Kind KIND>
+template <bool kInt8>
 __global__ void __launch_bounds__(GEMM8_THREADS, 1)
-gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-                  const __grid_constant__ CUtensorMap tmap_out, const Gemm8Args args) {
+gemm8_pair_kernel(const __grid_constant__ Gemm8Maps maps0, const __grid_constant__ Gemm8Maps maps1, const __grid_constant__ Gemm8Jobs jobs) {
   using Cfg = Gemm8Cfg;
   constexpr int STAGES = Cfg::STAGES;
-  constexpr bool kInt8 = KIND == Gemm8Kind::Q8, kAMn = KIND == Gemm8Kind::WGRAD, kBMn = KIND != Gemm8Kind::Q8;
   constexpr int BK = kInt8 ? 128 : 64;                         // k per stage
   constexpr int KSTEPS = 4;                                    // instructions per stage, 32 bytes of k each
-  constexpr uint32_t MN_STEP = 16 * 128;                       // bytes of an operand across k per instruction
-  constexpr uint32_t IDESC = kInt8 ? make_idesc_i8(256, 256) : make_idesc(true, 256, 256, kAMn, kBMn);
+  constexpr uint32_t ACROSS_STEP = 16 * 128;                   // bytes of an operand across k per instruction
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -241,7 +269,6 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
   const uint32_t rank = cluster_ctarank();                     // 0 = leader
   const bool leader = rank == 0;
   const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
-  const int tiles = args.tiles_m * args.tiles_n, items = tiles * args.splits;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -256,9 +283,9 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     }
     *abort_flag = 0;
     fence_mbar_init();
-    prefetch_tmap(&tmap_a);
-    prefetch_tmap(&tmap_b);
-    if (args.wide_store) prefetch_tmap(&tmap_out);
+    prefetch_tmap(&maps0.a);
+    prefetch_tmap(&maps0.b);
+    prefetch_tmap(&maps0.out);
   }
   if (warp == 1) {
     tmem_alloc_pair(tmem_holder, Cfg::TMEM_COLS);
@@ -272,16 +299,20 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
 
   // a failed wait stops both CTAs: the peer's waits poll its own flag
   auto fail = [&](int code) {
-    if (!*abort_flag) atomicCAS(args.err, 0, code);
+    if (!*abort_flag) atomicCAS(jobs.err, 0, code);
     *abort_flag = 1;
     st_cluster_u32(map_to_cta(const_cast<int*>(abort_flag), rank ^ 1u), 1u);
   };
-  auto k_range = [&](int item, int& k0, int& k1) {
-    const int part = args.by_tiles.quotient(item);
-    k0 = part * args.k_per_split;
-    k1 = min(args.k_blocks, k0 + args.k_per_split);
-    return item - part * tiles;
+  // tile and k-blocks of an item
+  auto place = [&](const Gemm8Args& a, int item, int& tm, int& tn, int& k0, int& k1) {
+    const int part = a.by_tiles.quotient(item);
+    gemm8_tile(a, item - part * static_cast<int>(a.by_tiles.d), tm, tn);
+    k0 = part * a.k_per_split;
+    k1 = min(a.k_blocks, k0 + a.k_per_split);
+    return part;
   };
+  Gemm8Walk walk(pair, num_pairs);
+  int job, item;
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (both CTAs, own halves)
@@ -289,29 +320,32 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int item = pair; item < items && ok; item += num_pairs) {
-        int k0, k1;
-        int tm, tn;
-        gemm8_tile(args, k_range(item, k0, k1), tm, tn);
-        const int a_row = tm * Cfg::TILE + static_cast<int>(rank) * 128;
-        const int b_row = tn * Cfg::TILE + static_cast<int>(rank) * 128;
+      while (ok && walk.next(jobs, job, item)) {
+        const Gemm8Args& a = jobs.job[job];
+        const Gemm8Maps& m = job ? maps1 : maps0;
+        int tm, tn, k0, k1;
+        place(a, item, tm, tn, k0, k1);
+        const int half_n = a.tile_n / 2;
+        const int a_row = tm * Cfg::TILE + static_cast<int>(rank) * 128, b_row = tn * a.tile_n + static_cast<int>(rank) * half_n;
+        // bytes of both CTAs: A's 128 rows, and B's rows (along k) or its columns in boxes of 64 (across k)
+        const uint32_t bytes = 2 * (Cfg::HALF_BYTES + (kInt8 ? half_n : (half_n + 63) / 64 * 64) * 128);
         for (int kb = k0; kb < k1; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) { fail(ERR_WAIT_EMPTY); ok = false; break; }
           uint8_t* sa = smem + stage * Cfg::STAGE_BYTES;
           uint8_t* sb = sa + Cfg::HALF_BYTES;
-          if (leader) mbar_expect_tx(&full_bar[stage], 2 * Cfg::STAGE_BYTES);   // both CTAs' bytes land on this barrier
+          if (leader) mbar_expect_tx(&full_bar[stage], bytes);   // both CTAs' bytes land on this barrier
           const uint32_t bar = map_to_cta(&full_bar[stage], 0);
-          if constexpr (kAMn) {
-            tma_load_2d_pair(sa, &tmap_a, bar, a_row, kb * BK);
-            tma_load_2d_pair(sa + Cfg::HALF_BYTES / 2, &tmap_a, bar, a_row + 64, kb * BK);
+          if (!kInt8 && a.a_across) {
+            tma_load_2d_pair(sa, &m.a, bar, a_row, kb * BK);
+            tma_load_2d_pair(sa + Cfg::HALF_BYTES / 2, &m.a, bar, a_row + 64, kb * BK);
           } else {
-            tma_load_2d_pair(sa, &tmap_a, bar, kb * BK, a_row);
+            tma_load_2d_pair(sa, &m.a, bar, kb * BK, a_row);
           }
-          if constexpr (kBMn) {
-            tma_load_2d_pair(sb, &tmap_b, bar, b_row, kb * BK);
-            tma_load_2d_pair(sb + Cfg::HALF_BYTES / 2, &tmap_b, bar, b_row + 64, kb * BK);
+          if constexpr (kInt8) {
+            tma_load_2d_pair(sb, &m.b, bar, kb * BK, b_row);
           } else {
-            tma_load_2d_pair(sb, &tmap_b, bar, kb * BK, b_row);
+            tma_load_2d_pair(sb, &m.b, bar, b_row, kb * BK);
+            if (half_n > 64) tma_load_2d_pair(sb + Cfg::HALF_BYTES / 2, &m.b, bar, b_row + 64, kb * BK);
           }
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
         }
@@ -325,16 +359,20 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
       int it = 0;
       bool ok = true;
       const uint32_t base = smem_u32(smem);
-      const uint64_t a0 = kAMn ? make_smem_desc_mn<true>(base, Cfg::HALF_BYTES / 2) : make_smem_desc_sw128(base, 16, 1024);
-      const uint64_t b0 = kBMn ? make_smem_desc_mn<true>(base + Cfg::HALF_BYTES, Cfg::HALF_BYTES / 2) : make_smem_desc_sw128(base + Cfg::HALF_BYTES, 16, 1024);
-      const uint32_t a_lo0 = static_cast<uint32_t>(a0), b_lo0 = static_cast<uint32_t>(b0);
-      const uint64_t a_hi = a0 & 0xffffffff00000000ull, b_hi = b0 & 0xffffffff00000000ull;
-      constexpr uint32_t A_STEP = (kAMn ? MN_STEP : 32) >> 4, B_STEP = (kBMn ? MN_STEP : 32) >> 4;
+      const uint64_t along_a = make_smem_desc_sw128(base, 16, 1024), along_b = make_smem_desc_sw128(base + Cfg::HALF_BYTES, 16, 1024);
+      const uint64_t across_a = make_smem_desc_mn<true>(base, Cfg::HALF_BYTES / 2), across_b = make_smem_desc_mn<true>(base + Cfg::HALF_BYTES, Cfg::HALF_BYTES / 2);
       const uint32_t peer_empty0 = map_to_cta(&empty_bar[0], 1), own_empty0 = map_to_cta(&empty_bar[0], 0);
       const uint32_t peer_tfull0 = map_to_cta(&tmem_full[0], 1), own_tfull0 = map_to_cta(&tmem_full[0], 0);
-      for (int item = pair; item < items && ok; item += num_pairs, ++it) {
-        int k0, k1;
-        k_range(item, k0, k1);
+      for (; ok && walk.next(jobs, job, item); ++it) {
+        const Gemm8Args& a = jobs.job[job];
+        const int k0 = a.by_tiles.quotient(item) * a.k_per_split, k1 = min(a.k_blocks, k0 + a.k_per_split);
+        const bool a_across = !kInt8 && a.a_across;
+        const uint64_t a0 = a_across ? across_a : along_a, b0 = kInt8 ? along_b : across_b;
+        const uint32_t a_step = (a_across ? ACROSS_STEP : 32) >> 4;
+        constexpr uint32_t B_STEP = (kInt8 ? 32 : ACROSS_STEP) >> 4;
+        const uint32_t a_lo0 = static_cast<uint32_t>(a0), b_lo0 = static_cast<uint32_t>(b0);
+        const uint64_t a_hi = a0 & 0xffffffff00000000ull, b_hi = b0 & 0xffffffff00000000ull;
+        const uint32_t idesc = kInt8 ? make_idesc_i8(256, a.tile_n) : make_idesc(true, 256, a.tile_n, a_across, true);
         const int acc = it & 1;
         if (!mbar_wait(&tmem_empty[acc], ((it >> 1) & 1u) ^ 1u, abort_flag)) { fail(ERR_WAIT_TMEM_EMPTY); break; }
         tc_fence_after();
@@ -345,10 +383,10 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
           const uint32_t a_lo = a_lo0 + stage * (Cfg::STAGE_BYTES >> 4), b_lo = b_lo0 + stage * (Cfg::STAGE_BYTES >> 4);
 #pragma unroll
           for (int ks = 0; ks < KSTEPS; ++ks) {
-            const uint64_t ad = a_hi | (a_lo + ks * A_STEP), bd = b_hi | (b_lo + ks * B_STEP);
+            const uint64_t ad = a_hi | (a_lo + ks * a_step), bd = b_hi | (b_lo + ks * B_STEP);
             const uint32_t more = (kb > k0 || ks > 0) ? 1u : 0u;
-            if constexpr (kInt8) umma_i8_pair(d_tmem, ad, bd, IDESC, more);
-            else umma_ss_pair<true>(d_tmem, ad, bd, IDESC, more);
+            if constexpr (kInt8) umma_i8_pair(d_tmem, ad, bd, idesc, more);
+            else umma_ss_pair<true>(d_tmem, ad, bd, idesc, more);
           }
           umma_commit_pair(own_empty0 + stage * 8);            // the stage is free in both CTAs once these have read it
           umma_commit_pair(peer_empty0 + stage * 8);
@@ -362,17 +400,17 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     }
   } else if (warp == GEMM8_PARAM_WARP) {
     // ------------------------------------------------------------ column scales and bias of the tiles, one tile ahead
-    if constexpr (KIND == Gemm8Kind::Q8) {
+    if constexpr (kInt8) {
+      const Gemm8Args& args = jobs.job[0];
       if (!args.raw) {
-        int it = 0;
-        for (int item = pair; item < items; item += num_pairs, ++it) {
+        for (int it = 0; walk.next(jobs, job, item); ++it) {
           const int buf = it & 1;
           int tm, tn;
           gemm8_tile(args, item, tm, tn);
           float c[Cfg::TILE / 32], d[Cfg::TILE / 32];
 #pragma unroll
           for (int j = 0; j < Cfg::TILE / 32; ++j) {
-            const int col = tn * Cfg::TILE + j * 32 + lane;
+            const int col = tn * args.tile_n + j * 32 + lane;
             c[j] = col < args.N ? __ldg(args.col_scale + col) : 0.f;
             d[j] = (col < args.N && args.bias) ? __ldg(args.bias + col) : 0.f;
           }
@@ -390,30 +428,30 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     }
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs, own 128 rows of the tile)
-    constexpr int NCHUNK = Cfg::TILE / 32, G = GEMM8_EPI_WARPS / 4, PER_WARP = NCHUNK / G;
+    constexpr int G = GEMM8_EPI_WARPS / 4, PER_WARP = Cfg::TILE / 32 / G;
     const int quad = warp & 3, group = (warp - 2) >> 2;
     uint8_t* stage = epi + (warp - 2) * Cfg::EPI_BYTES;
     const uint32_t leader_tempty0 = map_to_cta(&tmem_empty[0], 0);
-    const bool scaled = KIND == Gemm8Kind::Q8 && !args.raw;
+    const bool scaled = kInt8 && !jobs.job[0].raw;
     // the rows' scales are read one tile ahead
     auto row_of = [&](int tm) { return static_cast<long long>(tm) * Cfg::TILE + static_cast<int>(rank) * 128 + quad * 32; };
-    auto row_scale = [&](int item) {
+    auto row_scale = [&](int at) {
       int tm, tn;
-      if (!scaled || item >= items) return 0.f;
-      gemm8_tile(args, item, tm, tn);
+      if (!scaled || at >= jobs.items[0]) return 0.f;
+      gemm8_tile(jobs.job[0], at, tm, tn);
       const long long row = row_of(tm) + lane;
-      return row < args.M ? __ldg(args.row_scale + row) : 0.f;
+      return row < jobs.job[0].M ? __ldg(jobs.job[0].row_scale + row) : 0.f;
     };
     float rs = row_scale(pair);
-    int it = 0;
-    for (int item = pair; item < items; item += num_pairs, ++it) {
-      const int part = args.by_tiles.quotient(item);
-      int tm, tn;
-      gemm8_tile(args, item - part * tiles, tm, tn);
+    for (int it = 0; walk.next(jobs, job, item); ++it) {
+      const Gemm8Args& args = jobs.job[job];
+      const CUtensorMap* tmap_out = job ? &maps1.out : &maps0.out;
+      int tm, tn, k0, k1;
+      const int part = place(args, item, tm, tn, k0, k1);
       const long long row0 = row_of(tm);
-      const int first_col = tn * Cfg::TILE;
+      const int first_col = tn * args.tile_n;
       const int out_row = static_cast<int>(row0) + (args.raw ? part * args.tiles_m * Cfg::TILE : 0);
-      const int chunks = row0 >= args.M ? 0 : min(NCHUNK, (args.N - first_col + 31) / 32);   // warp-uniform
+      const int chunks = row0 >= args.M ? 0 : min(args.tile_n / 32, (args.N - first_col + 31) / 32);   // warp-uniform
       const float rs_next = row_scale(item + num_pairs);
       const int acc = it & 1;
       const float* p = params + acc * Cfg::PARAM_FLOATS;
@@ -432,13 +470,13 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
           if (scaled) {
             const float* cs = p + c * 32;
             switch (args.act) {
-              case GRILLY_ACT_GELU: gemm8_finish<KIND, GRILLY_ACT_GELU>(r, rs, cs, cs + Cfg::TILE); break;
-              case GRILLY_ACT_SILU: gemm8_finish<KIND, GRILLY_ACT_SILU>(r, rs, cs, cs + Cfg::TILE); break;
-              case GRILLY_ACT_RELU: gemm8_finish<KIND, GRILLY_ACT_RELU>(r, rs, cs, cs + Cfg::TILE); break;
-              default: gemm8_finish<KIND, GRILLY_ACT_NONE>(r, rs, cs, cs + Cfg::TILE);
+              case GRILLY_ACT_GELU: gemm8_finish<GRILLY_ACT_GELU>(r, rs, cs, cs + Cfg::TILE); break;
+              case GRILLY_ACT_SILU: gemm8_finish<GRILLY_ACT_SILU>(r, rs, cs, cs + Cfg::TILE); break;
+              case GRILLY_ACT_RELU: gemm8_finish<GRILLY_ACT_RELU>(r, rs, cs, cs + Cfg::TILE); break;
+              default: gemm8_finish<GRILLY_ACT_NONE>(r, rs, cs, cs + Cfg::TILE);
             }
           }
-          gemm8_write(args, &tmap_out, r, stage, row0, out_row, first_col + c * 32, lane);
+          gemm8_write(args, tmap_out, r, stage, row0, out_row, first_col + c * 32, lane);
         }
       }
       tc_fence_before();
@@ -463,53 +501,72 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
   if (warp == 1) tmem_dealloc_pair(tmem_base, Cfg::TMEM_COLS);
 }
 
-// Adds the parts of a product split along k, in order, and applies the epilogue. Four columns per thread.
-template <Gemm8Kind KIND>
-__global__ void __launch_bounds__(256) gemm8_join_kernel(const Gemm8Args a, const uint32_t* __restrict__ ws, long long ld_ws, long long plane) {
-  const int per_row = (a.N + 3) / 4;
-  const long long total = a.M * per_row;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const long long row = i / per_row;
-    const int col = static_cast<int>(i - row * per_row) * 4;
-    const uint4* src = reinterpret_cast<const uint4*>(ws + row * ld_ws + col);
-    float v[4];
-    if constexpr (KIND == Gemm8Kind::Q8) {
-      int s[4] = {0, 0, 0, 0};
+// Adds the parts of a product split along k, in order, and applies the epilogue to 4 columns.
+template <bool kInt8>
+__device__ __forceinline__ void gemm8_join(const Gemm8Args& a, const uint32_t* ws, long long ld_ws, long long plane, long long row, int col) {
+  const uint4* src = reinterpret_cast<const uint4*>(ws + row * ld_ws + col);
+  float v[4];
+  if constexpr (kInt8) {
+    int s[4] = {0, 0, 0, 0};
 #pragma unroll 4
-      for (int p = 0; p < a.splits; ++p) {
-        const uint4 t = __ldg(src + p * (plane / 4));
-        s[0] += static_cast<int>(t.x); s[1] += static_cast<int>(t.y); s[2] += static_cast<int>(t.z); s[3] += static_cast<int>(t.w);
-      }
-      const float rs = __ldg(a.row_scale + row);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool in = col + j < a.N;
-        v[j] = gemm8_act(fmaf(static_cast<float>(s[j]) * rs, in ? __ldg(a.col_scale + col + j) : 0.f, (in && a.bias) ? __ldg(a.bias + col + j) : 0.f), a.act);
-      }
-    } else {
-      v[0] = v[1] = v[2] = v[3] = 0.f;
-#pragma unroll 4
-      for (int p = 0; p < a.splits; ++p) {
-        const uint4 t = __ldg(src + p * (plane / 4));
-        v[0] += __uint_as_float(t.x); v[1] += __uint_as_float(t.y); v[2] += __uint_as_float(t.z); v[3] += __uint_as_float(t.w);
-      }
+    for (int p = 0; p < a.splits; ++p) {
+      const uint4 t = __ldg(src + p * (plane / 4));
+      s[0] += static_cast<int>(t.x); s[1] += static_cast<int>(t.y); s[2] += static_cast<int>(t.z); s[3] += static_cast<int>(t.w);
     }
-    const long long at = row * a.ld_out + col;
-    if (a.wide_store && col + 4 <= a.N) {
-      if (a.out_bf16) {
-        const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
-        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-      } else {
-        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
-      }
-      continue;
-    }
+    const float rs = __ldg(a.row_scale + row);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (col + j < a.N) {
-        if (a.out_bf16) static_cast<__nv_bfloat16*>(a.out)[at + j] = __float2bfloat16(v[j]);
-        else static_cast<float*>(a.out)[at + j] = v[j];
-      }
+      const bool in = col + j < a.N;
+      v[j] = gemm8_act(fmaf(static_cast<float>(s[j]) * rs, in ? __ldg(a.col_scale + col + j) : 0.f, (in && a.bias) ? __ldg(a.bias + col + j) : 0.f), a.act);
+    }
+  } else {
+    v[0] = v[1] = v[2] = v[3] = 0.f;
+#pragma unroll 4
+    for (int p = 0; p < a.splits; ++p) {
+      const uint4 t = __ldg(src + p * (plane / 4));
+      v[0] += __uint_as_float(t.x); v[1] += __uint_as_float(t.y); v[2] += __uint_as_float(t.z); v[3] += __uint_as_float(t.w);
+    }
+  }
+  const long long at = row * a.ld_out + col;
+  if (a.wide_store && col + 4 <= a.N) {
+    if (a.out_bf16) *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + at) = make_uint2(F2(v[0], v[1]).bf16(), F2(v[2], v[3]).bf16());
+    else *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (col + j < a.N) {
+      if (a.out_bf16) static_cast<__nv_bfloat16*>(a.out)[at + j] = __float2bfloat16(v[j]);
+      else static_cast<float*>(a.out)[at + j] = v[j];
+    }
+  }
+}
+// What the tensor-core launch left to be added up: the parts of its products (those with splits > 1), and in the blocks from
+// sum_at on the column sums, 32 columns per block of 512 threads.
+struct Gemm8Finish {
+  Gemm8Args job[2];
+  const uint32_t* ws[2];
+  long long ld_ws[2], plane[2], pieces[2];   // pieces of 4 columns; 0: nothing to join
+  Divisor per_row[2];
+  unsigned sum_at;
+  const float* partial;
+  float* sums;
+  int blocks, F;
+};
+template <bool kInt8>
+__global__ void __launch_bounds__(512) gemm8_finish_kernel(const __grid_constant__ Gemm8Finish f) {
+  __shared__ float part[16][33];
+  if (blockIdx.x >= f.sum_at) {
+    column_total(f.partial, f.sums, f.blocks, f.F, static_cast<int>(blockIdx.x - f.sum_at), part);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < (kInt8 ? 1 : 2); ++j) {
+    for (long long i = blockIdx.x * 512ll + threadIdx.x; i < f.pieces[j]; i += f.sum_at * 512ll) {
+      long long row;
+      if (f.pieces[j] < (1ll << 31)) row = f.per_row[j].quotient(static_cast<int>(i));
+      else row = i / f.per_row[j].d;
+      gemm8_join<kInt8>(f.job[j], f.ws[j], f.ld_ws[j], f.plane[j], row, static_cast<int>(i - row * f.per_row[j].d) * 4);
     }
   }
 }

@@ -702,6 +702,11 @@ __global__ void __launch_bounds__(256) rmsnorm_bwd_long_columns_kernel(const Nor
     a.partial[static_cast<long long>(blockIdx.x) * a.F + f] = acc;
   }
 }
+__global__ void __launch_bounds__(512) sum_partials_kernel(const float* __restrict__ partial, float* __restrict__ out, int blocks, int F) {
+  __shared__ float part[16][33];
+  column_total(partial, out, blocks, F, static_cast<int>(blockIdx.x), part);
+}
+
 // ---------------------------------------------------------------- launch shapes
 bool aligned16(std::initializer_list<const void*> ps) {
   for (const void* p : ps)

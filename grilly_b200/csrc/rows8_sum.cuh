@@ -4,12 +4,11 @@
 
 namespace gb {
 
-// out[f] = sum over the blocks of partial[block][f], always in the same order: 32 columns per block of 512 threads, 16
-// threads per column over every 16th block, added up in turn.
-static __global__ void __launch_bounds__(512) sum_partials_kernel(const float* __restrict__ partial, float* __restrict__ out, int blocks, int F) {
-  __shared__ float part[16][33];
+// out[f] = sum over the blocks of partial[block][f], always in the same order, for 32 columns: 512 threads, 16 per column
+// over every 16th block, added up in turn.
+__device__ __forceinline__ void column_total(const float* partial, float* out, int blocks, int F, int which, float (&part)[16][33]) {
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int f = blockIdx.x * 32 + tx;
+  const int f = which * 32 + tx;
   float acc = 0.f;
   if (f < F) {
 #pragma unroll 4
