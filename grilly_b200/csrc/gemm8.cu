@@ -40,13 +40,13 @@ __device__ __forceinline__ uint4 first_bytes(uint4 v, int n) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// 16 features per block; its 8 warps walk K in pieces of 64. Both operands come straight from memory in 16-byte pieces: the
+// 16 features per block; its warps walk K in pieces of 64. Both operands come straight from memory in 16-byte pieces: the
 // sum over k does not care which k a lane calls its own, so lane t of four takes 16 consecutive bytes of a row and feeds
 // them to two MMAs as if they were the fragment's columns, the same for weights and tokens. Rows past the end repeat the
 // last one (their results are dropped); bytes past K are zeroed on the tokens' side. The warps' sums join in shared memory.
-template <int NT>
-__global__ void __launch_bounds__(256) linear_q8_few_kernel(const FewArgs a) {
-  __shared__ int red[8][16][8 * NT];
+template <int NT, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) linear_q8_few_kernel(const FewArgs a) {
+  __shared__ int red[WARPS][16][8 * NT];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int f0 = blockIdx.x * 16;
   const int8_t* w0 = a.wq + static_cast<long long>(min(f0 + g, a.N - 1)) * a.ldw + t * 16;
@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(256) linear_q8_few_kernel(const FewArgs a) {
   for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0;
   const uint4 zero = make_uint4(0, 0, 0, 0);
 #pragma unroll 4
-  for (int k = warp * 64; k < a.K; k += 8 * 64) {
+  for (int k = warp * 64; k < a.K; k += WARPS * 64) {
     const int left = a.K - k - t * 16;         // bytes of this lane's piece inside the row
     uint4 p0 = zero, p1 = zero, q[NT];
     if (left > 0) {
@@ -86,12 +86,12 @@ __global__ void __launch_bounds__(256) linear_q8_few_kernel(const FewArgs a) {
     red[warp][g + 8][8 * n + 2 * t + 1] = acc[n][3];
   }
   __syncthreads();
-  for (int o = threadIdx.x; o < 16 * 8 * NT; o += 256) {
+  for (int o = threadIdx.x; o < 16 * 8 * NT; o += 32 * WARPS) {
     const int f = f0 + (o & 15), m = o >> 4;
     if (f >= a.N || m >= a.M) continue;
     int s = 0;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) s += red[w][o & 15][m];
+    for (int w = 0; w < WARPS; ++w) s += red[w][o & 15][m];
     const float v = gemm8_act(fmaf(static_cast<float>(s) * __ldg(a.xs + m), __ldg(a.ws + f), a.bias ? __ldg(a.bias + f) : 0.f), a.act);
     const long long at = static_cast<long long>(m) * a.N + f;
     if (a.out_bf16) static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16(v);
@@ -101,8 +101,7 @@ __global__ void __launch_bounds__(256) linear_q8_few_kernel(const FewArgs a) {
 
 // ---------------------------------------------------------------- operands of the backward pass
 // q * scale rounded to bf16, rows of ld values (what lies past the features is never read as a column): piece i of 16 bytes
-__device__ __forceinline__ void expand_piece(const int8_t* q, float s, __nv_bfloat16* y, long long i) {
-  const uint4 w = __ldg(reinterpret_cast<const uint4*>(q) + i);
+__device__ __forceinline__ void expand_piece(const uint4 w, float s, __nv_bfloat16* y, long long i) {
   const uint32_t in[4] = {w.x, w.y, w.z, w.w};
   const F2 s2(s, s), offset(-8388736.f, -8388736.f);
   uint32_t out[8];
@@ -119,30 +118,45 @@ __device__ __forceinline__ void expand_piece(const int8_t* q, float s, __nv_bflo
   yp[0] = make_uint4(out[0], out[1], out[2], out[3]);
   yp[1] = make_uint4(out[4], out[5], out[6], out[7]);
 }
-// partial[block][n] = sum over the block's rows, V columns per thread, 256 threads across
+// partial[block][n] = sum over the block's rows: 32 threads across with V columns each, 8 threads per column over every 8th
+// row, added in turn
 template <int V>
-__device__ __forceinline__ void sum_columns(const __nv_bfloat16* g, float* partial, long long M, int N, int across, int block, long long rows_per_block) {
-  const int n = (across * 256 + threadIdx.x) * V;
-  if (n >= N) return;
+__device__ __forceinline__ void sum_columns(const __nv_bfloat16* g, float* partial, long long M, int N, int across, int block, long long rows_per_block,
+                                            float (&part)[8][256]) {
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int n = (across * 32 + tx) * V;
   const long long r0 = block * rows_per_block, r1 = min(M, r0 + rows_per_block);
-  const __nv_bfloat16* p = g + r0 * N + n;
+  const __nv_bfloat16* p = g + (r0 + ty) * N + n;
+  const long long step = 8ll * N;
   if constexpr (V == 8) {
     F2 acc[4] = {F2(0.f, 0.f), F2(0.f, 0.f), F2(0.f, 0.f), F2(0.f, 0.f)};
+    if (n < N) {
 #pragma unroll 8
-    for (long long r = r0; r < r1; ++r, p += N) {
-      const uint4 t = __ldg(reinterpret_cast<const uint4*>(p));
-      const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+      for (long long r = r0 + ty; r < r1; r += 8, p += step) {
+        const uint4 t = __ldg(reinterpret_cast<const uint4*>(p));
+        const uint32_t w[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] = add2(acc[j], F2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u)));
+        for (int j = 0; j < 4; ++j) acc[j] = add2(acc[j], F2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u)));
+      }
     }
-    float* o = partial + static_cast<long long>(block) * N + n;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[j].get(o[2 * j], o[2 * j + 1]);
+    for (int j = 0; j < 4; ++j) acc[j].get(part[ty][(2 * j) * 32 + tx], part[ty][(2 * j + 1) * 32 + tx]);
   } else {
     float acc = 0.f;
+    if (n < N) {
 #pragma unroll 8
-    for (long long r = r0; r < r1; ++r, p += N) acc += __bfloat162float(*p);
-    partial[static_cast<long long>(block) * N + n] = acc;
+      for (long long r = r0 + ty; r < r1; r += 8, p += step) acc += __bfloat162float(*p);
+    }
+    part[ty][tx] = acc;
+  }
+  __syncthreads();
+  const int c = threadIdx.x;               // column c of the block's 32 V: thread c / V's value c % V
+  if (c < 32 * V && across * 32 * V + c < N) {
+    const int at = (c % V) * 32 + c / V;
+    float sum = part[0][at];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) sum += part[i][at];
+    partial[static_cast<long long>(block) * N + across * 32 * V + c] = sum;
   }
 }
 // What the tensor-core launch reads, and the column sums beside it: the first sum_blocks * across blocks sum columns of
@@ -159,24 +173,28 @@ struct PrepareArgs {
   int N, across, sum_blocks, wide;
 };
 __global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ PrepareArgs a) {
+  __shared__ float part[8][256];
   const unsigned sums = a.sum_blocks * a.across;
   if (blockIdx.x < sums) {
     const int block = blockIdx.x / a.across, across = blockIdx.x - block * a.across;
-    if (a.wide) sum_columns<8>(a.g, a.partial, a.M, a.N, across, block, a.rows_per_block);
-    else sum_columns<1>(a.g, a.partial, a.M, a.N, across, block, a.rows_per_block);
+    if (a.wide) sum_columns<8>(a.g, a.partial, a.M, a.N, across, block, a.rows_per_block, part);
+    else sum_columns<1>(a.g, a.partial, a.M, a.N, across, block, a.rows_per_block, part);
     return;
   }
   // 4 pieces per thread and turn, their loads together
   const long long step = (gridDim.x - sums) * 1024ll;
   for (long long base = (blockIdx.x - sums) * 1024ll + threadIdx.x; base < a.pieces; base += step) {
+    uint4 w[4];
+    float scale[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const long long i = base + u * 256;
-      if (i < a.pieces) {
-        const long long row = a.pieces < (1ll << 31) ? a.per_row.quotient(static_cast<int>(i)) : i / a.per_row.d;
-        expand_piece(a.q, __ldg(a.scale + row), a.x, i);
-      }
+      const long long i = min(base + u * 256, a.pieces - 1);
+      w[u] = __ldg(reinterpret_cast<const uint4*>(a.q) + i);
+      scale[u] = __ldg(a.scale + (a.pieces < (1ll << 31) ? a.per_row.quotient(static_cast<int>(i)) : i / a.per_row.d));
     }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (base + u * 256 < a.pieces) expand_piece(w[u], scale[u], a.x, base + u * 256);
   }
 }
 // rows of n bf16 values to rows of ld values, for TMA, which wants rows on 16-byte boundaries
@@ -194,24 +212,17 @@ struct Operand {
   long long ld;      // elements between rows
 };
 
-// The columns of a tile: as few of them past N as possible, then as wide as possible.
-int pick_tile_n(int N) {
-  int best = 256;
-  for (int w : {192, 128})
-    if ((N + w - 1) / w * w < (N + best - 1) / best * best) best = w;
-  return best;
-}
-
-// Geometry of C [M][N] over k. `pairs_for`: the pairs that this product may fill; parts along k until it does.
-int plan_gemm8(grilly_ctx* ctx, Gemm8Args& g, long long M, int N, long long k, int bk, int pairs_for) {
-  using Cfg = Gemm8Cfg;
+// Geometry of C [M][N] over k, in parts along k where its tiles are fewer than the CTA pairs.
+int plan_gemm8(grilly_ctx* ctx, Gemm8Args& g, long long M, int N, long long k, int bk, int pairs) {
+  constexpr int TILE = Gemm8Cfg<true>::TILE;
   if (M > 0x7fffff00ll || k > 0x7fffff00ll || N > 0x7fffff00) return set_error(ctx, GRILLY_ERR_UNSUPPORTED, "8-bit rows: more than 2^31 - 256 rows");
   g.M = M; g.N = N;
-  g.tile_n = pick_tile_n(N);
-  const long long tiles_m = (M + Cfg::TILE - 1) / Cfg::TILE, tiles_n = (N + g.tile_n - 1) / g.tile_n;
+  const long long tiles_m = (M + TILE - 1) / TILE, tiles_n = (N + TILE - 1) / TILE;
   g.k_blocks = static_cast<int>((k + bk - 1) / bk);
   const long long tiles = tiles_m * tiles_n;
-  const int want = static_cast<int>(std::max(1ll, std::min<long long>(pairs_for / tiles, g.k_blocks / 4)));
+  // parts of at least 16 k-blocks, and none of a product under 48: the join's launch and its workspace cost about as much as
+  // 16 k-blocks (256 x 4096 x 4096, 32 k-blocks: 14 us in one launch, 10 + 5 us in four parts)
+  const int want = g.k_blocks < 48 ? 1 : static_cast<int>(std::max(1ll, std::min<long long>(pairs / tiles, g.k_blocks / 16)));
   g.k_per_split = (g.k_blocks + want - 1) / want;
   g.splits = (g.k_blocks + g.k_per_split - 1) / g.k_per_split;
   if (tiles * g.splits > 0x1fffffffll) return set_error(ctx, GRILLY_ERR_UNSUPPORTED, "8-bit rows: too many tiles");
@@ -229,11 +240,11 @@ int plan_gemm8(grilly_ctx* ctx, Gemm8Args& g, long long M, int N, long long k, i
 
 // Tensor maps of one product, and where its parts go when it is split (the workspace is taken here).
 int map_gemm8(grilly_ctx* ctx, bool int8, Operand oa, Operand ob, long long k, Gemm8Args& g, Gemm8Maps& m, Rows8Scratch& ws, Gemm8Finish& f, int which) {
-  using Cfg = Gemm8Cfg;
+  constexpr int TILE = Gemm8Cfg<true>::TILE;
   int rc;
   if (int8) {
     if ((rc = get_tmap_2d(ctx, TM_U8, oa.p, k, g.M, oa.ld, 128, 128, &m.a))) return rc;
-    if ((rc = get_tmap_2d(ctx, TM_U8, ob.p, k, g.N, ob.ld, 128, g.tile_n / 2, &m.b))) return rc;
+    if ((rc = get_tmap_2d(ctx, TM_U8, ob.p, k, g.N, ob.ld, 128, 128, &m.b))) return rc;
   } else {
     if (g.a_across) rc = get_tmap_2d(ctx, TM_BF16, oa.p, g.M, k, oa.ld * 2, 64, 64, &m.a);
     else rc = get_tmap_2d(ctx, TM_BF16, oa.p, k, g.M, oa.ld * 2, 64, 128, &m.a);
@@ -248,7 +259,7 @@ int map_gemm8(grilly_ctx* ctx, bool int8, Operand oa, Operand ob, long long k, G
     return g.wide_store ? get_tmap_2d(ctx, g.out_bf16 ? TM_BF16 : TM_F32, g.out, g.N, g.M, g.ld_out * elt, 64 / elt, 32, &m.out, TM_SW64) : GRILLY_OK;
   }
   // planes of whole tiles, so that a store at the lower edge of one does not reach into the next
-  const long long ld_ws = (g.N + 3) / 4 * 4ll, plane_rows = static_cast<long long>(g.tiles_m) * Cfg::TILE;
+  const long long ld_ws = (g.N + 3) / 4 * 4ll, plane_rows = static_cast<long long>(g.tiles_m) * TILE;
   if ((rc = ws.take(static_cast<size_t>(g.splits) * plane_rows * ld_ws * 4))) return rc;
   f.job[which] = g;
   f.ws[which] = static_cast<const uint32_t*>(ws.p);
@@ -267,7 +278,7 @@ int pairs_that_fit(grilly_ctx* ctx, cudaLaunchConfig_t& cfg, cudaLaunchAttribute
   auto kern = gemm8_pair_kernel<kInt8>;
   const void* key = reinterpret_cast<const void*>(kern);
   if (!ctx->smem_attr_done.count(key)) {
-    GB_CUDA_CHECK(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Gemm8Cfg::SMEM_BYTES));
+    GB_CUDA_CHECK(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Gemm8Cfg<kInt8>::SMEM_BYTES));
     ctx->smem_attr_done.insert(key);
   }
   attr->id = cudaLaunchAttributeClusterDimension;
@@ -275,7 +286,7 @@ int pairs_that_fit(grilly_ctx* ctx, cudaLaunchConfig_t& cfg, cudaLaunchAttribute
   attr->val.clusterDim.y = 1;
   attr->val.clusterDim.z = 1;
   cfg.blockDim = dim3(GEMM8_THREADS, 1, 1);
-  cfg.dynamicSmemBytes = Gemm8Cfg::SMEM_BYTES;
+  cfg.dynamicSmemBytes = Gemm8Cfg<kInt8>::SMEM_BYTES;
   cfg.stream = ctx->stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
@@ -334,7 +345,13 @@ int launch_finish(grilly_ctx* ctx, Gemm8Finish& f) {
 
 template <int NT>
 void launch_few(grilly_ctx* ctx, const FewArgs& a) {
-  linear_q8_few_kernel<NT><<<(a.N + 15) / 16, 256, 0, ctx->stream>>>(a);
+  // about 4096 warps on the GPU, whatever N: many blocks of 4 warps, or few of 16 that share a longer row (for a single
+  // token 4096 x 4096 takes 6.7, 4.2 and 3.9 us with 4, 8 and 16 warps, 16384 x 4096 15.7, 16.6 and 18.6 us). 32 tokens
+  // make the warps' join dearer: at most 8 (22, 33 and 49 us at 16384 x 4096, 50, 30 and 36 us at 4096 x 16384).
+  const unsigned blocks = (a.N + 15) / 16;
+  if (blocks > 512) linear_q8_few_kernel<NT, 4><<<blocks, 128, 0, ctx->stream>>>(a);
+  else if (blocks > 256 || NT == 4) linear_q8_few_kernel<NT, 8><<<blocks, 256, 0, ctx->stream>>>(a);
+  else linear_q8_few_kernel<NT, NT == 4 ? 8 : 16><<<blocks, NT == 4 ? 256 : 512, 0, ctx->stream>>>(a);
 }
 
 // bf16 rows that TMA can read: the tensor itself, or a copy with padded rows in `scratch`
@@ -429,8 +446,8 @@ int grilly_linear_backward_q8(grilly_ctx* ctx, const void* go, const void* xq, c
       p.M = M;
       p.N = N;
       p.wide = N % 8 == 0 && (reinterpret_cast<uintptr_t>(go) & 15) == 0;
-      p.across = p.wide ? (N / 8 + 255) / 256 : (N + 255) / 256;
-      p.sum_blocks = static_cast<int>(std::max<long long>(1, std::min<long long>((M + 31) / 32, ctx->num_sms * 6ll / p.across)));
+      p.across = p.wide ? (N + 255) / 256 : (N + 31) / 32;
+      p.sum_blocks = static_cast<int>(std::max<long long>(1, std::min<long long>((M + 63) / 64, ctx->num_sms * 6ll / p.across)));
       p.rows_per_block = (M + p.sum_blocks - 1) / p.sum_blocks;
       if ((rc = sums.take(sizeof(float) * static_cast<size_t>(p.sum_blocks) * N))) return rc;
       p.partial = static_cast<float*>(sums.p);

@@ -5,8 +5,8 @@
 //     grad_x = grad_out W       A = grad_out [M][k] along k, B = W [k][N] across k
 //     grad_W = grad_out^T x     A = grad_out [k][M], B = x [k][N], both across k
 //
-// A pair of CTAs shares one tcgen05.mma (cta_group::2): a 256 x 256 tile of C (256 x 192 or 256 x 128 where that leaves less
-// of the last column block empty), of which each CTA loads half the rows of A and half of B per k-block of 128 bytes and keeps 128 rows of the accumulator in its own tensor memory, twice, so that one
+// A pair of CTAs shares one tcgen05.mma (cta_group::2): a 256 x 256 tile of C, of which each CTA loads 128 rows of A and
+// 128 of B per k-block of 128 bytes and keeps 128 rows of the accumulator in its own tensor memory, twice, so that one
 // tile is written while the next is computed. Roles per CTA: warp 0 TMA producer (own halves, bytes counted on the
 // leader's barrier), warp 1 MMA issuer (leader) and TMEM allocation, 16 epilogue warps, and for Q8 one warp that brings
 // the next tile's column scales and bias into shared memory (left to the epilogue warps, each tile waited twice for L2).
@@ -40,7 +40,6 @@ struct Gemm8Args {
   long long M;
   int N;
   int a_across;               // bf16: A lies across k
-  int tile_n;                 // columns of a tile
   int tiles_m, tiles_n, tile_group, k_blocks;
   int splits, k_per_split;    // k-blocks per part
   Divisor by_tiles, by_group_tiles, by_group, by_last_group;   // tiles, group * tiles_n, group, tiles_m % group (or 1)
@@ -90,13 +89,14 @@ constexpr int GEMM8_EPI_WARPS = 16;
 constexpr int GEMM8_PARAM_WARP = 2 + GEMM8_EPI_WARPS;
 constexpr int GEMM8_THREADS = 32 * (GEMM8_PARAM_WARP + 1);
 
+template <bool kInt8>
 struct Gemm8Cfg {
   static constexpr int TILE = 256;
   static constexpr int HALF_BYTES = 128 * 128;               // 128 rows (or columns) x 128 bytes
   static constexpr int STAGE_BYTES = 2 * HALF_BYTES;
-  static constexpr int STAGES = 5;
+  static constexpr int STAGES = kInt8 ? 5 : 6;               // what fits beside the rest
   static constexpr int EPI_BYTES = 32 * 64;                  // per epilogue warp: 32 rows x 64 bytes of C on their way out
-  static constexpr int PARAM_FLOATS = 2 * TILE;              // column scales and bias of a tile, double-buffered
+  static constexpr int PARAM_FLOATS = kInt8 ? 2 * TILE : 0;  // column scales and bias of a tile, double-buffered
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + GEMM8_EPI_WARPS * EPI_BYTES + 2 * PARAM_FLOATS * 4 + 1024 /*align slack*/ + 256 /*barriers*/;
   static constexpr int TMEM_COLS = 512;
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of one CTA");
@@ -246,7 +246,7 @@ __host__ __device__ constexpr uint32_t make_idesc_i8(int m, int n) {
 template <bool kInt8>
 __global__ void __launch_bounds__(GEMM8_THREADS, 1)
 gemm8_pair_kernel(const __grid_constant__ Gemm8Maps maps0, const __grid_constant__ Gemm8Maps maps1, const __grid_constant__ Gemm8Jobs jobs) {
-  using Cfg = Gemm8Cfg;
+  using Cfg = Gemm8Cfg<kInt8>;
   constexpr int STAGES = Cfg::STAGES;
   constexpr int BK = kInt8 ? 128 : 64;                         // k per stage
   constexpr int KSTEPS = 4;                                    // instructions per stage, 32 bytes of k each
@@ -321,19 +321,16 @@ gemm8_pair_kernel(const __grid_constant__ Gemm8Maps maps0, const __grid_constant
       uint32_t phase = 0;
       bool ok = true;
       while (ok && walk.next(jobs, job, item)) {
-        const Gemm8Args& a = jobs.job[job];
-        const Gemm8Maps& m = job ? maps1 : maps0;
+        const Gemm8Args& a = jobs.job[kInt8 ? 0 : job];
+        const Gemm8Maps& m = !kInt8 && job ? maps1 : maps0;
         int tm, tn, k0, k1;
         place(a, item, tm, tn, k0, k1);
-        const int half_n = a.tile_n / 2;
-        const int a_row = tm * Cfg::TILE + static_cast<int>(rank) * 128, b_row = tn * a.tile_n + static_cast<int>(rank) * half_n;
-        // bytes of both CTAs: A's 128 rows, and B's rows (along k) or its columns in boxes of 64 (across k)
-        const uint32_t bytes = 2 * (Cfg::HALF_BYTES + (kInt8 ? half_n : (half_n + 63) / 64 * 64) * 128);
+        const int a_row = tm * Cfg::TILE + static_cast<int>(rank) * 128, b_row = tn * Cfg::TILE + static_cast<int>(rank) * 128;
         for (int kb = k0; kb < k1; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) { fail(ERR_WAIT_EMPTY); ok = false; break; }
           uint8_t* sa = smem + stage * Cfg::STAGE_BYTES;
           uint8_t* sb = sa + Cfg::HALF_BYTES;
-          if (leader) mbar_expect_tx(&full_bar[stage], bytes);   // both CTAs' bytes land on this barrier
+          if (leader) mbar_expect_tx(&full_bar[stage], 2 * Cfg::STAGE_BYTES);   // both CTAs' bytes land on this barrier
           const uint32_t bar = map_to_cta(&full_bar[stage], 0);
           if (!kInt8 && a.a_across) {
             tma_load_2d_pair(sa, &m.a, bar, a_row, kb * BK);
@@ -345,7 +342,7 @@ gemm8_pair_kernel(const __grid_constant__ Gemm8Maps maps0, const __grid_constant
             tma_load_2d_pair(sb, &m.b, bar, kb * BK, b_row);
           } else {
             tma_load_2d_pair(sb, &m.b, bar, b_row, kb * BK);
-            if (half_n > 64) tma_load_2d_pair(sb + Cfg::HALF_BYTES / 2, &m.b, bar, b_row + 64, kb * BK);
+            tma_load_2d_pair(sb + Cfg::HALF_BYTES / 2, &m.b, bar, b_row + 64, kb * BK);
           }
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
         }
@@ -364,7 +361,7 @@ gemm8_pair_kernel(const __grid_constant__ Gemm8Maps maps0, const __grid_constant
       const uint32_t peer_empty0 = map_to_cta(&empty_bar[0], 1), own_empty0 = map_to_cta(&empty_bar[0], 0);
       const uint32_t peer_tfull0 = map_to_cta(&tmem_full[0], 1), own_tfull0 = map_to_cta(&tmem_full[0], 0);
       for (; ok && walk.next(jobs, job, item); ++it) {
-        const Gemm8Args& a = jobs.job[job];
+        const Gemm8Args& a = jobs.job[kInt8 ? 0 : job];
         const int k0 = a.by_tiles.quotient(item) * a.k_per_split, k1 = min(a.k_blocks, k0 + a.k_per_split);
         const bool a_across = !kInt8 && a.a_across;
         const uint64_t a0 = a_across ? across_a : along_a, b0 = kInt8 ? along_b : across_b;
@@ -372,7 +369,7 @@ gemm8_pair_kernel(const __grid_constant__ Gemm8Maps maps0, const __grid_constant
         constexpr uint32_t B_STEP = (kInt8 ? 32 : ACROSS_STEP) >> 4;
         const uint32_t a_lo0 = static_cast<uint32_t>(a0), b_lo0 = static_cast<uint32_t>(b0);
         const uint64_t a_hi = a0 & 0xffffffff00000000ull, b_hi = b0 & 0xffffffff00000000ull;
-        const uint32_t idesc = kInt8 ? make_idesc_i8(256, a.tile_n) : make_idesc(true, 256, a.tile_n, a_across, true);
+        const uint32_t idesc = kInt8 ? make_idesc_i8(256, 256) : make_idesc(true, 256, 256, a_across, true);
         const int acc = it & 1;
         if (!mbar_wait(&tmem_empty[acc], ((it >> 1) & 1u) ^ 1u, abort_flag)) { fail(ERR_WAIT_TMEM_EMPTY); break; }
         tc_fence_after();
@@ -410,7 +407,7 @@ gemm8_pair_kernel(const __grid_constant__ Gemm8Maps maps0, const __grid_constant
           float c[Cfg::TILE / 32], d[Cfg::TILE / 32];
 #pragma unroll
           for (int j = 0; j < Cfg::TILE / 32; ++j) {
-            const int col = tn * args.tile_n + j * 32 + lane;
+            const int col = tn * Cfg::TILE + j * 32 + lane;
             c[j] = col < args.N ? __ldg(args.col_scale + col) : 0.f;
             d[j] = (col < args.N && args.bias) ? __ldg(args.bias + col) : 0.f;
           }
@@ -444,14 +441,14 @@ gemm8_pair_kernel(const __grid_constant__ Gemm8Maps maps0, const __grid_constant
     };
     float rs = row_scale(pair);
     for (int it = 0; walk.next(jobs, job, item); ++it) {
-      const Gemm8Args& args = jobs.job[job];
-      const CUtensorMap* tmap_out = job ? &maps1.out : &maps0.out;
+      const Gemm8Args& args = jobs.job[kInt8 ? 0 : job];
+      const CUtensorMap* tmap_out = !kInt8 && job ? &maps1.out : &maps0.out;
       int tm, tn, k0, k1;
       const int part = place(args, item, tm, tn, k0, k1);
       const long long row0 = row_of(tm);
-      const int first_col = tn * args.tile_n;
+      const int first_col = tn * Cfg::TILE;
       const int out_row = static_cast<int>(row0) + (args.raw ? part * args.tiles_m * Cfg::TILE : 0);
-      const int chunks = row0 >= args.M ? 0 : min(args.tile_n / 32, (args.N - first_col + 31) / 32);   // warp-uniform
+      const int chunks = row0 >= args.M ? 0 : min(Cfg::TILE / 32, (args.N - first_col + 31) / 32);   // warp-uniform
       const float rs_next = row_scale(item + num_pairs);
       const int acc = it & 1;
       const float* p = params + acc * Cfg::PARAM_FLOATS;
