@@ -8,8 +8,9 @@
 // A pair of CTAs shares one tcgen05.mma (cta_group::2): a 256 x 256 tile of C, of which each CTA loads 128 rows of A and
 // 128 of B per k-block of 128 bytes and keeps 128 rows of the accumulator in its own tensor memory, twice, so that one
 // tile is written while the next is computed. Roles per CTA: warp 0 TMA producer (own halves, bytes counted on the
-// leader's barrier), warp 1 MMA issuer (leader) and TMEM allocation, 16 epilogue warps, and for Q8 one warp that brings
-// the next tile's column scales and bias into shared memory (left to the epilogue warps, each tile waited twice for L2).
+// leader's barrier), warp 1 MMA issuer (leader) and TMEM allocation, 16 epilogue warps, and one warp that works out the next
+// tile's place and brings its scales and bias into shared memory (left to the epilogue warps, 16 of them did the same
+// integer work for 1000 of the 5000 cycles of a 384-deep tile, and waited for L2 twice).
 // Every wait is bounded and reports through the device status word. Nothing is broadcast by TMA.
 //
 // Few tiles of a long product are split along k: every part stores its raw 32-bit sums to its own plane of a workspace and
@@ -85,6 +86,14 @@ struct Gemm8Walk {
   }
 };
 
+// Where the epilogue finds its tile, double-buffered in shared memory.
+struct Gemm8Place {
+  long long row0;        // first row of the CTA's half
+  int out_row;           // the same as a coordinate of the output's tensor map
+  int col0, chunks;      // first column; blocks of 32 columns that lie in C
+  int job;
+};
+static_assert(sizeof(Gemm8Place) <= 32, "Gemm8Place");
 constexpr int GEMM8_EPI_WARPS = 16;
 constexpr int GEMM8_PARAM_WARP = 2 + GEMM8_EPI_WARPS;
 constexpr int GEMM8_THREADS = 32 * (GEMM8_PARAM_WARP + 1);
@@ -96,8 +105,8 @@ struct Gemm8Cfg {
   static constexpr int STAGE_BYTES = 2 * HALF_BYTES;
   static constexpr int STAGES = kInt8 ? 5 : 6;               // what fits beside the rest
   static constexpr int EPI_BYTES = 32 * 64;                  // per epilogue warp: 32 rows x 64 bytes of C on their way out
-  static constexpr int PARAM_FLOATS = kInt8 ? 2 * TILE : 0;  // column scales and bias of a tile, double-buffered
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + GEMM8_EPI_WARPS * EPI_BYTES + 2 * PARAM_FLOATS * 4 + 1024 /*align slack*/ + 256 /*barriers*/;
+  static constexpr int PARAM_BYTES = 32 + (kInt8 ? (2 * TILE + 128) * 4 : 0);   // a Gemm8Place; column scales, bias, row scales
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + GEMM8_EPI_WARPS * EPI_BYTES + 2 * PARAM_BYTES + 1024 /*align slack*/ + 256 /*barriers*/;
   static constexpr int TMEM_COLS = 512;
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of one CTA");
 };
@@ -255,8 +264,8 @@ gemm8_pair_kernel(const __grid_constant__ Gemm8Maps maps0, const __grid_constant
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* epi = smem + STAGES * Cfg::STAGE_BYTES;
-  float* params = reinterpret_cast<float*>(epi + GEMM8_EPI_WARPS * Cfg::EPI_BYTES);
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(params + 2 * Cfg::PARAM_FLOATS);
+  uint8_t* params = epi + GEMM8_EPI_WARPS * Cfg::EPI_BYTES;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(params + 2 * Cfg::PARAM_BYTES);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* tmem_full = empty_bar + STAGES;
   uint64_t* tmem_empty = tmem_full + 2;
@@ -396,32 +405,49 @@ gemm8_pair_kernel(const __grid_constant__ Gemm8Maps maps0, const __grid_constant
       }
     }
   } else if (warp == GEMM8_PARAM_WARP) {
-    // ------------------------------------------------------------ column scales and bias of the tiles, one tile ahead
-    if constexpr (kInt8) {
-      const Gemm8Args& args = jobs.job[0];
-      if (!args.raw) {
-        for (int it = 0; walk.next(jobs, job, item); ++it) {
-          const int buf = it & 1;
-          int tm, tn;
-          gemm8_tile(args, item, tm, tn);
-          float c[Cfg::TILE / 32], d[Cfg::TILE / 32];
+    // ------------------------------------------------------------ the tiles' places, scales and bias, up to two tiles ahead
+    constexpr int PER_LANE = Cfg::TILE / 32;
+    for (int it = 0; walk.next(jobs, job, item); ++it) {
+      const Gemm8Args& a = jobs.job[kInt8 ? 0 : job];
+      const int buf = it & 1;
+      int tm, tn, k0, k1;
+      const int part = place(a, item, tm, tn, k0, k1);
+      Gemm8Place at;
+      at.row0 = static_cast<long long>(tm) * Cfg::TILE + static_cast<int>(rank) * 128;
+      at.out_row = static_cast<int>(at.row0) + (a.raw ? part * a.tiles_m * Cfg::TILE : 0);
+      at.col0 = tn * Cfg::TILE;
+      at.chunks = min(Cfg::TILE / 32, (a.N - at.col0 + 31) / 32);
+      at.job = job;
+      float c[PER_LANE], d[PER_LANE], r[4];
+      const bool scaled = kInt8 && !a.raw;
+      if (scaled) {
 #pragma unroll
-          for (int j = 0; j < Cfg::TILE / 32; ++j) {
-            const int col = tn * Cfg::TILE + j * 32 + lane;
-            c[j] = col < args.N ? __ldg(args.col_scale + col) : 0.f;
-            d[j] = (col < args.N && args.bias) ? __ldg(args.bias + col) : 0.f;
-          }
-          if (!mbar_wait(&param_empty[buf], ((it >> 1) & 1u) ^ 1u, abort_flag)) { fail(ERR_WAIT_EMPTY); break; }
-          float* p = params + buf * Cfg::PARAM_FLOATS;
+        for (int j = 0; j < PER_LANE; ++j) {
+          const int col = at.col0 + j * 32 + lane;
+          c[j] = col < a.N ? __ldg(a.col_scale + col) : 0.f;
+          d[j] = (col < a.N && a.bias) ? __ldg(a.bias + col) : 0.f;
+        }
 #pragma unroll
-          for (int j = 0; j < Cfg::TILE / 32; ++j) {
-            p[j * 32 + lane] = c[j];
-            p[Cfg::TILE + j * 32 + lane] = d[j];
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&param_full[buf]);
+        for (int j = 0; j < 4; ++j) {
+          const long long row = at.row0 + j * 32 + lane;
+          r[j] = row < a.M ? __ldg(a.row_scale + row) : 0.f;
         }
       }
+      if (!mbar_wait(&param_empty[buf], ((it >> 1) & 1u) ^ 1u, abort_flag)) { fail(ERR_WAIT_EMPTY); break; }
+      uint8_t* p = params + buf * Cfg::PARAM_BYTES;
+      if (lane == 0) *reinterpret_cast<Gemm8Place*>(p) = at;
+      if (scaled) {
+        float* f = reinterpret_cast<float*>(p + 32);
+#pragma unroll
+        for (int j = 0; j < PER_LANE; ++j) {
+          f[j * 32 + lane] = c[j];
+          f[Cfg::TILE + j * 32 + lane] = d[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[2 * Cfg::TILE + j * 32 + lane] = r[j];
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&param_full[buf]);
     }
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs, own 128 rows of the tile)
@@ -430,33 +456,24 @@ gemm8_pair_kernel(const __grid_constant__ Gemm8Maps maps0, const __grid_constant
     uint8_t* stage = epi + (warp - 2) * Cfg::EPI_BYTES;
     const uint32_t leader_tempty0 = map_to_cta(&tmem_empty[0], 0);
     const bool scaled = kInt8 && !jobs.job[0].raw;
-    // the rows' scales are read one tile ahead
-    auto row_of = [&](int tm) { return static_cast<long long>(tm) * Cfg::TILE + static_cast<int>(rank) * 128 + quad * 32; };
-    auto row_scale = [&](int at) {
-      int tm, tn;
-      if (!scaled || at >= jobs.items[0]) return 0.f;
-      gemm8_tile(jobs.job[0], at, tm, tn);
-      const long long row = row_of(tm) + lane;
-      return row < jobs.job[0].M ? __ldg(jobs.job[0].row_scale + row) : 0.f;
-    };
-    float rs = row_scale(pair);
-    for (int it = 0; walk.next(jobs, job, item); ++it) {
-      const Gemm8Args& args = jobs.job[kInt8 ? 0 : job];
-      const CUtensorMap* tmap_out = !kInt8 && job ? &maps1.out : &maps0.out;
-      int tm, tn, k0, k1;
-      const int part = place(args, item, tm, tn, k0, k1);
-      const long long row0 = row_of(tm);
-      const int first_col = tn * Cfg::TILE;
-      const int out_row = static_cast<int>(row0) + (args.raw ? part * args.tiles_m * Cfg::TILE : 0);
-      const int chunks = row0 >= args.M ? 0 : min(Cfg::TILE / 32, (args.N - first_col + 31) / 32);   // warp-uniform
-      const float rs_next = row_scale(item + num_pairs);
+    int items = 0;                                             // of this pair: the same walk, counted
+    while (walk.next(jobs, job, item)) ++items;
+    for (int it = 0; it < items; ++it) {
       const int acc = it & 1;
-      const float* p = params + acc * Cfg::PARAM_FLOATS;
-      if (scaled && !mbar_wait(&param_full[acc], (it >> 1) & 1u, abort_flag)) { fail(ERR_WAIT_FULL); break; }
-      if (!mbar_wait(&tmem_full[acc], (it >> 1) & 1u, abort_flag)) { fail(ERR_WAIT_TMEM_FULL); break; }
+      const uint32_t parity = (it >> 1) & 1u;
+      const uint8_t* p = params + acc * Cfg::PARAM_BYTES;
+      if (!mbar_wait(&param_full[acc], parity, abort_flag)) { fail(ERR_WAIT_FULL); break; }
+      const Gemm8Place at = *reinterpret_cast<const Gemm8Place*>(p);
+      const Gemm8Args& args = jobs.job[kInt8 ? 0 : at.job];
+      const CUtensorMap* tmap_out = !kInt8 && at.job ? &maps1.out : &maps0.out;
+      const float* f = reinterpret_cast<const float*>(p + 32);
+      const float rs = scaled ? f[2 * Cfg::TILE + quad * 32 + lane] : 0.f;
+      const long long row0 = at.row0 + quad * 32;
+      const int chunks = row0 < args.M ? at.chunks : 0;        // warp-uniform
+      if (!mbar_wait(&tmem_full[acc], parity, abort_flag)) { fail(ERR_WAIT_TMEM_FULL); break; }
       tc_fence_after();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * Cfg::TILE;
-#pragma unroll
+#pragma unroll 1   // one copy of the code: it has to stay in the instruction cache
       for (int i = 0; i < PER_WARP; ++i) {
         const int c = group + i * G;
         __syncwarp();
@@ -465,7 +482,7 @@ gemm8_pair_kernel(const __grid_constant__ Gemm8Maps maps0, const __grid_constant
           tmem_ld_32x32(taddr + c * 32, r);
           tmem_ld_wait();
           if (scaled) {
-            const float* cs = p + c * 32;
+            const float* cs = f + c * 32;
             switch (args.act) {
               case GRILLY_ACT_GELU: gemm8_finish<GRILLY_ACT_GELU>(r, rs, cs, cs + Cfg::TILE); break;
               case GRILLY_ACT_SILU: gemm8_finish<GRILLY_ACT_SILU>(r, rs, cs, cs + Cfg::TILE); break;
@@ -473,16 +490,21 @@ gemm8_pair_kernel(const __grid_constant__ Gemm8Maps maps0, const __grid_constant
               default: gemm8_finish<GRILLY_ACT_NONE>(r, rs, cs, cs + Cfg::TILE);
             }
           }
-          gemm8_write(args, tmap_out, r, stage, row0, out_row, first_col + c * 32, lane);
+          if (i == PER_WARP - 1) {
+            // the accumulator is in registers: the next tile's sums may start
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(leader_tempty0 + acc * 8);
+          }
+          gemm8_write(args, tmap_out, r, stage, row0, at.out_row + quad * 32, at.col0 + c * 32, lane);
+        } else if (i == PER_WARP - 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(leader_tempty0 + acc * 8);
         }
       }
-      tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive_cluster(leader_tempty0 + acc * 8);
-        if (scaled) mbar_arrive(&param_empty[acc]);
-      }
-      rs = rs_next;
+      if (lane == 0) mbar_arrive(&param_empty[acc]);
     }
     if (lane == 0) tma_store_wait_all<0>();
   }
