@@ -238,9 +238,13 @@ int plan_gemm8(grilly_ctx* ctx, Gemm8Args& g, long long M, int N, long long k, i
   return GRILLY_OK;
 }
 
-// Tensor maps of one product, and where its parts go when it is split (the workspace is taken here).
-int map_gemm8(grilly_ctx* ctx, bool int8, Operand oa, Operand ob, long long k, Gemm8Args& g, Gemm8Maps& m, Rows8Scratch& ws, Gemm8Finish& f, int which) {
-  constexpr int TILE = Gemm8Cfg<true>::TILE;
+// A split product's parts: planes of whole tiles, so that a store at the lower edge of one does not reach into the next.
+long long part_ld(const Gemm8Args& g) { return (g.N + 3) / 4 * 4ll; }
+long long part_rows(const Gemm8Args& g) { return static_cast<long long>(g.tiles_m) * Gemm8Cfg<true>::TILE; }
+size_t part_bytes(const Gemm8Args& g) { return g.splits > 1 ? static_cast<size_t>(g.splits) * part_rows(g) * part_ld(g) * 4 : 0; }
+
+// Tensor maps of one product, and where its parts go (`parts`: part_bytes) when it is split.
+int map_gemm8(grilly_ctx* ctx, bool int8, Operand oa, Operand ob, long long k, Gemm8Args& g, Gemm8Maps& m, uint32_t* parts, Gemm8Finish& f, int which) {
   int rc;
   if (int8) {
     if ((rc = get_tmap_2d(ctx, TM_U8, oa.p, k, g.M, oa.ld, 128, 128, &m.a))) return rc;
@@ -258,19 +262,16 @@ int map_gemm8(grilly_ctx* ctx, bool int8, Operand oa, Operand ob, long long k, G
     // 64 bytes of 32 rows per store, cut off at the edges
     return g.wide_store ? get_tmap_2d(ctx, g.out_bf16 ? TM_BF16 : TM_F32, g.out, g.N, g.M, g.ld_out * elt, 64 / elt, 32, &m.out, TM_SW64) : GRILLY_OK;
   }
-  // planes of whole tiles, so that a store at the lower edge of one does not reach into the next
-  const long long ld_ws = (g.N + 3) / 4 * 4ll, plane_rows = static_cast<long long>(g.tiles_m) * TILE;
-  if ((rc = ws.take(static_cast<size_t>(g.splits) * plane_rows * ld_ws * 4))) return rc;
   f.job[which] = g;
-  f.ws[which] = static_cast<const uint32_t*>(ws.p);
-  f.ld_ws[which] = ld_ws;
-  f.plane[which] = plane_rows * ld_ws;
-  f.pieces[which] = g.M * (ld_ws / 4);
-  f.per_row[which] = Divisor(static_cast<uint32_t>(ld_ws / 4));
-  g.out = ws.p;
-  g.ld_out = ld_ws;
+  f.ws[which] = parts;
+  f.ld_ws[which] = part_ld(g);
+  f.plane[which] = part_rows(g) * part_ld(g);
+  f.pieces[which] = g.M * (part_ld(g) / 4);
+  f.per_row[which] = Divisor(static_cast<uint32_t>(part_ld(g) / 4));
+  g.out = parts;
+  g.ld_out = part_ld(g);
   g.raw = g.wide_store = 1;
-  return get_tmap_2d(ctx, TM_F32, ws.p, g.N, g.splits * plane_rows, ld_ws * 4, 16, 32, &m.out, TM_SW64);
+  return get_tmap_2d(ctx, TM_F32, parts, g.N, g.splits * part_rows(g), g.ld_out * 4, 16, 32, &m.out, TM_SW64);
 }
 
 template <bool kInt8>
@@ -354,21 +355,22 @@ void launch_few(grilly_ctx* ctx, const FewArgs& a) {
   else linear_q8_few_kernel<NT, NT == 4 ? 8 : 16><<<blocks, NT == 4 ? 256 : 512, 0, ctx->stream>>>(a);
 }
 
-// bf16 rows that TMA can read: the tensor itself, or a copy with padded rows in `scratch`
-int tma_rows(grilly_ctx* ctx, const void* x, long long rows, int n, Rows8Scratch& scratch, Operand* out) {
-  if (n % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
+// bf16 rows that TMA can read: the tensor itself, or a copy with rows of a multiple of 8 values
+bool tma_reads(const void* x, int n) { return n % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
+int pitch_rows(grilly_ctx* ctx, const void* x, long long rows, int n, __nv_bfloat16* copy, Operand* out) {
+  if (tma_reads(x, n)) {
     *out = {x, n};
     return GRILLY_OK;
   }
   const int ld = (n + 7) / 8 * 8;
-  if (int rc = scratch.take(static_cast<size_t>(rows) * ld * 2)) return rc;
   pitch_rows_kernel<<<static_cast<unsigned>(std::min<long long>((rows + 7) / 8, ctx->num_sms * 16ll)), 256, 0, ctx->stream>>>(
-      static_cast<const __nv_bfloat16*>(x), static_cast<__nv_bfloat16*>(scratch.p), rows, n, ld);
+      static_cast<const __nv_bfloat16*>(x), copy, rows, n, ld);
   ctx->launches++;
   GB_CUDA_CHECK(ctx, cudaGetLastError());
-  *out = {scratch.p, ld};
+  *out = {copy, ld};
   return GRILLY_OK;
 }
+size_t pitch_bytes(const void* x, long long rows, int n) { return tma_reads(x, n) ? 0 : static_cast<size_t>(rows) * ((n + 7) / 8 * 8) * 2; }
 
 }  // namespace
 }  // namespace gb
@@ -412,7 +414,9 @@ int grilly_linear_q8(grilly_ctx* ctx, const void* xq, const float* xs, const voi
     g.out = y; g.ld_out = N; g.out_bf16 = out_bf16;
     g.row_scale = xs; g.col_scale = ws; g.bias = bias; g.act = act;
     if ((rc = plan_gemm8(ctx, g, M, N, K, 128, pairs))) return rc;
-    if ((rc = map_gemm8(ctx, true, {xq, ldx}, {wq, ldw}, K, g, maps, parts, finish, 0))) return rc;
+    const size_t at = parts.reserve(part_bytes(g));
+    if ((rc = parts.take())) return rc;
+    if ((rc = map_gemm8(ctx, true, {xq, ldx}, {wq, ldw}, K, g, maps, parts.at<uint32_t>(at), finish, 0))) return rc;
     if ((rc = launch_gemm8<true>(ctx, cfg, pairs, &maps, jobs))) return rc;
     return launch_finish<true>(ctx, finish);
   });
@@ -435,22 +439,42 @@ int grilly_linear_backward_q8(grilly_ctx* ctx, const void* go, const void* xq, c
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr;
     if ((rc = pairs_that_fit<false>(ctx, cfg, &attr, &pairs))) return rc;
-    Rows8Scratch g_rows(ctx), w_rows(ctx), x_rows(ctx), sums(ctx), parts_w(ctx), parts_x(ctx);
-    Gemm8Finish finish{};
-    // the checkpoint as bf16 rows, and the column sums of grad_out by blocks of rows
+    // the products, the one with the longer sums first
+    Gemm8Jobs jobs{};
+    bool is_w[2] = {};
+    const bool w_first = gw && (!gx || M >= N);
+    for (int j = 0; j < 2; ++j) {
+      const bool w_job = (j == 0) == w_first;
+      if (w_job ? !gw : !gx) continue;
+      is_w[jobs.count] = w_job;
+      Gemm8Args& a = jobs.job[jobs.count++];
+      a.out = w_job ? gw : gx;
+      a.ld_out = K;
+      a.out_bf16 = bf16;
+      a.a_across = w_job;
+      if ((rc = plan_gemm8(ctx, a, w_job ? N : M, K, w_job ? M : N, 64, pairs))) return rc;
+    }
     PrepareArgs p{};
     p.per_row = Divisor(1);
+    if (gbias) {
+      p.wide = tma_reads(go, N);
+      p.across = p.wide ? (N + 255) / 256 : (N + 31) / 32;
+      p.sum_blocks = static_cast<int>(std::max<long long>(1, std::min<long long>((M + 63) / 64, ctx->num_sms * 4ll / p.across)));
+    }
+    Rows8Scratch scratch(ctx);
+    const size_t at_g = scratch.reserve(jobs.count ? pitch_bytes(go, M, N) : 0), at_w = scratch.reserve(gx ? pitch_bytes(w, N, K) : 0);
+    const size_t at_x = scratch.reserve(gw ? static_cast<size_t>(M) * ldx * 2 : 0), at_sums = scratch.reserve(sizeof(float) * static_cast<size_t>(p.sum_blocks) * N);
+    const size_t at_parts[2] = {scratch.reserve(part_bytes(jobs.job[0])), scratch.reserve(part_bytes(jobs.job[1]))};
+    if ((rc = scratch.take())) return rc;
+    Gemm8Finish finish{};
+    // the checkpoint as bf16 rows, and the column sums of grad_out by blocks of rows
     unsigned blocks = 0;
     if (gbias) {
       p.g = static_cast<const __nv_bfloat16*>(go);
       p.M = M;
       p.N = N;
-      p.wide = N % 8 == 0 && (reinterpret_cast<uintptr_t>(go) & 15) == 0;
-      p.across = p.wide ? (N + 255) / 256 : (N + 31) / 32;
-      p.sum_blocks = static_cast<int>(std::max<long long>(1, std::min<long long>((M + 63) / 64, ctx->num_sms * 6ll / p.across)));
       p.rows_per_block = (M + p.sum_blocks - 1) / p.sum_blocks;
-      if ((rc = sums.take(sizeof(float) * static_cast<size_t>(p.sum_blocks) * N))) return rc;
-      p.partial = static_cast<float*>(sums.p);
+      p.partial = scratch.at<float>(at_sums);
       blocks = p.across * p.sum_blocks;
       finish.partial = p.partial;
       finish.sums = gbias;
@@ -458,13 +482,12 @@ int grilly_linear_backward_q8(grilly_ctx* ctx, const void* go, const void* xq, c
       finish.F = N;
     }
     if (gw) {
-      if ((rc = x_rows.take(static_cast<size_t>(M) * ldx * 2))) return rc;
       p.q = static_cast<const int8_t*>(xq);
       p.scale = xs;
-      p.x = static_cast<__nv_bfloat16*>(x_rows.p);
+      p.x = scratch.at<__nv_bfloat16>(at_x);
       p.pieces = M * (ldx / 16);
       p.per_row = Divisor(static_cast<uint32_t>(ldx / 16));
-      blocks += static_cast<unsigned>(std::min<long long>((p.pieces + 1023) / 1024, ctx->num_sms * 16ll));
+      blocks += static_cast<unsigned>(std::min<long long>((p.pieces + 1023) / 1024, ctx->num_sms * 4ll));
     }
     if (blocks) {
       const int pi = prof_begin(ctx, PROF_OTHER, 0.0, (gw ? 3.0 * M * K : 0.0) + (gbias ? 2.0 * M * N : 0.0));
@@ -473,26 +496,14 @@ int grilly_linear_backward_q8(grilly_ctx* ctx, const void* go, const void* xq, c
       ctx->launches++;
       GB_CUDA_CHECK(ctx, cudaGetLastError());
     }
-    // both products in one launch, the one with the longer sums first
-    if (gx || gw) {
+    if (jobs.count) {
       Operand g{}, weights{};
-      if ((rc = tma_rows(ctx, go, M, N, g_rows, &g))) return rc;
-      if (gx && (rc = tma_rows(ctx, w, N, K, w_rows, &weights))) return rc;
-      Gemm8Jobs jobs{};
+      if ((rc = pitch_rows(ctx, go, M, N, scratch.at<__nv_bfloat16>(at_g), &g))) return rc;
+      if (gx && (rc = pitch_rows(ctx, w, N, K, scratch.at<__nv_bfloat16>(at_w), &weights))) return rc;
       Gemm8Maps maps[2];
-      const bool w_first = gw && (!gx || M >= N);
-      for (int j = 0; j < 2; ++j) {
-        const bool is_w = (j == 0) == w_first;
-        if (is_w ? !gw : !gx) continue;
-        const int at = jobs.count++;
-        Gemm8Args& a = jobs.job[at];
-        a.out = is_w ? gw : gx;
-        a.ld_out = K;
-        a.out_bf16 = bf16;
-        a.a_across = is_w;
-        const long long k = is_w ? M : N;
-        if ((rc = plan_gemm8(ctx, a, is_w ? N : M, K, k, 64, pairs))) return rc;
-        if ((rc = map_gemm8(ctx, false, g, is_w ? Operand{x_rows.p, ldx} : weights, k, a, maps[at], is_w ? parts_w : parts_x, finish, at))) return rc;
+      for (int j = 0; j < jobs.count; ++j) {
+        const Operand b = is_w[j] ? Operand{scratch.at<void>(at_x), ldx} : weights;
+        if ((rc = map_gemm8(ctx, false, g, b, is_w[j] ? M : N, jobs.job[j], maps[j], scratch.at<uint32_t>(at_parts[j]), finish, j))) return rc;
       }
       if ((rc = launch_gemm8<false>(ctx, cfg, pairs, maps, jobs))) return rc;
     }

@@ -852,8 +852,9 @@ int launch_rmsnorm_bwd(grilly_ctx* ctx, NormBwdQ8Args& a, float* grad_gamma) {
 #undef PICK
     if (int rc = allow_ring(ctx, kern)) return rc;
     if (grad_gamma) {
-      if (int rc = scratch.take(sizeof(float) * grid * static_cast<size_t>(a.F))) return rc;
-      a.partial = static_cast<float*>(scratch.p);
+      const size_t at = scratch.reserve(sizeof(float) * grid * static_cast<size_t>(a.F));
+      if (int rc = scratch.take()) return rc;
+      a.partial = scratch.at<float>(at);
     }
     kern<<<grid, CTA, smem, ctx->stream>>>(ring, a);
     ctx->launches++;
@@ -867,8 +868,9 @@ int launch_rmsnorm_bwd(grilly_ctx* ctx, NormBwdQ8Args& a, float* grad_gamma) {
   if (grad_gamma) {
     const int blocks = static_cast<int>(std::min<long long>((a.rows + 31) / 32, ctx->num_sms));
     const long long per = (a.rows + blocks - 1) / blocks;
-    if (int rc = scratch.take(sizeof(float) * blocks * static_cast<size_t>(a.F))) return rc;
-    a.partial = static_cast<float*>(scratch.p);
+    const size_t at = scratch.reserve(sizeof(float) * blocks * static_cast<size_t>(a.F));
+    if (int rc = scratch.take()) return rc;
+    a.partial = scratch.at<float>(at);
     rmsnorm_bwd_long_columns_kernel<T><<<blocks, 256, 0, ctx->stream>>>(a, per);
     sum_partials_kernel<<<(a.F + 31) / 32, 512, 0, ctx->stream>>>(a.partial, grad_gamma, blocks, a.F);
     ctx->launches += 2;

@@ -30,21 +30,34 @@ int rows8_entry(grilly_ctx* ctx, F&& body) noexcept {
 }
 
 // Scratch of one call from the stream-ordered pool: taken and given back on the context's stream, so calls on other
-// streams and captured graphs never share it.
-struct Rows8Scratch {
-  grilly_ctx* ctx;
-  void* p = nullptr;
+// streams and captured graphs never share it. One allocation a call: parts are reserved first, then take() gets them all.
+class Rows8Scratch {
+ public:
   explicit Rows8Scratch(grilly_ctx* c) : ctx(c) {}
   Rows8Scratch(const Rows8Scratch&) = delete;
-  int take(size_t bytes) {
-    const cudaError_t e = cudaMallocAsync(&p, bytes ? bytes : 16, ctx->stream);
+  // offset of a part of `bytes` bytes, on a 256-byte boundary
+  size_t reserve(size_t bytes) {
+    const size_t at = total;
+    total += (bytes + 255) / 256 * 256;
+    return at;
+  }
+  int take() {
+    if (!total) return GRILLY_OK;
+    const cudaError_t e = cudaMallocAsync(&p, total, ctx->stream);
     if (e == cudaSuccess) return GRILLY_OK;
     cudaGetLastError();
     p = nullptr;
     return set_error(ctx, e == cudaErrorMemoryAllocation ? GRILLY_ERR_OOM : GRILLY_ERR_CUDA,
                      std::string("8-bit rows: scratch: ") + cudaGetErrorString(e));
   }
+  template <class T>
+  T* at(size_t offset) const { return reinterpret_cast<T*>(static_cast<char*>(p) + offset); }
   ~Rows8Scratch() { if (p) cudaFreeAsync(p, ctx->stream); }
+
+ private:
+  grilly_ctx* ctx;
+  void* p = nullptr;
+  size_t total = 0;
 };
 
 // Checks the geometry of an 8-bit row tensor.
