@@ -34,48 +34,67 @@ __device__ __forceinline__ float warp_sum(float v) {
 __device__ __forceinline__ float warp_max(float v) { return __uint_as_float(__reduce_max_sync(FULL, __float_as_uint(v))); }
 __device__ __forceinline__ bool not_finite(float magnitude) { return __float_as_uint(magnitude) >= INF_BITS; }
 
-// A piece: VEC neighbouring values of a row (16 bytes of T, or one value), held as pairs (one value: the pair's second is 0).
+// A piece of a row, as a thread holds it in pairs: VEC neighbouring values (16 bytes of T), or where rows are not on 16-byte
+// boundaries (VEC = 1) two values that lie a team apart, so that neighbouring lanes still touch neighbouring values.
 template <int VEC>
 struct Piece {
-  static constexpr int PAIRS = (VEC + 1) / 2;
+  static constexpr int WIDTH = VEC == 1 ? 2 : VEC, PAIRS = WIDTH / 2;
   F2 v[PAIRS];
 };
-__device__ __forceinline__ void load_piece(const float* p, Piece<4>& x) {
+__device__ __forceinline__ void load_vec(const float* p, Piece<4>& x) {
   const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(p);
   x.v[0].v = t.x;
   x.v[1].v = t.y;
 }
-__device__ __forceinline__ void load_piece(const __nv_bfloat16* p, Piece<8>& x) {
+__device__ __forceinline__ void load_vec(const __nv_bfloat16* p, Piece<8>& x) {
   const uint4 t = *reinterpret_cast<const uint4*>(p);
   const uint32_t w[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) x.v[i] = F2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
 }
-__device__ __forceinline__ void load_piece(const float* p, Piece<1>& x) { x.v[0] = F2(*p, 0.f); }
-__device__ __forceinline__ void load_piece(const __nv_bfloat16* p, Piece<1>& x) { x.v[0] = F2(__bfloat162float(*p), 0.f); }
-__device__ __forceinline__ void store_piece(float* p, const Piece<4>& x) { *reinterpret_cast<ulonglong2*>(p) = make_ulonglong2(x.v[0].v, x.v[1].v); }
-__device__ __forceinline__ void store_piece(__nv_bfloat16* p, const Piece<8>& x) {
+__device__ __forceinline__ void store_vec(float* p, const Piece<4>& x) { *reinterpret_cast<ulonglong2*>(p) = make_ulonglong2(x.v[0].v, x.v[1].v); }
+__device__ __forceinline__ void store_vec(__nv_bfloat16* p, const Piece<8>& x) {
   *reinterpret_cast<uint4*>(p) = make_uint4(x.v[0].bf16(), x.v[1].bf16(), x.v[2].bf16(), x.v[3].bf16());
 }
-__device__ __forceinline__ float only(const Piece<1>& x) {
-  float a, b;
-  x.v[0].get(a, b);
-  return a;
+__device__ __forceinline__ float load_one(const float* p) { return *p; }
+__device__ __forceinline__ float load_one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void store_one(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_one(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
+// the piece at column c of a row of F values (0 past its end)
+template <int VEC, int TEAM, class T>
+__device__ __forceinline__ void load_piece(const T* row, int c, int F, Piece<VEC>& x) {
+  if constexpr (VEC == 1) x.v[0] = F2(load_one(row + c), c + TEAM < F ? load_one(row + c + TEAM) : 0.f);
+  else load_vec(row + c, x);
 }
-__device__ __forceinline__ void store_piece(float* p, const Piece<1>& x) { *p = only(x); }
-__device__ __forceinline__ void store_piece(__nv_bfloat16* p, const Piece<1>& x) { *p = __float2bfloat16(only(x)); }
-// VEC fp32 parameters of the columns (1 where there are none)
+template <int VEC, int TEAM, class T>
+__device__ __forceinline__ void store_piece(T* row, int c, int F, const Piece<VEC>& x) {
+  if constexpr (VEC == 1) {
+    float a, b;
+    x.v[0].get(a, b);
+    store_one(row + c, a);
+    if (c + TEAM < F) store_one(row + c + TEAM, b);
+  } else {
+    store_vec(row + c, x);
+  }
+}
+// Gamma in shared memory: as it is, or for pieces of 8 first every piece's first four values, then every piece's last four
+// (neighbouring lanes then read neighbouring 16 bytes instead of every second 16).
 template <int VEC>
-__device__ __forceinline__ void load_gamma(const float* gamma, int col, Piece<VEC>& g) {
+__device__ __forceinline__ int gamma_at(int col, int F) {
+  return VEC == 8 ? ((col >> 2) & 1) * (F >> 1) + (col >> 3) * 4 + (col & 3) : col;
+}
+// the columns' fp32 parameters (1 where there are none)
+template <int VEC, int TEAM>
+__device__ __forceinline__ void load_gamma(const float* gamma, int c, int F, Piece<VEC>& g) {
   if (!gamma) {
 #pragma unroll
     for (int j = 0; j < Piece<VEC>::PAIRS; ++j) g.v[j] = F2(1.f, 1.f);
   } else if constexpr (VEC == 1) {
-    g.v[0] = F2(gamma[col], 0.f);
+    g.v[0] = F2(gamma[c], c + TEAM < F ? gamma[c + TEAM] : 0.f);
   } else {
 #pragma unroll
     for (int j = 0; j < VEC; j += 4) {
-      const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(gamma + col + j);
+      const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(gamma + gamma_at<VEC>(c + j, F));
       g.v[j / 2].v = t.x;
       g.v[j / 2 + 1].v = t.y;
     }
@@ -101,14 +120,21 @@ __device__ __forceinline__ uint32_t round4(F2 a, F2 b, F2 inv) {
   return __byte_perm(__byte_perm(__float_as_uint(f[0]), __float_as_uint(f[1]), 0x0040),
                      __byte_perm(__float_as_uint(f[2]), __float_as_uint(f[3]), 0x0040), 0x5410);
 }
-__device__ __forceinline__ void store_q(int8_t* p, const Piece<8>& x, F2 inv, uint32_t keep) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(round4(x.v[0], x.v[1], inv) & keep, round4(x.v[2], x.v[3], inv) & keep);
+__device__ __forceinline__ int8_t round1(float x, float inv, uint32_t keep) {
+  return static_cast<int8_t>(__float_as_uint(fmaf(x, inv, 12582912.f)) & keep);
 }
-__device__ __forceinline__ void store_q(int8_t* p, const Piece<4>& x, F2 inv, uint32_t keep) {
-  *reinterpret_cast<uint32_t*>(p) = round4(x.v[0], x.v[1], inv) & keep;
-}
-__device__ __forceinline__ void store_q(int8_t* p, const Piece<1>& x, F2 inv, uint32_t keep) {
-  *p = static_cast<int8_t>(round4(x.v[0], x.v[0], inv) & keep);
+template <int VEC, int TEAM>
+__device__ __forceinline__ void store_q(int8_t* row, int c, int F, const Piece<VEC>& x, F2 inv, uint32_t keep) {
+  if constexpr (VEC == 8) {
+    *reinterpret_cast<uint2*>(row + c) = make_uint2(round4(x.v[0], x.v[1], inv) & keep, round4(x.v[2], x.v[3], inv) & keep);
+  } else if constexpr (VEC == 4) {
+    *reinterpret_cast<uint32_t*>(row + c) = round4(x.v[0], x.v[1], inv) & keep;
+  } else {
+    float a, b;
+    fma2(x.v[0], inv, F2(12582912.f, 12582912.f)).get(a, b);
+    row[c] = static_cast<int8_t>(__float_as_uint(a) & keep);
+    if (c + TEAM < F) row[c + TEAM] = static_cast<int8_t>(__float_as_uint(b) & keep);
+  }
 }
 // four signed bytes as floats: byte + 128 below the bits of 2^23, then the offset taken off; exact
 __device__ __forceinline__ void unpack4(uint32_t w, F2& lo, F2& hi) {
@@ -117,13 +143,18 @@ __device__ __forceinline__ void unpack4(uint32_t w, F2& lo, F2& hi) {
   lo = add2(F2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440)), __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7441))), offset);
   hi = add2(F2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7442)), __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7443))), offset);
 }
-__device__ __forceinline__ void load_q(const int8_t* p, Piece<8>& x) {
-  const uint2 t = *reinterpret_cast<const uint2*>(p);
-  unpack4(t.x, x.v[0], x.v[1]);
-  unpack4(t.y, x.v[2], x.v[3]);
+template <int VEC, int TEAM>
+__device__ __forceinline__ void load_q(const int8_t* row, int c, int F, Piece<VEC>& x) {
+  if constexpr (VEC == 8) {
+    const uint2 t = *reinterpret_cast<const uint2*>(row + c);
+    unpack4(t.x, x.v[0], x.v[1]);
+    unpack4(t.y, x.v[2], x.v[3]);
+  } else if constexpr (VEC == 4) {
+    unpack4(*reinterpret_cast<const uint32_t*>(row + c), x.v[0], x.v[1]);
+  } else {
+    x.v[0] = F2(static_cast<float>(row[c]), c + TEAM < F ? static_cast<float>(row[c + TEAM]) : 0.f);
+  }
 }
-__device__ __forceinline__ void load_q(const int8_t* p, Piece<4>& x) { unpack4(*reinterpret_cast<const uint32_t*>(p), x.v[0], x.v[1]); }
-__device__ __forceinline__ void load_q(const int8_t* p, Piece<1>& x) { x.v[0] = F2(static_cast<float>(*p), 0.f); }
 
 // ---- the ring
 // Up to three row tensors (all 16-byte aligned) and the geometry that the host chose.
@@ -178,6 +209,7 @@ struct Team {
     parity = 0;
   }
   // whole CTA: barriers, gamma, the first rows on their way
+  template <int VEC>
   __device__ void start(const float* gamma) {
     if (threadIdx.x == 0) {
       for (int i = 0; i < TEAMS * g.depth; ++i) mbar_init(reinterpret_cast<uint64_t*>(smem) + i, 1);
@@ -190,7 +222,7 @@ struct Team {
     }
     float* gm = reinterpret_cast<float*>(smem + g.gamma_at);
     if (gamma)
-      for (int c = threadIdx.x; c < g.F; c += CTA) gm[c] = __ldg(gamma + c);
+      for (int c = threadIdx.x; c < g.F; c += CTA) gm[gamma_at<VEC>(c, g.F)] = __ldg(gamma + c);
     __syncthreads();
   }
   // the aligned bytes [from, to) of row r of tensor i that a copy brings, relative to the tensor
@@ -307,8 +339,8 @@ struct Team {
 // The pieces of a row that a thread has: i counts them, c is the first column. Rows shorter than a team's full width leave
 // the loop for all threads at once.
 #define FOR_PIECES(i, c)                                                                       \
-  _Pragma("unroll") for (int i = 0, c = t.tid * VEC; i < NV; ++i, c += TEAM * VEC)              \
-    if (i * TEAM * VEC >= F) break;                                                            \
+  _Pragma("unroll") for (int i = 0, c = t.tid * VEC; i < NV; ++i, c += TEAM * Piece<VEC>::WIDTH) \
+    if (i * TEAM * Piece<VEC>::WIDTH >= F) break;                                              \
     else if (c < F)
 
 // ---- a row per block of 1024 threads, for what the ring does not take
@@ -329,10 +361,10 @@ __device__ __forceinline__ RowStats block_reduce(RowStats s, RowStats* red) {
 // ---------------------------------------------------------------- quantise
 template <class T, int VEC, int TEAM>
 __global__ void __launch_bounds__(CTA, 1) quantize_rows_kernel(const __grid_constant__ Ring ring, int8_t* q, float* scale, long long ld) {
-  constexpr int NV = PER_THREAD / VEC, PAIRS = Piece<VEC>::PAIRS;
+  constexpr int NV = PER_THREAD / Piece<VEC>::WIDTH, PAIRS = Piece<VEC>::PAIRS;
   extern __shared__ __align__(16) uint8_t smem[];
   Team<TEAM> t(ring, smem);
-  t.start(nullptr);
+  t.template start<VEC>(nullptr);
   const int F = ring.F;
   for (; t.row < ring.rows; t.done()) {
     if (!t.next()) break;
@@ -340,7 +372,7 @@ __global__ void __launch_bounds__(CTA, 1) quantize_rows_kernel(const __grid_cons
     Piece<VEC> x[NV];
     float m = 0.f;
     FOR_PIECES(i, c) {
-      load_piece(xp + c, x[i]);
+      load_piece<VEC, TEAM>(xp, c, F, x[i]);
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j) m = max_abs(m, x[i].v[j]);
     }
@@ -349,7 +381,7 @@ __global__ void __launch_bounds__(CTA, 1) quantize_rows_kernel(const __grid_cons
     const F2 inv2(inv, inv);
     const uint32_t keep = not_finite(m) ? 0u : FULL;
     int8_t* qp = q + t.row * ld;
-    FOR_PIECES(i, c) store_q(qp + c, x[i], inv2, keep);
+    FOR_PIECES(i, c) store_q<VEC, TEAM>(qp, c, F, x[i], inv2, keep);
     for (long long c = F + t.tid; c < ld; c += TEAM) qp[c] = 0;
     if (t.tid == 0) scale[t.row] = sc;
   }
@@ -362,19 +394,11 @@ __global__ void __launch_bounds__(1024) quantize_long_rows_kernel(const T* x, in
   for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* xp = x + row * F;
     RowStats s{0.f, 0.f, 0.f};
-    Piece<1> v;
-    for (int c = threadIdx.x; c < F; c += blockDim.x) {
-      load_piece(xp + c, v);
-      s.mh = max_abs(s.mh, v.v[0]);
-    }
+    for (int c = threadIdx.x; c < F; c += blockDim.x) s.mh = max_abs(s.mh, load_one(xp + c), 0.f);
     s = block_reduce(s, red);
     const float sc = row_scale(s.mh), inv = row_inverse(sc);
     const uint32_t keep = not_finite(s.mh) ? 0u : FULL;
-    for (long long c = threadIdx.x; c < ld; c += blockDim.x) {
-      v.v[0] = F2(0.f, 0.f);
-      if (c < F) load_piece(xp + c, v);
-      store_q(q + row * ld + c, v, F2(inv, inv), keep);
-    }
+    for (long long c = threadIdx.x; c < ld; c += blockDim.x) q[row * ld + c] = round1(c < F ? load_one(xp + c) : 0.f, inv, keep);
     if (threadIdx.x == 0) scale[row] = sc;
     __syncthreads();
   }
@@ -399,7 +423,7 @@ __global__ void __launch_bounds__(256) dequantize_vec_kernel(const int8_t* __res
       Piece<VEC> o;
 #pragma unroll
       for (int j = 0; j < VEC / 2; ++j) o.v[j] = mul2(v[k / 2 + j], s2);
-      store_piece(yp + k, o);
+      store_vec(yp + k, o);
     }
   }
 }
@@ -412,9 +436,7 @@ __global__ void __launch_bounds__(256) dequantize_any_kernel(const int8_t* __res
     const float s = __ldg(scale + row);
 #pragma unroll 8
     for (int c = lane; c < F; c += 32) {
-      Piece<1> v;
-      v.v[0] = F2(static_cast<float>(q[row * ld + c]) * s, 0.f);
-      store_piece(y + row * F + c, v);
+      store_one(y + row * F + c, static_cast<float>(q[row * ld + c]) * s);
     }
   }
 }
@@ -462,10 +484,10 @@ __device__ __forceinline__ void norm_row_done(const NormQ8Args& a, const NormSca
 // max |h| are taken together and nothing waits for rstd. A row has been read whole before h is written (in place).
 template <class T, int VEC, int TEAM>
 __global__ void __launch_bounds__(CTA, 1) rmsnorm_q8_kernel(const __grid_constant__ Ring ring, const NormQ8Args a) {
-  constexpr int NV = PER_THREAD / VEC, PAIRS = Piece<VEC>::PAIRS;
+  constexpr int NV = PER_THREAD / Piece<VEC>::WIDTH, PAIRS = Piece<VEC>::PAIRS;
   extern __shared__ __align__(16) uint8_t smem[];
   Team<TEAM> t(ring, smem);
-  t.start(a.gamma);
+  t.template start<VEC>(a.gamma);
   const float* gamma = a.gamma ? reinterpret_cast<const float*>(smem + ring.gamma_at) : nullptr;
   const int F = ring.F;
   const float inv_f = 1.f / static_cast<float>(F);
@@ -477,15 +499,15 @@ __global__ void __launch_bounds__(CTA, 1) rmsnorm_q8_kernel(const __grid_constan
     F2 sum[2] = {F2(0.f, 0.f), F2(0.f, 0.f)};
     RowStats s{0.f, 0.f, 0.f};
     FOR_PIECES(i, c) {
-      load_piece(xp + c, h[i]);
+      load_piece<VEC, TEAM>(xp, c, F, h[i]);
       if (rp) {
         Piece<VEC> r;
-        load_piece(rp + c, r);
+        load_piece<VEC, TEAM>(rp, c, F, r);
 #pragma unroll
         for (int j = 0; j < PAIRS; ++j) h[i].v[j] = add2(h[i].v[j], r.v[j]);
       }
       Piece<VEC> gm;
-      load_gamma(gamma, c, gm);
+      load_gamma<VEC, TEAM>(gamma, c, F, gm);
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j) {
         F2& acc = sum[(i * PAIRS + j) & 1];
@@ -504,13 +526,13 @@ __global__ void __launch_bounds__(CTA, 1) rmsnorm_q8_kernel(const __grid_constan
     int8_t* yq = a.yq + t.row * a.ld;
     int8_t* hq = a.hq ? a.hq + t.row * a.ld : nullptr;
     FOR_PIECES(i, c) {
-      if (hp) store_piece(hp + c, h[i]);
-      if (hq) store_q(hq + c, h[i], hi, r.keep);
+      if (hp) store_piece<VEC, TEAM>(hp, c, F, h[i]);
+      if (hq) store_q<VEC, TEAM>(hq, c, F, h[i], hi, r.keep);
       Piece<VEC> y;
-      load_gamma(gamma, c, y);
+      load_gamma<VEC, TEAM>(gamma, c, F, y);
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j) y.v[j] = mul2(mul2(h[i].v[j], rstd), y.v[j]);
-      store_q(yq + c, y, yi, r.keep);
+      store_q<VEC, TEAM>(yq, c, F, y, yi, r.keep);
     }
     for (long long c = F + t.tid; c < a.ld; c += TEAM) {
       yq[c] = 0;
@@ -528,32 +550,27 @@ __global__ void __launch_bounds__(1024) rmsnorm_q8_long_kernel(const NormQ8Args 
     const T* xp = static_cast<const T*>(a.x) + row * a.F;
     const T* rp = a.residual ? static_cast<const T*>(a.residual) + row * a.F : nullptr;
     RowStats s{0.f, 0.f, 0.f};
-    Piece<1> h, r, gm;
-    auto in = [&](int c) {
-      load_piece(xp + c, h);
-      if (rp) {
-        load_piece(rp + c, r);
-        h.v[0] = add2(h.v[0], r.v[0]);
-      }
-      load_gamma(a.gamma, c, gm);
+    float h, gm;
+    auto in = [&](long long c) {
+      h = load_one(xp + c) + (rp ? load_one(rp + c) : 0.f);
+      gm = a.gamma ? a.gamma[c] : 1.f;
     };
     for (int c = threadIdx.x; c < a.F; c += blockDim.x) {
       in(c);
-      s.sq = fmaf(only(h), only(h), s.sq);
-      s.my = max_abs(s.my, mul2(h.v[0], gm.v[0]));
-      s.mh = max_abs(s.mh, h.v[0]);
+      s.sq = fmaf(h, h, s.sq);
+      s.my = max_abs(s.my, h * gm, 0.f);
+      s.mh = max_abs(s.mh, h, 0.f);
     }
     s = block_reduce(s, red);
     const NormScales n = norm_scales(s, 1.f / static_cast<float>(a.F), a.eps);
     for (long long c = threadIdx.x; c < a.ld; c += blockDim.x) {
-      h.v[0] = gm.v[0] = F2(0.f, 0.f);
+      h = gm = 0.f;
       if (c < a.F) {
-        in(static_cast<int>(c));
-        if (a.h) store_piece(static_cast<T*>(a.h) + row * a.F + c, h);
+        in(c);
+        if (a.h) store_one(static_cast<T*>(a.h) + row * a.F + c, h);
       }
-      if (a.hq) store_q(a.hq + row * a.ld + c, h, F2(n.hi, n.hi), n.keep);
-      gm.v[0] = mul2(mul2(h.v[0], F2(n.rstd, n.rstd)), gm.v[0]);
-      store_q(a.yq + row * a.ld + c, gm, F2(n.yi, n.yi), n.keep);
+      if (a.hq) a.hq[row * a.ld + c] = round1(h, n.hi, n.keep);
+      a.yq[row * a.ld + c] = round1(h * n.rstd * gm, n.yi, n.keep);
     }
     if (threadIdx.x == 0) norm_row_done(a, n, row);
     __syncthreads();
@@ -579,10 +596,10 @@ struct NormBwdQ8Args {
 // twice (before and after its one sum) instead of being held next to those sums.
 template <class T, int VEC, int TEAM>
 __global__ void __launch_bounds__(CTA, 1) rmsnorm_bwd_kernel(const __grid_constant__ Ring ring, const NormBwdQ8Args a) {
-  constexpr int NV = PER_THREAD / VEC, PAIRS = Piece<VEC>::PAIRS;
+  constexpr int NV = PER_THREAD / Piece<VEC>::WIDTH, PAIRS = Piece<VEC>::PAIRS;
   extern __shared__ __align__(16) uint8_t smem[];
   Team<TEAM> t(ring, smem);
-  t.start(a.gamma);
+  t.template start<VEC>(a.gamma);
   const float* gamma = a.gamma ? reinterpret_cast<const float*>(smem + ring.gamma_at) : nullptr;
   const int F = ring.F;
   const float inv_f = 1.f / static_cast<float>(F);
@@ -601,9 +618,9 @@ __global__ void __launch_bounds__(CTA, 1) rmsnorm_bwd_kernel(const __grid_consta
     F2 dots[2] = {F2(0.f, 0.f), F2(0.f, 0.f)};
     FOR_PIECES(i, c) {
       Piece<VEC> g, n, gm;
-      load_piece(gp + c, g);
-      load_q(qp + c, n);
-      load_gamma(gamma, c, gm);
+      load_piece<VEC, TEAM>(gp, c, F, g);
+      load_q<VEC, TEAM>(qp, c, F, n);
+      load_gamma<VEC, TEAM>(gamma, c, F, gm);
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j) {
         n.v[j] = mul2(n.v[j], s2);
@@ -619,20 +636,20 @@ __global__ void __launch_bounds__(CTA, 1) rmsnorm_bwd_kernel(const __grid_consta
     T* op = static_cast<T*>(a.gh) + t.row * F;
     FOR_PIECES(i, c) {
       Piece<VEC> g, n, r;
-      load_piece(gp + c, g);
-      load_q(qp + c, n);
-      load_gamma(gamma, c, r);
+      load_piece<VEC, TEAM>(gp, c, F, g);
+      load_q<VEC, TEAM>(qp, c, F, n);
+      load_gamma<VEC, TEAM>(gamma, c, F, r);
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j) g.v[j] = fma2(n.v[j], back, mul2(g.v[j], r.v[j]));
       if (rp) {
-        load_piece(rp + c, r);
+        load_piece<VEC, TEAM>(rp, c, F, r);
 #pragma unroll
         for (int j = 0; j < PAIRS; ++j) g.v[j] = fma2(g.v[j], rstd2, r.v[j]);
       } else {
 #pragma unroll
         for (int j = 0; j < PAIRS; ++j) g.v[j] = mul2(g.v[j], rstd2);
       }
-      store_piece(op + c, g);
+      store_piece<VEC, TEAM>(op, c, F, g);
     }
   }
   t.end();
@@ -647,7 +664,8 @@ __global__ void __launch_bounds__(CTA, 1) rmsnorm_bwd_kernel(const __grid_consta
       float lo, hi;
       acc[i].v[j].get(lo, hi);
       mine[c + 2 * j] = lo;
-      if constexpr (VEC > 1) mine[c + 2 * j + 1] = hi;
+      if (VEC > 1) mine[c + 2 * j + 1] = hi;
+      else if (c + TEAM < F) mine[c + TEAM] = hi;
     }
   }
   __syncthreads();
@@ -670,21 +688,11 @@ __global__ void __launch_bounds__(1024) rmsnorm_bwd_long_rows_kernel(const NormB
     const int8_t* qp = a.hq + row * a.ld;
     const float rstd = a.rstd[row], s = a.hs[row] * rstd;
     RowStats st{0.f, 0.f, 0.f};
-    Piece<1> g, gm, r;
-    for (int c = threadIdx.x; c < a.F; c += blockDim.x) {
-      load_piece(gp + c, g);
-      load_gamma(a.gamma, c, gm);
-      st.sq = fmaf(only(g) * only(gm), static_cast<float>(qp[c]) * s, st.sq);
-    }
+    auto scaled = [&](int c) { return load_one(gp + c) * (a.gamma ? a.gamma[c] : 1.f); };
+    for (int c = threadIdx.x; c < a.F; c += blockDim.x) st.sq = fmaf(scaled(c), static_cast<float>(qp[c]) * s, st.sq);
     const float dot = block_reduce(st, red).sq / static_cast<float>(a.F);
-    for (int c = threadIdx.x; c < a.F; c += blockDim.x) {
-      load_piece(gp + c, g);
-      load_gamma(a.gamma, c, gm);
-      r.v[0] = F2(0.f, 0.f);
-      if (rp) load_piece(rp + c, r);
-      g.v[0] = F2(rstd * (only(g) * only(gm) - static_cast<float>(qp[c]) * s * dot) + only(r), 0.f);
-      store_piece(op + c, g);
-    }
+    for (int c = threadIdx.x; c < a.F; c += blockDim.x)
+      store_one(op + c, rstd * (scaled(c) - static_cast<float>(qp[c]) * s * dot) + (rp ? load_one(rp + c) : 0.f));
     __syncthreads();
   }
 }
@@ -694,11 +702,8 @@ __global__ void __launch_bounds__(256) rmsnorm_bwd_long_columns_kernel(const Nor
   const long long r1 = min(a.rows, r0 + rows_per_block);
   for (int f = threadIdx.x; f < a.F; f += blockDim.x) {
     float acc = 0.f;
-    Piece<1> g;
-    for (long long r = r0; r < r1; ++r) {
-      load_piece(static_cast<const T*>(a.go) + r * a.F + f, g);
-      acc = fmaf(only(g), static_cast<float>(a.hq[r * a.ld + f]) * (a.hs[r] * a.rstd[r]), acc);
-    }
+    for (long long r = r0; r < r1; ++r)
+      acc = fmaf(load_one(static_cast<const T*>(a.go) + r * a.F + f), static_cast<float>(a.hq[r * a.ld + f]) * (a.hs[r] * a.rstd[r]), acc);
     a.partial[static_cast<long long>(blockIdx.x) * a.F + f] = acc;
   }
 }
