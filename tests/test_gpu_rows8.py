@@ -344,6 +344,108 @@ def test_norm_backward_in_place(backend):
             assert np.array_equal(gh.numpy(), want.numpy()) and np.array_equal(gg.numpy(), wg.numpy())
 
 
+def shifted(b, x, dtype, by):
+    """(x on the device, ``by`` elements past a 16-byte boundary with 7s around it, and a check that those are still there)."""
+    item = 2 if dtype == "bf16" else 4
+    n = int(np.prod(x.shape))
+    flat = np.full(n + 64, 7.0, np.float32)
+    flat[32 + by: 32 + by + n] = np.asarray(x, np.float32).reshape(-1)
+    buf = b.device.upload(flat, dtype)
+    view = DeviceTensor(b.device, buf.ptr + (32 + by) * item, x.shape, dtype, owned=False)
+    view._owned = buf
+
+    def untouched():
+        got = buf.numpy()
+        return np.all(got[: 32 + by] == 7) and np.all(got[32 + by + n:] == 7)
+
+    return view, untouched
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,features", [(1, 8), (3, 100), (40, 384), (150, 1001), (5, 17000)])
+@pytest.mark.parametrize("by", [0, 1, 3])
+def test_tensors_on_any_boundary_and_what_lies_around_them(backend, rows, features, dtype, by):
+    """Views that start off a 16-byte boundary give what aligned tensors give; nothing outside an output is written."""
+    b, f, rng = backend, backend.fnn, rng_for(22, rows, features)
+    x, r = (R.bf16(t) if dtype == "bf16" else t for t in (acts(rng, rows, features), acts(rng, rows, features)))
+    gm = (1 + 0.1 * rng.standard_normal(features)).astype(np.float32)
+    zeros = np.zeros((rows, features), np.float32)
+    xd, rd, gd = shifted(b, x, dtype, by)[0], shifted(b, r, dtype, by)[0], shifted(b, gm, "f32", by)[0]
+    h, h_ok = shifted(b, zeros, dtype, by)
+    got = f.rmsnorm_residual_q8(xd, rd, gd, keep=True, out=(None, h, None, None))
+    want = f.rmsnorm_residual_q8(b.device.upload(x, dtype), b.device.upload(r, dtype), gm, keep=True)
+    assert h_ok() and np.array_equal(h.numpy(), want.h.numpy())
+    for a, w in ((got.y8, want.y8), (got.h8, want.h8)):
+        # the sums may be taken in another order: half a step, and the scales to the roundings of the sum
+        assert np.allclose(a.scale.numpy(), w.scale.numpy(), rtol=(features / 4 + 16) * U, atol=0)
+        assert np.mean(a.q.numpy() != w.q.numpy()) < 1e-3 and np.abs(a.q.numpy().astype(int) - w.q.numpy()).max() <= 1
+    q8 = f.quantize_rows(xd)
+    assert np.array_equal(q8.scale.numpy(), R.quantize(x)[1]) and np.array_equal(q8.q.numpy(), f.quantize_rows(b.device.upload(x, dtype)).q.numpy())
+    y, y_ok = shifted(b, zeros, dtype, by)
+    f.dequantize_rows(q8, out=y)
+    assert y_ok() and np.array_equal(y.numpy(), f.dequantize_rows(q8, dtype).numpy())
+    go, gh_ok = shifted(b, x, dtype, by)
+    gg, gg_ok = shifted(b, gm, "f32", by)
+    f.rmsnorm_backward_q8(go, want.h8, want.rstd, gd, rd, out=(go, gg))
+    wh, wg = f.rmsnorm_backward_q8(b.device.upload(x, dtype), want.h8, want.rstd, gm, b.device.upload(r, dtype))
+    assert gh_ok() and gg_ok()
+    # both sides have these roundings (see norm_backward_case)
+    n = np.abs(want.h8.numpy().astype(np.float64)) * want.rstd.numpy()[:, None]
+    g = np.abs(x * gm)
+    part = want.rstd.numpy()[:, None] * (g + n * (g * n).mean(-1, keepdims=True)) + np.abs(r)
+    tol = 2 * (part * (2 * features + 16) * U + (B if dtype == "bf16" else U) * np.abs(wh.numpy()))
+    assert np.all(np.abs(go.numpy() - wh.numpy()) <= tol)
+    assert np.all(np.abs(gg.numpy() - wg.numpy()) <= 2 * (2 * rows + 8) * U * (np.abs(x) * n).sum(0) + 1e-30)
+
+
+@pytest.mark.parametrize("by", [1, 4])
+def test_products_on_any_boundary(backend, by):
+    """Scales, bias, gradients, weights and results that start off a 16-byte boundary; results keep to themselves."""
+    b, f = backend, backend.fnn
+    for M, N, K in ((5, 100, 64), (70, 264, 128), (300, 520, 1300)):
+        rng = rng_for(23, M, N, K)
+        xq, xs = R.quantize(acts(rng, M, K))
+        wq, ws = R.quantize(acts(rng, N, K))
+        bias = rng.standard_normal(N).astype(np.float32)
+        x8, w8 = put_rows8(b, xq, xs), put_rows8(b, wq, ws)
+        xv, wv = Rows8(x8.q, shifted(b, xs, "f32", by)[0], (M, K)), Rows8(w8.q, shifted(b, ws, "f32", by)[0], (N, K))
+        for dtype in ("f32", "bf16"):
+            y, ok = shifted(b, np.zeros((M, N), np.float32), dtype, by)
+            f.linear_q8(xv, wv, shifted(b, bias, "f32", by)[0], act="silu", out=y)
+            assert ok() and np.array_equal(y.numpy(), f.linear_q8(x8, w8, bias, act="silu", dtype=dtype).numpy())
+            g, w = R.bf16(rng.standard_normal((M, N)).astype(np.float32)), R.bf16(rng.standard_normal((N, K)).astype(np.float32))
+            gx, gx_ok = shifted(b, np.zeros((M, K), np.float32), dtype, by)
+            gw, gw_ok = shifted(b, np.zeros((N, K), np.float32), dtype, by)
+            gb, gb_ok = shifted(b, bias, "f32", by)
+            f.linear_backward_q8(shifted(b, g, "bf16", by)[0], xv, shifted(b, w, "bf16", by)[0], out=(gx, gw, gb))
+            want = f.linear_backward_q8(b.device.upload(g, "bf16"), x8, b.device.upload(w, "bf16"), dtype=dtype)
+            assert gx_ok() and gw_ok() and gb_ok()
+            assert np.array_equal(gx.numpy(), want[0].numpy()) and np.array_equal(gw.numpy(), want[1].numpy())
+            assert np.all(np.abs(gb.numpy() - want[2].numpy()) <= 4 * M * U * np.abs(g.astype(np.float64)).sum(0))
+
+
+def test_backward_outputs_by_themselves(backend):
+    """The library computes the gradients that it is asked for, each the same as with the others."""
+    d, lib = backend.device, backend.device.lib
+    rng = rng_for(24)
+    M, N, K = 300, 72, 200
+    xq, xs = R.quantize(acts(rng, M, K))
+    x8 = put_rows8(backend, xq, xs)
+    g, w = d.upload(rng.standard_normal((M, N)).astype(np.float32), "bf16"), d.upload(rng.standard_normal((N, K)).astype(np.float32), "bf16")
+    all3 = [t.numpy() for t in backend.fnn.linear_backward_q8(g, x8, w, dtype="f32")]
+    for which in range(3):
+        outs = [d.empty(s) if i == which else None for i, s in enumerate(((M, K), (N, K), (N,)))]
+        p = [None if t is None else t.ptr for t in outs]
+        d.check(lib.grilly_linear_backward_q8(d.ctx, g.ptr, x8.q.ptr, x8.scale.ptr, w.ptr if which == 0 else None, *p, M, N, K, x8.ld, 0))
+        assert np.array_equal(outs[which].numpy(), all3[which])
+    hs = backend.fnn.rmsnorm_backward_q8(backend.fnn.dequantize_rows(x8), x8, np.ones(M, np.float32))[0].numpy()
+    gh = d.empty((M, K))
+    go = backend.fnn.dequantize_rows(x8)
+    one = d.upload(np.ones(M, np.float32))
+    d.check(lib.grilly_rmsnorm_backward_q8(d.ctx, go.ptr, x8.q.ptr, x8.scale.ptr, one.ptr, None, None, gh.ptr, None, M, K, x8.ld, 0))
+    assert np.array_equal(gh.numpy(), hs)
+
+
 def test_no_rows(backend):
     d, f = backend.device, backend.fnn
     e8, w = Rows8.empty(d, (0, 64)), np.ones((8, 64), np.float32)
