@@ -158,79 +158,86 @@ __device__ __forceinline__ void gemm8_tile(const Gemm8Args& a, int tile, int& m,
   m = first + r - n * static_cast<int>(whole ? a.by_group.d : a.by_last_group.d);
 }
 
-// One warp writes 32 rows x 32 columns of C. r: the lane's row, 32 neighbouring columns, as raw sums (int32 for Q8).
+// The epilogue works on 32 rows x 16 columns at a time: a lane has 16 neighbouring columns of its row, as raw sums.
 // int8: times the row's scale, times the column's scale plus bias (shared memory, the same address in every lane), activation.
-// The values go to the warp's 2 KB of shared memory as rows of 64 bytes (32 columns of bf16, or 16 of fp32 twice) whose
-// 16-byte pieces are exchanged as TMA's 64-byte swizzle does, so neither side has bank conflicts, and one TMA store takes
-// them out, cut off at the edges of C. Where C's rows are not on 16-byte boundaries the lanes store them themselves.
 template <int ACT>
-__device__ __forceinline__ void gemm8_finish(uint32_t (&r)[32], float rs, const float* cs, const float* bias) {
+__device__ __forceinline__ void gemm8_finish(uint32_t (&r)[16], float rs, const float* cs, const float* bias) {
   const F2 rs2(rs, rs);
+  ulonglong2 c[4], d[4];
 #pragma unroll
-  for (int j = 0; j < 32; j += 4) {
-    const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(cs + j), d = *reinterpret_cast<const ulonglong2*>(bias + j);
+  for (int j = 0; j < 4; ++j) {
+    c[j] = reinterpret_cast<const ulonglong2*>(cs)[j];
+    d[j] = reinterpret_cast<const ulonglong2*>(bias)[j];
+  }
 #pragma unroll
-    for (int i = 0; i < 4; i += 2) {
-      F2 c2, d2;
-      c2.v = i ? c.y : c.x;
-      d2.v = i ? d.y : d.x;
-      const F2 v(static_cast<float>(static_cast<int>(r[j + i])), static_cast<float>(static_cast<int>(r[j + i + 1])));
-      float a, b;
-      gemm8_act2<ACT>(fma2(mul2(v, rs2), c2, d2)).get(a, b);
-      r[j + i] = __float_as_uint(a);
-      r[j + i + 1] = __float_as_uint(b);
-    }
+  for (int j = 0; j < 16; j += 2) {
+    F2 c2, d2;
+    c2.v = j & 2 ? c[j / 4].y : c[j / 4].x;
+    d2.v = j & 2 ? d[j / 4].y : d[j / 4].x;
+    const F2 v(static_cast<float>(static_cast<int>(r[j])), static_cast<float>(static_cast<int>(r[j + 1])));
+    float a, b;
+    gemm8_act2<ACT>(fma2(mul2(v, rs2), c2, d2)).get(a, b);
+    r[j] = __float_as_uint(a);
+    r[j + 1] = __float_as_uint(b);
   }
 }
-// 16 words of a lane's row into the warp's staging rows
-__device__ __forceinline__ void gemm8_stage(uint8_t* stage, int lane, const uint32_t (&w)[16]) {
-#pragma unroll
-  for (int p = 0; p < 4; ++p)
-    *reinterpret_cast<uint4*>(stage + lane * 64 + ((p ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]);
+__device__ __forceinline__ void gemm8_finish(uint32_t (&r)[16], float rs, const float* cs, const float* bias, int act) {
+  switch (act) {
+    case GRILLY_ACT_GELU: return gemm8_finish<GRILLY_ACT_GELU>(r, rs, cs, bias);
+    case GRILLY_ACT_SILU: return gemm8_finish<GRILLY_ACT_SILU>(r, rs, cs, bias);
+    case GRILLY_ACT_RELU: return gemm8_finish<GRILLY_ACT_RELU>(r, rs, cs, bias);
+    default: return gemm8_finish<GRILLY_ACT_NONE>(r, rs, cs, bias);
+  }
 }
-__device__ __forceinline__ void gemm8_write(const Gemm8Args& a, const CUtensorMap* tmap_out, const uint32_t (&r)[32], uint8_t* stage, long long row0,
-                                            int out_row, int col0, int lane) {
+// 4 words of a lane's row of 64 bytes, as piece p; pieces are exchanged as TMA's 64-byte swizzle does, so neither side has
+// bank conflicts
+__device__ __forceinline__ void gemm8_stage(uint8_t* stage, int lane, int p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  *reinterpret_cast<uint4*>(stage + lane * 64 + ((p ^ ((lane >> 1) & 3)) << 4)) = make_uint4(a, b, c, d);
+}
+// The 16 columns from `first` on go to the warp's 2 KB of shared memory, rows of 64 bytes: 16 columns of 32 bits, or a half
+// (h) of 32 columns of bf16. A full row leaves by one TMA store, cut off at the edges of C; where C's rows are not on
+// 16-byte boundaries the lanes store 16 columns themselves.
+__device__ __forceinline__ void gemm8_write(const Gemm8Args& a, const CUtensorMap* tmap_out, const uint32_t (&r)[16], uint8_t* stage, long long row0,
+                                            int out_row, int first, int h, int lane) {
   const bool half = a.out_bf16 && !a.raw;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if (h == 1 && half && a.wide_store) break;               // 32 columns of bf16 went out at once
-    const int first = col0 + 16 * h;
-    if (first >= a.N) break;
-    uint32_t w[16];
-    if (half && a.wide_store) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const __nv_bfloat162 t = __floats2bfloat162_rn(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
-        w[j] = *reinterpret_cast<const uint32_t*>(&t);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) w[j] = r[16 * h + j];
-    }
-    if (a.wide_store) {
+  if (a.wide_store) {
+    if (!half || h == 0) {
       if (lane == 0) tma_store_wait_read<0>();               // the warp's last store has left the staging rows
       __syncwarp();
-      gemm8_stage(stage, lane, w);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        tma_store_2d(tmap_out, stage, first, out_row);
-        tma_store_commit();
-      }
+    }
+    if (half) {
+      uint32_t w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = F2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])).bf16();
+      gemm8_stage(stage, lane, 2 * h, w[0], w[1], w[2], w[3]);
+      gemm8_stage(stage, lane, 2 * h + 1, w[4], w[5], w[6], w[7]);
+      if (h == 0) return;
+      first -= 16;
     } else {
-      __syncwarp();
-      gemm8_stage(stage, lane, w);
-      __syncwarp();
-      const int c = lane & 15, rows = static_cast<int>(a.M - row0 < 32 ? a.M - row0 : 32);
-      if (first + c < a.N) {
+#pragma unroll
+      for (int p = 0; p < 4; ++p) gemm8_stage(stage, lane, p, r[4 * p], r[4 * p + 1], r[4 * p + 2], r[4 * p + 3]);
+      if (first >= a.N) return;                              // the block's second half lies past C
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_2d(tmap_out, stage, first, out_row);
+      tma_store_commit();
+    }
+    return;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int p = 0; p < 4; ++p) gemm8_stage(stage, lane, p, r[4 * p], r[4 * p + 1], r[4 * p + 2], r[4 * p + 3]);
+  __syncwarp();
+  const int c = lane & 15, rows = static_cast<int>(a.M - row0 < 32 ? a.M - row0 : 32);
+  if (first + c < a.N) {
 #pragma unroll 8
-        for (int q = lane >> 4; q < rows; q += 2) {
-          const float v = *reinterpret_cast<const float*>(stage + q * 64 + (((c >> 2) ^ ((q >> 1) & 3)) << 4) + (c & 3) * 4);
-          const long long at = (row0 + q) * a.ld_out + first + c;
-          if (half) static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16(v);
-          else static_cast<float*>(a.out)[at] = v;
-        }
-      }
+    for (int q = lane >> 4; q < rows; q += 2) {
+      const float v = *reinterpret_cast<const float*>(stage + q * 64 + (((c >> 2) ^ ((q >> 1) & 3)) << 4) + (c & 3) * 4);
+      const long long at = (row0 + q) * a.ld_out + first + c;
+      if (half) static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16(v);
+      else static_cast<float*>(a.out)[at] = v;
     }
   }
 }
@@ -451,7 +458,7 @@ gemm8_pair_kernel(const __grid_constant__ Gemm8Maps maps0, const __grid_constant
     }
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs, own 128 rows of the tile)
-    constexpr int G = GEMM8_EPI_WARPS / 4, PER_WARP = Cfg::TILE / 32 / G;
+    constexpr int G = GEMM8_EPI_WARPS / 4;
     const int quad = warp & 3, group = (warp - 2) >> 2;
     uint8_t* stage = epi + (warp - 2) * Cfg::EPI_BYTES;
     const uint32_t leader_tempty0 = map_to_cta(&tmem_empty[0], 0);
@@ -473,36 +480,28 @@ gemm8_pair_kernel(const __grid_constant__ Gemm8Maps maps0, const __grid_constant
       if (!mbar_wait(&tmem_full[acc], parity, abort_flag)) { fail(ERR_WAIT_TMEM_FULL); break; }
       tc_fence_after();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * Cfg::TILE;
+      // 16 columns at a time, the next 16 on their way from tensor memory meanwhile
+      uint32_t r0[16], r1[16];
+      __syncwarp();
+      if (group < chunks) tmem_ld_32x16(taddr + group * 32, r0);
 #pragma unroll 1   // one copy of the code: it has to stay in the instruction cache
-      for (int i = 0; i < PER_WARP; ++i) {
-        const int c = group + i * G;
+      for (int c = group; c < chunks; c += G) {
+        const float* cs = f + c * 32;
+        const int col0 = at.col0 + c * 32;
+        tmem_ld_wait();
+        tmem_ld_32x16(taddr + c * 32 + 16, r1);
+        if (scaled) gemm8_finish(r0, rs, cs, cs + Cfg::TILE, args.act);
+        gemm8_write(args, tmap_out, r0, stage, row0, at.out_row + quad * 32, col0, 0, lane);
         __syncwarp();
-        if (c < chunks) {
-          uint32_t r[32];
-          tmem_ld_32x32(taddr + c * 32, r);
-          tmem_ld_wait();
-          if (scaled) {
-            const float* cs = f + c * 32;
-            switch (args.act) {
-              case GRILLY_ACT_GELU: gemm8_finish<GRILLY_ACT_GELU>(r, rs, cs, cs + Cfg::TILE); break;
-              case GRILLY_ACT_SILU: gemm8_finish<GRILLY_ACT_SILU>(r, rs, cs, cs + Cfg::TILE); break;
-              case GRILLY_ACT_RELU: gemm8_finish<GRILLY_ACT_RELU>(r, rs, cs, cs + Cfg::TILE); break;
-              default: gemm8_finish<GRILLY_ACT_NONE>(r, rs, cs, cs + Cfg::TILE);
-            }
-          }
-          if (i == PER_WARP - 1) {
-            // the accumulator is in registers: the next tile's sums may start
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(leader_tempty0 + acc * 8);
-          }
-          gemm8_write(args, tmap_out, r, stage, row0, at.out_row + quad * 32, at.col0 + c * 32, lane);
-        } else if (i == PER_WARP - 1) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(leader_tempty0 + acc * 8);
-        }
+        tmem_ld_wait();
+        if (c + G < chunks) tmem_ld_32x16(taddr + (c + G) * 32, r0);
+        if (scaled) gemm8_finish(r1, rs, cs + 16, cs + Cfg::TILE + 16, args.act);
+        gemm8_write(args, tmap_out, r1, stage, row0, at.out_row + quad * 32, col0 + 16, 1, lane);
+        __syncwarp();
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(leader_tempty0 + acc * 8);
       __syncwarp();
       if (lane == 0) mbar_arrive(&param_empty[acc]);
     }
