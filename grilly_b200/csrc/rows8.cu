@@ -1,7 +1,7 @@
 // Rows in 8 bits: quantise, read back, RMSNorm with the residual's addition into 8-bit rows, and that norm's backward
 // pass from the 8-bit checkpoint of its input. The definitions stand with the entry points in include/grilly_b200.h.
 //
-// All of them are bound by HBM. A persistent CTA of 512 threads per SM works on several rows at a time, a team of 32 to 512
+// All of them are bound by HBM. A persistent CTA of 512 threads per SM works on several rows at a time, a team of 16 to 512
 // threads on each (32 values per thread). Every team has a ring of rows in shared memory that bulk copies fill several rows
 // ahead, so that memory is read all the time and not only while a block has nothing else to do (blocks that each load,
 // reduce and store a row reached half the bandwidth). A row goes from there into registers, is reduced once and written once.
@@ -19,7 +19,8 @@ namespace {
 
 constexpr int PER_THREAD = 32;         // values of a row per thread
 constexpr int CTA = 512;
-constexpr int MAX_TEAMS = CTA / 32;
+constexpr int MIN_TEAM = 16;
+constexpr int MAX_TEAMS = CTA / MIN_TEAM;
 constexpr int MAX_DEPTH = 8;           // rows in a team's ring
 constexpr uint32_t FULL = 0xffffffffu;
 constexpr uint32_t INF_BITS = 0x7f800000u;
@@ -225,6 +226,8 @@ struct Team {
       for (int c = threadIdx.x; c < g.F; c += CTA) gm[gamma_at<VEC>(c, g.F)] = __ldg(gamma + c);
     __syncthreads();
   }
+  // the team's lanes of its warp (a team of 16: half a warp)
+  __device__ __forceinline__ uint32_t lanes() const { return TEAM >= 32 ? FULL : 0xffffu << (threadIdx.x & 16); }
   // the aligned bytes [from, to) of row r of tensor i that a copy brings, relative to the tensor
   __device__ void span(int i, long long r, long long& from, long long& to) const {
     from = r * g.pitch[i] & ~15ll;
@@ -258,7 +261,7 @@ struct Team {
         bulk_load(slot_of(d) + g.at[i], static_cast<const uint8_t*>(g.src[i]) + from[i], static_cast<uint32_t>(to[i] - from[i]), &bars[d]);
   }
   __device__ void sync() const {
-    if constexpr (TEAM == 32) __syncwarp();
+    if constexpr (TEAM <= 32) __syncwarp(lanes());
     else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(TEAM) : "memory");
   }
   // waits for the current row; false: the wait ran out (reported) and the team stops
@@ -280,8 +283,8 @@ struct Team {
         }
       }
     }
-    if constexpr (TEAM == 32) {
-      ok = __all_sync(FULL, ok);
+    if constexpr (TEAM <= 32) {
+      ok = __all_sync(lanes(), ok);
     } else {
       asm volatile(
           "{\n\t"
@@ -318,6 +321,15 @@ struct Team {
   // over the team, in an order that its size alone decides
   template <bool kSum, bool kMax, bool kTwo>
   __device__ RowStats reduce(RowStats s) {
+    if constexpr (TEAM == 16) {
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) {
+        if constexpr (kSum) s.sq += __shfl_xor_sync(lanes(), s.sq, o);
+        if constexpr (kMax) s.mh = max_abs(s.mh, __shfl_xor_sync(lanes(), s.mh, o), 0.f);
+        if constexpr (kTwo) s.my = max_abs(s.my, __shfl_xor_sync(lanes(), s.my, o), 0.f);
+      }
+      return s;
+    }
     if constexpr (kSum) s.sq = warp_sum(s.sq);
     if constexpr (kMax) s.mh = warp_max(s.mh);
     if constexpr (kTwo) s.my = warp_max(s.my);
@@ -755,7 +767,7 @@ int make_ring(grilly_ctx* ctx, Ring& g, long long rows, int F, const RowTensor* 
   // the smallest team that holds a row, but few enough of them that each has two rows in shared memory: the threads that
   // long rows leave without a row of their own join the others
   const int room = RING_BYTES - g.slots_at;
-  int team = 32;
+  int team = MIN_TEAM;
   while (team < CTA && (team * PER_THREAD < F || CTA / team * 2 * g.slot > room)) team *= 2;
   const int teams = CTA / team;
   if (teams * 2 * g.slot > room) return 0;
@@ -768,6 +780,7 @@ int make_ring(grilly_ctx* ctx, Ring& g, long long rows, int F, const RowTensor* 
 // CALL(TEAM) for the team of a ring
 #define WITH_TEAM(team, CALL)      \
   switch (team) {                  \
+    case 16: CALL(16); break;      \
     case 32: CALL(32); break;      \
     case 64: CALL(64); break;      \
     case 128: CALL(128); break;    \
