@@ -421,21 +421,31 @@ __global__ void __launch_bounds__(1024) quantize_long_rows_kernel(const T* x, in
 template <class T>
 __global__ void __launch_bounds__(256) dequantize_vec_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale, T* __restrict__ y,
                                                              uint32_t vectors, uint32_t per_row, long long ld) {
-  constexpr int VEC = 16 / sizeof(T);
-  for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < vectors; i += gridDim.x * 256u) {
-    const uint32_t row = i / per_row, c = (i - row * per_row) * 16;
-    const uint4 w = *reinterpret_cast<const uint4*>(q + row * ld + c);
-    const float s = __ldg(scale + row);
-    const F2 s2(s, s);
-    F2 v[8];
-    unpack4(w.x, v[0], v[1]); unpack4(w.y, v[2], v[3]); unpack4(w.z, v[4], v[5]); unpack4(w.w, v[6], v[7]);
-    T* yp = y + (static_cast<long long>(row) * per_row * 16 + c);
+  constexpr int VEC = 16 / sizeof(T), AT_ONCE = 2;
+  for (uint32_t base = blockIdx.x * (256u * AT_ONCE) + threadIdx.x; base < vectors; base += gridDim.x * (256u * AT_ONCE)) {
+    uint4 w[AT_ONCE];
+    float s[AT_ONCE];
 #pragma unroll
-    for (int k = 0; k < 16; k += VEC) {
-      Piece<VEC> o;
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const uint32_t i = min(base + u * 256u, vectors - 1), row = i / per_row;
+      w[u] = *reinterpret_cast<const uint4*>(q + row * ld + (i - row * per_row) * 16);
+      s[u] = __ldg(scale + row);
+    }
 #pragma unroll
-      for (int j = 0; j < VEC / 2; ++j) o.v[j] = mul2(v[k / 2 + j], s2);
-      store_vec(yp + k, o);
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const uint32_t i = base + u * 256u;
+      if (i >= vectors) break;
+      const F2 s2(s[u], s[u]);
+      F2 v[8];
+      unpack4(w[u].x, v[0], v[1]); unpack4(w[u].y, v[2], v[3]); unpack4(w[u].z, v[4], v[5]); unpack4(w[u].w, v[6], v[7]);
+      T* yp = y + static_cast<long long>(i) * 16;
+#pragma unroll
+      for (int k = 0; k < 16; k += VEC) {
+        Piece<VEC> o;
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) o.v[j] = mul2(v[k / 2 + j], s2);
+        store_vec(yp + k, o);
+      }
     }
   }
 }
@@ -741,7 +751,7 @@ struct RowTensor {
   int bytes;
 };
 // Returns the threads per row, or 0.
-int make_ring(grilly_ctx* ctx, Ring& g, long long rows, int F, const RowTensor* tensors, int count, bool gamma, size_t* smem, unsigned* grid) {
+int make_ring(grilly_ctx* ctx, Ring& g, long long rows, int F, const RowTensor* tensors, int count, bool gamma, bool gamma_sums, size_t* smem, unsigned* grid) {
   if (F > CTA * PER_THREAD) return 0;
   g = Ring{};
   g.rows = rows;
@@ -774,7 +784,7 @@ int make_ring(grilly_ctx* ctx, Ring& g, long long rows, int F, const RowTensor* 
   *grid = static_cast<unsigned>(std::min<long long>(rows, ctx->num_sms));
   const long long per_team = (rows + static_cast<long long>(*grid) * teams - 1) / (static_cast<long long>(*grid) * teams);
   g.depth = static_cast<int>(std::min<long long>(std::min(MAX_DEPTH, room / (g.slot * teams)), per_team));
-  *smem = g.slots_at + std::max(static_cast<size_t>(g.slot) * teams * g.depth, sizeof(float) * static_cast<size_t>(F) * teams);
+  *smem = g.slots_at + std::max(static_cast<size_t>(g.slot) * teams * g.depth, gamma_sums ? sizeof(float) * static_cast<size_t>(F) * teams : 0);
   return team;
 }
 // CALL(TEAM) for the team of a ring
@@ -805,7 +815,7 @@ int launch_quantize(grilly_ctx* ctx, const T* x, int8_t* q, float* scale, long l
   size_t smem;
   unsigned grid;
   const RowTensor in[1] = {{x, static_cast<long long>(sizeof(T)) * F, static_cast<int>(sizeof(T)) * F}};
-  const int team = make_ring(ctx, ring, rows, F, in, 1, false, &smem, &grid);
+  const int team = make_ring(ctx, ring, rows, F, in, 1, false, false, &smem, &grid);
   if (!team) {
     quantize_long_rows_kernel<<<any_grid(rows), 1024, 0, ctx->stream>>>(x, q, scale, rows, F, ld);
     return GRILLY_OK;
@@ -824,7 +834,7 @@ void launch_dequantize(grilly_ctx* ctx, const int8_t* q, const float* scale, T* 
   const cudaStream_t st = ctx->stream;
   const long long vectors = rows * (F / 16);
   if (F % 16 == 0 && aligned16({y}) && vectors < (1ll << 31)) {
-    const unsigned grid = static_cast<unsigned>(std::min<long long>((vectors + 255) / 256, ctx->num_sms * 32ll));
+    const unsigned grid = static_cast<unsigned>(std::min<long long>((vectors + 511) / 512, ctx->num_sms * 32ll));
     dequantize_vec_kernel<T><<<grid, 256, 0, st>>>(q, scale, y, static_cast<uint32_t>(vectors), static_cast<uint32_t>(F / 16), ld);
   } else {
     dequantize_any_kernel<T><<<any_grid((rows + 7) / 8), 256, 0, st>>>(q, scale, y, rows, F, ld);
@@ -839,7 +849,7 @@ int launch_rmsnorm(grilly_ctx* ctx, const NormQ8Args& a) {
   unsigned grid;
   const long long pitch = static_cast<long long>(sizeof(T)) * a.F;
   const RowTensor in[2] = {{a.x, pitch, static_cast<int>(pitch)}, {a.residual, pitch, static_cast<int>(pitch)}};
-  const int team = aligned16({a.h}) ? make_ring(ctx, ring, a.rows, a.F, in, a.residual ? 2 : 1, a.gamma != nullptr, &smem, &grid) : 0;
+  const int team = aligned16({a.h}) ? make_ring(ctx, ring, a.rows, a.F, in, a.residual ? 2 : 1, a.gamma != nullptr, false, &smem, &grid) : 0;
   if (!team) {
     rmsnorm_q8_long_kernel<T><<<any_grid(a.rows), 1024, 0, ctx->stream>>>(a);
     return GRILLY_OK;
@@ -862,7 +872,7 @@ int launch_rmsnorm_bwd(grilly_ctx* ctx, NormBwdQ8Args& a, float* grad_gamma) {
   unsigned grid;
   const long long pitch = static_cast<long long>(sizeof(T)) * a.F;
   const RowTensor in[3] = {{a.hq, a.ld, (a.F + 15) / 16 * 16}, {a.go, pitch, static_cast<int>(pitch)}, {a.gr, pitch, static_cast<int>(pitch)}};
-  const int team = aligned16({a.gh}) ? make_ring(ctx, ring, a.rows, a.F, in, a.gr ? 3 : 2, a.gamma != nullptr, &smem, &grid) : 0;
+  const int team = aligned16({a.gh}) ? make_ring(ctx, ring, a.rows, a.F, in, a.gr ? 3 : 2, a.gamma != nullptr, grad_gamma != nullptr, &smem, &grid) : 0;
   if (team) {
     void (*kern)(const Ring, const NormBwdQ8Args) = nullptr;
 #define PICK(TEAM) kern = a.F % VEC == 0 ? rmsnorm_bwd_kernel<T, VEC, TEAM> : rmsnorm_bwd_kernel<T, 1, TEAM>
