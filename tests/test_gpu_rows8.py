@@ -446,6 +446,22 @@ def test_backward_outputs_by_themselves(backend):
     assert np.array_equal(gh.numpy(), hs)
 
 
+@pytest.mark.parametrize("features,outs", [(384, 200), (1001, 96), (4096, 264)])
+def test_a_row_gives_the_same_bits_in_every_batch(backend, features, outs):
+    """Norm, quantisation and product of a row do not depend on how many rows there are, whatever kernel they take."""
+    f, rng = backend.fnn, rng_for(25, features)
+    x, r = R.bf16(acts(rng, 700, features)), R.bf16(acts(rng, 700, features))
+    w8 = f.quantize_rows((rng.standard_normal((outs, features)) * 0.05).astype(np.float32))
+    put2 = lambda t, n: backend.device.upload(t[:n], "bf16")  # noqa: E731
+    results = []
+    for n in (700, 257, 33, 20, 3, 1):
+        got = f.rmsnorm_residual_q8(put2(x, n), put2(r, n), keep=True)
+        y = f.linear_q8(got.y8, w8, act="gelu")
+        results.append([t.numpy()[:1] for t in (got.y8.q, got.y8.scale, got.h8.q, got.h8.scale, got.rstd, got.h, y, f.quantize_rows(put2(x, n)).q)])
+    for one in results[1:]:
+        assert all(np.array_equal(a, b) for a, b in zip(results[0], one))
+
+
 def test_no_rows(backend):
     d, f = backend.device, backend.fnn
     e8, w = Rows8.empty(d, (0, 64)), np.ones((8, 64), np.float32)
