@@ -386,11 +386,15 @@ int grilly_linear_q8(grilly_ctx* ctx, const void* xq, const float* xs, const voi
     if (int rc = rows8_check(ctx, "linear_q8: x", xq, xs, M, K, ldx)) return rc;
     if (int rc = rows8_check(ctx, "linear_q8: weights", wq, ws, N, K, ldw)) return rc;
     if (N < 1) return set_error(ctx, GRILLY_ERR_INVALID_ARG, "linear_q8: N must be positive");
+    if (N > ROWS8_MAX_FEATURES) return set_error(ctx, GRILLY_ERR_UNSUPPORTED, "linear_q8: more than 2^30 output features");
     if (K > 131071) return set_error(ctx, GRILLY_ERR_UNSUPPORTED, "linear_q8: more than 131071 features can overflow the 32-bit sums");
     if (act < GRILLY_ACT_NONE || act > GRILLY_ACT_RELU) return set_error(ctx, GRILLY_ERR_INVALID_ARG, "linear_q8: unknown activation");
     if (M == 0) return GRILLY_OK;
     if (!y) return set_error(ctx, GRILLY_ERR_INVALID_ARG, "linear_q8: null output");
     const int out_bf16 = (flags & GRILLY_FLAG_OUT_BF16) ? 1 : 0;
+    const Rows8Span outs[] = {{y, M * N * (out_bf16 ? 2 : 4)}};
+    const Rows8Span ins[] = {{xq, M * ldx}, {xs, 4 * M}, {wq, N * ldw}, {ws, 4ll * N}, {bias, 4ll * N}};
+    if (int rc = rows8_apart(ctx, "linear_q8", outs, ins)) return rc;
     if (M <= FEW_TOKENS) {
       const FewArgs a{static_cast<const int8_t*>(xq), xs, static_cast<const int8_t*>(wq), ws, bias, y, static_cast<int>(M), N, K, ldx, ldw, act, out_bf16};
       const int pi = prof_begin(ctx, PROF_GEMM, 2.0 * M * N * K, static_cast<double>(N) * K + M * (K + (out_bf16 ? 2.0 : 4.0) * N));
@@ -428,9 +432,14 @@ int grilly_linear_backward_q8(grilly_ctx* ctx, const void* go, const void* xq, c
   return rows8_entry(ctx, [&]() -> int {
     if (int rc = rows8_check(ctx, "linear_backward_q8: x", xq, xs, M, K, ldx)) return rc;
     if (N < 1) return set_error(ctx, GRILLY_ERR_INVALID_ARG, "linear_backward_q8: N must be positive");
+    if (N > ROWS8_MAX_FEATURES) return set_error(ctx, GRILLY_ERR_UNSUPPORTED, "linear_backward_q8: more than 2^30 output features");
     const bool bf16 = flags & GRILLY_FLAG_OUT_BF16;
     if (M > 0 && !go) return set_error(ctx, GRILLY_ERR_INVALID_ARG, "linear_backward_q8: null gradient");
     if (gx && !w) return set_error(ctx, GRILLY_ERR_INVALID_ARG, "linear_backward_q8: grad_x needs the weights");
+    const int elt = bf16 ? 2 : 4;
+    const Rows8Span outs[] = {{gx, M * K * elt}, {gw, static_cast<long long>(N) * K * elt}, {gbias, 4ll * N}};
+    const Rows8Span ins[] = {{go, M * N * 2}, {xq, M * ldx}, {xs, 4 * M}, {w, static_cast<long long>(N) * K * 2}};
+    if (int rc = rows8_apart(ctx, "linear_backward_q8", outs, ins)) return rc;
     if (M == 0) {
       if (gw) GB_CUDA_CHECK(ctx, cudaMemsetAsync(gw, 0, static_cast<size_t>(N) * K * (bf16 ? 2 : 4), ctx->stream));
       if (gbias) GB_CUDA_CHECK(ctx, cudaMemsetAsync(gbias, 0, sizeof(float) * N, ctx->stream));

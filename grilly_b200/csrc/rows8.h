@@ -60,12 +60,39 @@ class Rows8Scratch {
   size_t total = 0;
 };
 
-// Checks the geometry of an 8-bit row tensor.
+// Checks the geometry of an 8-bit row tensor. Indices within a row are 32-bit, with room for a block's stride above them.
+constexpr long long ROWS8_MAX_FEATURES = 1ll << 30;
 inline int rows8_check(grilly_ctx* ctx, const char* who, const void* q, const void* scale, long long rows, int features, long long ld) {
   if (rows < 0 || features < 1) return set_error(ctx, GRILLY_ERR_INVALID_ARG, std::string(who) + ": rows must not be negative and features must be positive");
   if (ld < features || ld % 16 != 0) return set_error(ctx, GRILLY_ERR_INVALID_ARG, std::string(who) + ": the rows' pitch must be a multiple of 16 and at least the features");
+  if (features > ROWS8_MAX_FEATURES || ld > 2 * ROWS8_MAX_FEATURES || rows > (1ll << 60) / ld)
+    return set_error(ctx, GRILLY_ERR_UNSUPPORTED, std::string(who) + ": more than 2^30 features, a pitch above 2^31, or too many rows");
   if (rows > 0 && (!q || !scale)) return set_error(ctx, GRILLY_ERR_INVALID_ARG, std::string(who) + ": null 8-bit rows");
   if (reinterpret_cast<uintptr_t>(q) & 15) return set_error(ctx, GRILLY_ERR_INVALID_ARG, std::string(who) + ": 8-bit rows must be 16-byte aligned");
+  return GRILLY_OK;
+}
+
+// An operand's memory. `in_place`: number (from 1) of the output that may be this very memory.
+struct Rows8Span {
+  const void* p;
+  long long bytes;
+  int in_place = 0;
+};
+// Outputs may overlap neither each other nor an input, but for an input that is an output's very memory where that is
+// offered: the kernels read inputs while other blocks write.
+template <int OUTS, int INS>
+int rows8_apart(grilly_ctx* ctx, const char* who, const Rows8Span (&outs)[OUTS], const Rows8Span (&ins)[INS]) {
+  auto overlap = [](const Rows8Span& a, const Rows8Span& b) {
+    const auto x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    return a.p && b.p && x < y + static_cast<uintptr_t>(b.bytes) && y < x + static_cast<uintptr_t>(a.bytes);
+  };
+  for (int i = 0; i < OUTS; ++i) {
+    for (int j = 0; j < i; ++j)
+      if (overlap(outs[i], outs[j])) return set_error(ctx, GRILLY_ERR_INVALID_ARG, std::string(who) + ": two results share memory");
+    for (const Rows8Span& in : ins)
+      if (overlap(outs[i], in) && !(in.in_place == i + 1 && in.p == outs[i].p))
+        return set_error(ctx, GRILLY_ERR_INVALID_ARG, std::string(who) + ": a result shares memory with an operand");
+  }
   return GRILLY_OK;
 }
 

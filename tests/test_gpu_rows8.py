@@ -462,6 +462,39 @@ def test_a_row_gives_the_same_bits_in_every_batch(backend, features, outs):
         assert all(np.array_equal(a, b) for a, b in zip(results[0], one))
 
 
+def test_rows_further_apart_than_they_need_be(backend):
+    """8-bit rows with room between them are written and read like dense ones, and one row without leading dimensions is a row."""
+    f, d, rng = backend.fnn, backend.device, rng_for(26)
+    for rows, features in ((5, 33), (70, 384), (40, 1001)):
+        x = acts(rng, rows, features)
+        far = lambda: Rows8(d.empty((rows, (features + 15) // 16 * 16 + 48), "i8"), d.empty((rows,)), (rows, features))  # noqa: E731
+        xd, w = d.upload(x), d.upload(rng.standard_normal((40, features)).astype(np.float32), "bf16")
+        y8, h8 = far(), far()
+        got = f.rmsnorm_residual_q8(xd, xd, keep=True, out=(y8, None, h8, None))
+        want = f.rmsnorm_residual_q8(xd, xd, keep=True)
+        q8, p8 = f.quantize_rows(xd, out=far()), f.quantize_rows(xd)
+        for a, b in ((y8, want.y8), (h8, want.h8), (q8, p8)):
+            assert np.array_equal(a.q.numpy()[:, :features], b.q.numpy()[:, :features]) and np.all(a.q.numpy()[:, features:] == 0)
+            assert np.array_equal(a.scale.numpy(), b.scale.numpy()) and np.array_equal(f.dequantize_rows(a).numpy(), f.dequantize_rows(b).numpy())
+        go = d.upload(rng.standard_normal((rows, features)).astype(np.float32))
+        for a, b in zip(f.rmsnorm_backward_q8(go, h8, got.rstd), f.rmsnorm_backward_q8(go, want.h8, want.rstd)):
+            assert np.array_equal(a.numpy(), b.numpy())
+        g = d.upload(rng.standard_normal((rows, 40)).astype(np.float32), "bf16")
+        for a, b in zip(f.linear_backward_q8(g, y8, w), f.linear_backward_q8(g, want.y8, w)):
+            assert np.array_equal(a.numpy(), b.numpy())
+        w8 = f.quantize_rows(w)
+        assert np.array_equal(f.linear_q8(y8, w8).numpy(), f.linear_q8(want.y8, w8).numpy())
+        one = f.rmsnorm_residual_q8(x[0], x[0], keep=True)
+        assert one.y8.shape == (features,) and one.h.shape == (features,) and one.rstd.shape == (1,)
+        assert np.array_equal(one.y8.q.numpy()[0], want.y8.q.numpy()[0])
+        line = f.linear_q8(one.y8, w8)
+        assert line.shape == (40,) and np.array_equal(line.numpy(), f.linear_q8(want.y8, w8).numpy()[0])
+        gx, gw, gb = f.linear_backward_q8(rng.standard_normal(40).astype(np.float32), one.y8, w)
+        assert gx.shape == (features,) and gw.shape == (40, features) and gb.shape == (40,)
+        gh, gg = f.rmsnorm_backward_q8(gx, one.h8, one.rstd)
+        assert gh.shape == (features,) and gg.shape == (features,)
+
+
 def test_no_rows(backend):
     d, f = backend.device, backend.fnn
     e8, w = Rows8.empty(d, (0, 64)), np.ones((8, 64), np.float32)
@@ -493,7 +526,25 @@ def test_library_refuses_bad_geometry(backend):
            lib.grilly_linear_backward_q8(d.ctx, None, q.ptr, s.ptr, x.ptr, x.ptr, None, None, 4, 4, 64, 64, 0),
            lib.grilly_linear_backward_q8(d.ctx, x.ptr, q.ptr, s.ptr, None, x.ptr, None, None, 4, 4, 64, 64, 0),
            lib.grilly_rmsnorm_backward_q8(d.ctx, x.ptr, q.ptr, s.ptr, None, None, None, x.ptr, None, 4, 64, 64, 0)]
+    # results over operands or over each other
+    w, big = d.empty((4, 64), "bf16"), d.empty((8, 64))
+    bad += [lib.grilly_quantize_rows(d.ctx, x.ptr, x.ptr, s.ptr, 4, 64, 64, 0), lib.grilly_dequantize_rows(d.ctx, q.ptr, s.ptr, q.ptr, 4, 64, 64, 0),
+            lib.grilly_dequantize_rows(d.ctx, q.ptr, x.ptr + 512, x.ptr, 4, 64, 64, 0),
+            lib.grilly_rmsnorm_residual_q8(d.ctx, x.ptr, None, None, None, q.ptr, s.ptr, q.ptr, x.ptr, None, 4, 64, 64, 1e-5, 0),
+            lib.grilly_rmsnorm_residual_q8(d.ctx, x.ptr, None, None, None, q.ptr, s.ptr, None, None, s.ptr, 4, 64, 64, 1e-5, 0),
+            lib.grilly_rmsnorm_residual_q8(d.ctx, big.ptr, None, None, big.ptr + 256, q.ptr, s.ptr, None, None, None, 4, 64, 64, 1e-5, 0),
+            lib.grilly_linear_q8(d.ctx, q.ptr, s.ptr, q.ptr, s.ptr, None, q.ptr, 4, 4, 64, 64, 64, 0, 0),
+            lib.grilly_linear_q8(d.ctx, q.ptr, s.ptr, q.ptr, s.ptr, x.ptr + 32, x.ptr, 4, 4, 64, 64, 64, 0, 0),
+            lib.grilly_linear_backward_q8(d.ctx, w.ptr, q.ptr, s.ptr, x.ptr, w.ptr, None, None, 4, 64, 64, 64, 1),
+            lib.grilly_linear_backward_q8(d.ctx, big.ptr, q.ptr, s.ptr, w.ptr, None, w.ptr, None, 4, 4, 64, 64, 1),
+            lib.grilly_linear_backward_q8(d.ctx, w.ptr, q.ptr, s.ptr, x.ptr, big.ptr, big.ptr, None, 4, 4, 64, 64, 0),
+            lib.grilly_rmsnorm_backward_q8(d.ctx, x.ptr, q.ptr, s.ptr, s.ptr, w.ptr, None, x.ptr, w.ptr, 4, 64, 64, 0),
+            lib.grilly_rmsnorm_backward_q8(d.ctx, big.ptr, q.ptr, s.ptr, s.ptr, None, None, big.ptr + 256, None, 4, 64, 64, 0)]
     assert bad == [L.ERR_INVALID_ARG] * len(bad)
+    many = [lib.grilly_quantize_rows(d.ctx, x.ptr, q.ptr, s.ptr, 1, (1 << 30) + 1, (1 << 30) + 16, 0),
+            lib.grilly_quantize_rows(d.ctx, x.ptr, q.ptr, s.ptr, 1, 64, 1 << 32, 0), lib.grilly_quantize_rows(d.ctx, x.ptr, q.ptr, s.ptr, 1 << 55, 64, 64, 0),
+            lib.grilly_linear_q8(d.ctx, q.ptr, s.ptr, q.ptr, s.ptr, None, x.ptr, 1, (1 << 30) + 1, 64, 64, 64, 0, 0)]
+    assert many == [L.ERR_UNSUPPORTED] * len(many)
     assert lib.grilly_linear_q8(d.ctx, q.ptr, s.ptr, q.ptr, s.ptr, None, x.ptr, 1, 1, 131072, 131072, 131072, 0, 0) == L.ERR_UNSUPPORTED
     assert d.launch_count() == before
 
@@ -559,7 +610,7 @@ def test_a_layer_forward_and_backward(backend_bf16, rows, features, outs):
 
 
 def test_captured_and_replayed(lib):
-    """The layer in two CUDA graphs that are replayed in turn, on a stream of torch's, with inputs that change in between."""
+    """The layer in two CUDA graphs that are replayed at once on two streams of torch's, with inputs that change in between."""
     import torch
 
     import grilly_b200
@@ -567,7 +618,7 @@ def test_captured_and_replayed(lib):
     b = grilly_b200.Compute(precision="bf16")
     try:
         d, f, rng = b.device, b.fnn, rng_for(20)
-        stream = torch.cuda.Stream()
+        stream, other = torch.cuda.Stream(), torch.cuda.Stream()
         d.set_stream(stream.cuda_stream)
         rows, features, outs = 2100, 384, 264
         names = {torch.bfloat16: "bf16", torch.float32: "f32", torch.int8: "i8"}
@@ -609,9 +660,12 @@ def test_captured_and_replayed(lib):
                 for t in sets:
                     t["x"].normal_()
                     t["go"].normal_()
-                graphs[0].replay()
-                graphs[1].replay()
                 stream.synchronize()
+                graphs[0].replay()
+                with torch.cuda.stream(other):                        # at the same time as the first
+                    graphs[1].replay()
+                stream.synchronize()
+                other.synchronize()
                 got = [{k: t[k].clone() for k in outputs} for t in sets]
                 for t in sets:
                     for k in outputs:
