@@ -209,11 +209,12 @@ __device__ __forceinline__ void gemm8_stage(uint8_t* stage, int lane, int p, uin
 __device__ __forceinline__ void gemm8_write(const Gemm8Args& a, const CUtensorMap* tmap_out, const uint32_t (&r)[16], uint8_t* stage, long long row0,
                                             int out_row, int first, int h, int lane) {
   const bool half = a.out_bf16 && !a.raw;
+  if (!(a.wide_store && half && h == 1)) {
+    // the warp's last store has left the staging rows (it may have been of the launch's other product, stored otherwise)
+    if (lane == 0) tma_store_wait_read<0>();
+    __syncwarp();
+  }
   if (a.wide_store) {
-    if (!half || h == 0) {
-      if (lane == 0) tma_store_wait_read<0>();               // the warp's last store has left the staging rows
-      __syncwarp();
-    }
     if (half) {
       uint32_t w[8];
 #pragma unroll
@@ -235,7 +236,6 @@ __device__ __forceinline__ void gemm8_write(const Gemm8Args& a, const CUtensorMa
     }
     return;
   }
-  __syncwarp();
 #pragma unroll
   for (int p = 0; p < 4; ++p) gemm8_stage(stage, lane, p, r[4 * p], r[4 * p + 1], r[4 * p + 2], r[4 * p + 3]);
   __syncwarp();

@@ -269,6 +269,16 @@ def test_linear_backward_q8(backend, M, N, K):
         assert np.array_equal(s.numpy(), t.numpy())
 
 
+@pytest.mark.parametrize("M,N,K", [(19968, 32, 1925), (5000, 40, 1001), (6000, 300, 77), (4100, 9, 2000)])
+def test_linear_backward_whose_products_are_stored_differently(backend, M, N, K):
+    """One product split along k (its parts leave by TMA), the other with rows of C off 16-byte boundaries (its lanes store),
+    by the same warps of one launch: the same bits every time, and right."""
+    a = backward_case(backend, M, N, K, "bf16")
+    for _ in range(5):
+        for s, t in zip(a, backward_case(backend, M, N, K, "bf16")):
+            assert np.array_equal(s.numpy(), t.numpy())
+
+
 def test_linear_backward_from_arrays(backend):
     rng = rng_for(12)
     x, w, g = acts(rng, 20, 48).reshape(4, 5, 48), rng.standard_normal((30, 48)).astype(np.float32), rng.standard_normal((4, 5, 30)).astype(np.float32)
