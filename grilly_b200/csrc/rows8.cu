@@ -6,8 +6,8 @@
 // ahead, so that memory is read all the time and not only while a block has nothing else to do (blocks that each load,
 // reduce and store a row reached half the bandwidth). A row goes from there into registers, is reduced once and written once.
 // Rows that start off 16-byte boundaries (odd lengths) are copied from the boundary below and read value by value.
-// 16384 x 4096 bf16: the norm with both outputs 88 us (6.1 TB/s), its backward pass with the residual's gradient 86 us
-// (5.5 TB/s), quantise 39 us (5.2 TB/s), read back 35 us (5.8 TB/s); a plain copy runs at 6.5 TB/s.
+// 16384 x 4096 bf16: the norm with both outputs 91 us (5.9 TB/s), its backward pass with the residual's gradient 86 us
+// (5.5 TB/s), quantise 40 us (5.0 TB/s), read back 35 us (5.8 TB/s); a plain copy runs at 6.5 TB/s.
 #include "rows8.h"
 #include "rows8_sum.cuh"
 #include "ptx.cuh"
@@ -110,31 +110,60 @@ __device__ __forceinline__ float row_scale(float a) {
   const float r = 1.f / 127.f, q = a * r;
   return not_finite(a) ? ROWS8_NAN : fmaxf(fmaf(fmaf(-127.f, q, a), r, q), ROWS8_TINY);
 }
-// 1 / scale to 1 ulp: it only decides values next to a tie. Scales lie in [2^-126, 2^121], where the approximation holds.
-__device__ __forceinline__ float row_inverse(float scale) { return __fdividef(1.f, scale); }
-// x * inv rounded to the nearest integer (ties to even), in the low byte: adding 1.5 * 2^23 leaves no fraction bits, and
-// one fused multiply-add rounds once. Four bytes come out of three byte permutes; conversions would run at a quarter rate.
-// keep: all ones, or zero for a row that is not finite.
-__device__ __forceinline__ uint32_t round4(F2 a, F2 b, F2 inv) {
-  const F2 magic(12582912.f, 12582912.f);
+// q is 127 x / a rounded to the nearest integer (ties to even), a the row's largest |x|: the quotient by the scale before
+// the scale's own rounding. Ties are common where the values lie on a coarse grid, x = a / 2 for one, and a product with
+// one float falls to either side of them.
+struct RowInverse {
+  float hi, lo;
+};
+struct RowInverse2 {
+  F2 hi, lo;
+  __device__ __forceinline__ explicit RowInverse2(RowInverse r) : hi(r.hi, r.hi), lo(r.lo, r.lo) {}
+};
+// ONE = false: 127 / a as a sum of two floats. A product and a fused multiply-add give the quotient right to 2^-47 before
+// its rounding to fp32, so that a tie comes out as that tie.
+// ONE: for bf16 values one float rounded up and one fused multiply-add do. 254 x and a (2 k + 1) have 16 bits each and are
+// equal or 2^-16 apart, equal only where a is 127 * 2^j (the inverse is a power of two then, the product exact) or
+// x = a / 2, and that tie goes up, to 64.
+// scale: a / 127 or, for a of at most 127 * 2^-126, 2^-126, whose inverse is exact. No division: it would stand between a
+// row's reduction and its stores (quantise 44 us with it, 40 without, at 16384 x 4096 bf16).
+template <bool ONE>
+__device__ __forceinline__ RowInverse row_inverse(float scale, float a) {
+  const float t = __fdividef(1.f, scale), d = t * (1.f / 127.f);   // t to 2 ulp; scales lie in [2^-126, 2^121]
+  const float rest = a > 127.f * ROWS8_TINY ? fmaf(-a, t, 127.f) : 0.f;
+  if (!ONE) return {t, rest * d};
+  const float hi = fmaf(rest, d, t);                               // to half an ulp; exact where 127 / a is a power of two
+  return {rest != 0.f && fmaf(-a, hi, 127.f) > 0.f ? fmaf(hi, 0x1p-23f, hi) : hi, 0.f};
+}
+constexpr float MAGIC = 12582912.f;   // 1.5 * 2^23: the sum has no fraction bits, and the integer is in its low byte
+template <bool ONE>
+__device__ __forceinline__ F2 quotient2(F2 x, const RowInverse2& inv) {
+  const F2 magic(MAGIC, MAGIC);
+  return ONE ? fma2(x, inv.hi, magic) : add2(fma2(x, inv.hi, mul2(x, inv.lo)), magic);
+}
+// Four bytes come out of three byte permutes; conversions would run at a quarter rate.
+template <bool ONE>
+__device__ __forceinline__ uint32_t round4(F2 a, F2 b, const RowInverse2& inv) {
   float f[4];
-  fma2(a, inv, magic).get(f[0], f[1]);
-  fma2(b, inv, magic).get(f[2], f[3]);
+  quotient2<ONE>(a, inv).get(f[0], f[1]);
+  quotient2<ONE>(b, inv).get(f[2], f[3]);
   return __byte_perm(__byte_perm(__float_as_uint(f[0]), __float_as_uint(f[1]), 0x0040),
                      __byte_perm(__float_as_uint(f[2]), __float_as_uint(f[3]), 0x0040), 0x5410);
 }
-__device__ __forceinline__ int8_t round1(float x, float inv, uint32_t keep) {
-  return static_cast<int8_t>(__float_as_uint(fmaf(x, inv, 12582912.f)) & keep);
+// keep: all ones, or zero for a row that is not finite.
+template <bool ONE>
+__device__ __forceinline__ int8_t round1(float x, RowInverse inv, uint32_t keep) {
+  return static_cast<int8_t>(__float_as_uint(ONE ? fmaf(x, inv.hi, MAGIC) : __fadd_rn(fmaf(x, inv.hi, __fmul_rn(x, inv.lo)), MAGIC)) & keep);
 }
-template <int VEC, int TEAM>
-__device__ __forceinline__ void store_q(int8_t* row, int c, int F, const Piece<VEC>& x, F2 inv, uint32_t keep) {
+template <int VEC, int TEAM, bool ONE>
+__device__ __forceinline__ void store_q(int8_t* row, int c, int F, const Piece<VEC>& x, const RowInverse2& inv, uint32_t keep) {
   if constexpr (VEC == 8) {
-    *reinterpret_cast<uint2*>(row + c) = make_uint2(round4(x.v[0], x.v[1], inv) & keep, round4(x.v[2], x.v[3], inv) & keep);
+    *reinterpret_cast<uint2*>(row + c) = make_uint2(round4<ONE>(x.v[0], x.v[1], inv) & keep, round4<ONE>(x.v[2], x.v[3], inv) & keep);
   } else if constexpr (VEC == 4) {
-    *reinterpret_cast<uint32_t*>(row + c) = round4(x.v[0], x.v[1], inv) & keep;
+    *reinterpret_cast<uint32_t*>(row + c) = round4<ONE>(x.v[0], x.v[1], inv) & keep;
   } else {
     float a, b;
-    fma2(x.v[0], inv, F2(12582912.f, 12582912.f)).get(a, b);
+    quotient2<ONE>(x.v[0], inv).get(a, b);
     row[c] = static_cast<int8_t>(__float_as_uint(a) & keep);
     if (c + TEAM < F) row[c + TEAM] = static_cast<int8_t>(__float_as_uint(b) & keep);
   }
@@ -391,11 +420,11 @@ __global__ void __launch_bounds__(CTA, 1) quantize_rows_kernel(const __grid_cons
       for (int j = 0; j < PAIRS; ++j) m = max_abs(m, x[i].v[j]);
     }
     m = t.template reduce<false, true, false>(RowStats{0.f, 0.f, m}).mh;
-    const float sc = row_scale(m), inv = row_inverse(sc);
-    const F2 inv2(inv, inv);
+    const float sc = row_scale(m);
+    const RowInverse2 inv(row_inverse<sizeof(T) == 2>(sc, m));
     const uint32_t keep = not_finite(m) ? 0u : FULL;
     int8_t* qp = q + t.row * ld;
-    FOR_PIECES(i, c) store_q<VEC, TEAM>(qp, c, F, x[i], inv2, keep);
+    FOR_PIECES(i, c) store_q<VEC, TEAM, sizeof(T) == 2>(qp, c, F, x[i], inv, keep);
     for (long long c = F + t.tid; c < ld; c += TEAM) qp[c] = 0;
     if (t.tid == 0) scale[t.row] = sc;
   }
@@ -410,9 +439,10 @@ __global__ void __launch_bounds__(1024) quantize_long_rows_kernel(const T* x, in
     RowStats s{0.f, 0.f, 0.f};
     for (int c = threadIdx.x; c < F; c += blockDim.x) s.mh = max_abs(s.mh, load_one(xp + c), 0.f);
     s = block_reduce(s, red);
-    const float sc = row_scale(s.mh), inv = row_inverse(sc);
+    const float sc = row_scale(s.mh);
+    const RowInverse inv = row_inverse<sizeof(T) == 2>(sc, s.mh);
     const uint32_t keep = not_finite(s.mh) ? 0u : FULL;
-    for (long long c = threadIdx.x; c < ld; c += blockDim.x) q[row * ld + c] = round1(c < F ? load_one(xp + c) : 0.f, inv, keep);
+    for (long long c = threadIdx.x; c < ld; c += blockDim.x) q[row * ld + c] = round1<sizeof(T) == 2>(c < F ? load_one(xp + c) : 0.f, inv, keep);
     if (threadIdx.x == 0) scale[row] = sc;
     __syncthreads();
   }
@@ -481,7 +511,7 @@ struct NormQ8Args {
   float eps;
 };
 struct NormScales {
-  float rstd, ys, hs, yi, hi;
+  float rstd, ys, hs;
   uint32_t keep;
 };
 __device__ __forceinline__ NormScales norm_scales(const RowStats& s, float inv_f, float eps) {
@@ -494,8 +524,6 @@ __device__ __forceinline__ NormScales norm_scales(const RowStats& s, float inv_f
   r.rstd = bad ? ROWS8_NAN : t;
   r.ys = bad ? ROWS8_NAN : row_scale(s.my * r.rstd);
   r.hs = bad ? ROWS8_NAN : row_scale(s.mh);
-  r.yi = row_inverse(r.ys);
-  r.hi = row_inverse(r.hs);
   return r;
 }
 __device__ __forceinline__ void norm_row_done(const NormQ8Args& a, const NormScales& r, long long row) {
@@ -545,18 +573,19 @@ __global__ void __launch_bounds__(CTA, 1) rmsnorm_q8_kernel(const __grid_constan
     s.sq = even + odd;
     s = t.template reduce<true, true, true>(s);
     const NormScales r = norm_scales(s, inv_f, a.eps);
-    const F2 rstd(r.rstd, r.rstd), yi(r.yi, r.yi), hi(r.hi, r.hi);
+    const F2 rstd(r.rstd, r.rstd);
+    const RowInverse2 yi(row_inverse<true>(r.ys, s.my * r.rstd)), hi(row_inverse<false>(r.hs, s.mh));
     T* hp = a.h ? static_cast<T*>(a.h) + t.row * F : nullptr;
     int8_t* yq = a.yq + t.row * a.ld;
     int8_t* hq = a.hq ? a.hq + t.row * a.ld : nullptr;
     FOR_PIECES(i, c) {
       if (hp) store_piece<VEC, TEAM>(hp, c, F, h[i]);
-      if (hq) store_q<VEC, TEAM>(hq, c, F, h[i], hi, r.keep);
+      if (hq) store_q<VEC, TEAM, false>(hq, c, F, h[i], hi, r.keep);
       Piece<VEC> y;
       load_gamma<VEC, TEAM>(gamma, c, F, y);
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j) y.v[j] = mul2(mul2(h[i].v[j], rstd), y.v[j]);
-      store_q<VEC, TEAM>(yq, c, F, y, yi, r.keep);
+      store_q<VEC, TEAM, true>(yq, c, F, y, yi, r.keep);
     }
     for (long long c = F + t.tid; c < a.ld; c += TEAM) {
       yq[c] = 0;
@@ -587,14 +616,15 @@ __global__ void __launch_bounds__(1024) rmsnorm_q8_long_kernel(const NormQ8Args 
     }
     s = block_reduce(s, red);
     const NormScales n = norm_scales(s, 1.f / static_cast<float>(a.F), a.eps);
+    const RowInverse yi = row_inverse<true>(n.ys, s.my * n.rstd), hi = row_inverse<false>(n.hs, s.mh);
     for (long long c = threadIdx.x; c < a.ld; c += blockDim.x) {
       h = gm = 0.f;
       if (c < a.F) {
         in(c);
         if (a.h) store_one(static_cast<T*>(a.h) + row * a.F + c, h);
       }
-      if (a.hq) a.hq[row * a.ld + c] = round1(h, n.hi, n.keep);
-      a.yq[row * a.ld + c] = round1(h * n.rstd * gm, n.yi, n.keep);
+      if (a.hq) a.hq[row * a.ld + c] = round1<false>(h, hi, n.keep);
+      a.yq[row * a.ld + c] = round1<true>(h * n.rstd * gm, yi, n.keep);
     }
     if (threadIdx.x == 0) norm_row_done(a, n, row);
     __syncthreads();

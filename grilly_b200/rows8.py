@@ -157,7 +157,7 @@ class Rows8Ops:
     # ---- operators --------------------------------------------------------------------------
     def quantize_rows(self, x, out=None) -> Rows8:
         """``x`` (..., features) in 8-bit rows: per row scale = max|x| / 127 (at least 2^-126) and x / scale rounded to the
-        nearest integer, ties to even, so a value is off by at most scale / 2. A row with a NaN or an infinity reads back
+        nearest integer, ties to even (a tie is one of x / (max|x| / 127) in exact arithmetic), so a value is off by at most scale / 2. A row with a NaN or an infinity reads back
         as NaN. An activation's checkpoint, or a weight (out, in) with one scale per output channel for ``linear_q8``."""
         shape = self._shape(x, "x")
         y8 = self._rows8_out(out, shape)

@@ -279,8 +279,8 @@ int grilly_transpose_2d(grilly_ctx* ctx, const float* in_dev, float* out_dev, in
 /* ---- rows in 8 bits: written, multiplied and kept for the backward pass ---------------------------------------
  * A tensor in 8-bit rows is an int8 matrix q [rows][ld] (ld >= features, a multiple of 16; the base 16-byte aligned;
  * the buffer holds rows * ld bytes) and one fp32 scale per row; element (r, c) stands for q[r][c] * scale[r].
- * Written here: scale = max(max|row| / 127, 2^-126), q = x / scale rounded to the nearest integer (ties to even), so
- * |q| <= 127 and a value is off by at most scale / 2; a zero row is exact. A row that holds a NaN or an infinity gets
+ * Written here: scale = max(max|row| / 127, 2^-126), q = x / scale rounded to the nearest integer (ties to even; the
+ * quotient by the scale before its own rounding to fp32, so max|row| / 2 is a tie and gives 64), so |q| <= 127 and a value is off by at most scale / 2; a zero row is exact. A row that holds a NaN or an infinity gets
  * scale NaN and q = 0: every value read back from it is NaN. Bytes between features and ld are written as 0 and never
  * change a result when read. The reference has no 8-bit type (its layers store fp32, backend/fnn.py:1437-1489); these
  * stand beside its linear, RMSNorm and backward entry points. All are asynchronous on the context's stream, keep no

@@ -25,11 +25,12 @@ def scale_of(amax):
 
 
 def quantize(x):
-    """(q float64, scale fp32) of rows x (rows, features)."""
+    """(q float64, scale fp32) of rows x (rows, features). q is the quotient by the scale before its rounding to fp32."""
     x = np.asarray(x, dtype=np.float32)
-    s = scale_of(np.abs(x).max(-1))
+    a = np.abs(x).max(-1)
+    s = scale_of(a)
     with np.errstate(invalid="ignore"):
-        q = np.rint(x.astype(F64) / s[:, None].astype(F64))
+        q = np.rint(127.0 * x.astype(F64) / np.maximum(a.astype(F64), 127.0 * 2.0 ** -126)[:, None])
     return np.where(np.isnan(q), 0.0, q), s
 
 

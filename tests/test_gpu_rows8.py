@@ -74,6 +74,42 @@ def test_quantize_and_read_back(backend, rows, features, dtype):
     assert np.array_equal(half, R.bf16(want.astype(np.float32)))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("features", [384, 1001, 17000])
+def test_ties_go_to_the_even_integer(backend, features, dtype):
+    """Rows whose scale is m 2^j: every second value on half its grid is an exact tie of x / scale."""
+    rng = rng_for(27, features)
+    ms = [1, 1, 1, 1] if dtype == "bf16" else [1, 3, 5, 7, 11, 13, 23, 101, 641, 8191]     # 127 m 2^j is a bf16 number for m = 1
+    x = np.stack([m * (rng.integers(-253, 254, features) / 2.0) * 2.0 ** (3 * i - 20) for i, m in enumerate(ms)]).astype(np.float32)
+    if dtype == "bf16":
+        x = R.bf16(x)
+    for i, m in enumerate(ms):
+        x[i, rng.integers(features)] = 127 * m * 2.0 ** (3 * i - 20)
+    q, s = R.quantize(x)
+    assert np.array_equal(s, [np.float32(m * 2.0 ** (3 * i - 20)) for i, m in enumerate(ms)])
+    assert np.mean(np.abs(x / s[:, None] % 1) == 0.5) > 0.2
+    xd = backend.device.upload(x, dtype)
+    got = backend.fnn.rmsnorm_residual_q8(xd, backend.device.upload(np.zeros_like(x), dtype), keep=True).h8
+    for r8 in (backend.fnn.quantize_rows(xd), got):
+        assert np.array_equal(r8.scale.numpy(), s) and np.array_equal(r8.q.numpy()[:, :features], q)
+
+
+@pytest.mark.parametrize("features", [384, 1001, 17000])
+def test_half_of_the_largest_value(backend, features):
+    """x = amax / 2 is 127 / 2 steps, a tie, however the scale itself is rounded: q = 64."""
+    b, ms = backend, np.arange(128, 256)
+    x = rng_for(28, features).uniform(-128, 128, (128, features))
+    x[:, 1::7] = ms[:, None] * np.where(np.arange(len(x[0, 1::7])) % 2, 1.0, -1.0)
+    x[:, 3::7] = x[:, 1::7][:, :x[:, 3::7].shape[1]] / 2
+    x = R.bf16((x * np.exp2(ms % 60 - 30.0)[:, None]).astype(np.float32))
+    want, s = R.quantize(x)
+    assert np.all(np.abs(want[:, 3::7]) == 64)
+    xd = b.device.upload(x, "bf16")
+    kept = b.fnn.rmsnorm_residual_q8(xd, b.device.upload(np.zeros_like(x), "bf16"), keep=True).h8
+    for r8 in (b.fnn.quantize_rows(xd), kept, b.fnn.quantize_rows(b.device.upload(x))):
+        assert np.array_equal(r8.scale.numpy(), s) and np.array_equal(r8.q.numpy()[:, :features], want)
+
+
 def test_rows_that_are_zero_tiny_or_not_finite(backend):
     x = acts(rng_for(2), 12, 130)
     x[0] = 0
