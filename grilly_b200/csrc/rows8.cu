@@ -5,9 +5,13 @@
 // threads on each (32 values per thread). Every team has a ring of rows in shared memory that bulk copies fill several rows
 // ahead, so that memory is read all the time and not only while a block has nothing else to do (blocks that each load,
 // reduce and store a row reached half the bandwidth). A row goes from there into registers, is reduced once and written once.
-// Rows that start off 16-byte boundaries (odd lengths) are copied from the boundary below and read value by value.
+// Rows that start off 16-byte boundaries (odd lengths) are copied from the boundary below and shifted into place as they are
+// read (load_piece); 16-bit and 32-bit results leave in the vectors that memory has, 8-bit rows start on boundaries always.
 // 16384 x 4096 bf16: the norm with both outputs 91 us (5.9 TB/s), its backward pass with the residual's gradient 86 us
 // (5.5 TB/s), quantise 40 us (5.0 TB/s), read back 35 us (5.8 TB/s); a plain copy runs at 6.5 TB/s.
+// 16384 x 4001 bf16: 129 us (4.1 TB/s), 133 (3.5), 55 (3.6) and 36 (5.5); fp32: 191 us (4.8), 185 (4.6), 69 (4.8). The
+// shifts are the difference: half of the issue slots are used, by 66 % more instructions than for aligned rows. Read and
+// stored value by value the same took 177, 146, 79 and 59 us in bf16; only fp32's backward pass was faster, 171.
 #include "rows8.h"
 #include "rows8_sum.cuh"
 #include "ptx.cuh"
@@ -37,11 +41,11 @@ __device__ __forceinline__ float warp_sum(float v) {
 __device__ __forceinline__ float warp_max(float v) { return __uint_as_float(__reduce_max_sync(FULL, __float_as_uint(v))); }
 __device__ __forceinline__ bool not_finite(float magnitude) { return __float_as_uint(magnitude) >= INF_BITS; }
 
-// A piece of a row, as a thread holds it in pairs: VEC neighbouring values (16 bytes of T), or where rows are not on 16-byte
-// boundaries (VEC = 1) two values that lie a team apart, so that neighbouring lanes still touch neighbouring values.
+// A piece of a row, as a thread holds it in pairs: VEC neighbouring values (16 bytes of T) from a column that is a multiple
+// of VEC, wherever the row starts in memory.
 template <int VEC>
 struct Piece {
-  static constexpr int WIDTH = VEC == 1 ? 2 : VEC, PAIRS = WIDTH / 2;
+  static constexpr int PAIRS = VEC / 2;
   F2 v[PAIRS];
 };
 __device__ __forceinline__ void load_vec(const float* p, Piece<4>& x) {
@@ -63,37 +67,130 @@ __device__ __forceinline__ float load_one(const float* p) { return *p; }
 __device__ __forceinline__ float load_one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ void store_one(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_one(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
-// the piece at column c of a row of F values (0 past its end)
-template <int VEC, int TEAM, class T>
-__device__ __forceinline__ void load_piece(const T* row, int c, int F, Piece<VEC>& x) {
-  if constexpr (VEC == 1) x.v[0] = F2(load_one(row + c), c + TEAM < F ? load_one(row + c + TEAM) : 0.f);
-  else load_vec(row + c, x);
+__device__ __forceinline__ void from_words(const uint32_t* w, Piece<4>& x) {
+  x.v[0] = F2(__uint_as_float(w[0]), __uint_as_float(w[1]));
+  x.v[1] = F2(__uint_as_float(w[2]), __uint_as_float(w[3]));
 }
-template <int VEC, int TEAM, class T>
-__device__ __forceinline__ void store_piece(T* row, int c, int F, const Piece<VEC>& x) {
-  if constexpr (VEC == 1) {
-    float a, b;
-    x.v[0].get(a, b);
-    store_one(row + c, a);
-    if (c + TEAM < F) store_one(row + c + TEAM, b);
+__device__ __forceinline__ void from_words(const uint32_t* w, Piece<8>& x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x.v[i] = F2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
+// The piece at column c of a row of F values (0 past its end) in shared memory. ODD: rows are not on 16-byte boundaries;
+// the row starts `off` bytes behind `row`. Two vectors then hold the piece, and what belongs to it is shifted out of them:
+// by words with two selections, by half a word with a funnel shift, the same for all threads. (Values read one by one
+// took twice as long: two thirds of the instructions of a kernel were loads and conversions.)
+template <bool ODD, int VEC, class T>
+__device__ __forceinline__ void load_piece(const uint8_t* row, int off, int c, int F, Piece<VEC>& x) {
+  const uint8_t* p = row + c * sizeof(T);
+  if constexpr (!ODD) {
+    load_vec(reinterpret_cast<const T*>(p), x);
   } else {
-    store_vec(row + c, x);
+    uint32_t w[6];
+    if constexpr (sizeof(T) == 4) {
+      const uint4 a = *reinterpret_cast<const uint4*>(p), b = *reinterpret_cast<const uint4*>(p + 16);
+      const uint32_t v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int k = 0; k < 5; ++k) w[k] = off & 8 ? v[k + 2] : v[k];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = off & 4 ? w[k + 1] : w[k];
+    } else {
+      const uint2* p8 = reinterpret_cast<const uint2*>(p + (off & 8));
+      const uint2 a = p8[0], b = p8[1], d = p8[2];
+      const uint32_t v[6] = {a.x, a.y, b.x, b.y, d.x, d.y};
+#pragma unroll
+      for (int k = 0; k < 5; ++k) w[k] = off & 4 ? v[k + 1] : v[k];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], (off & 2) * 8);
+    }
+    if (c + VEC > F) {
+      constexpr int PER_WORD = 4 / sizeof(T);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int left = F - c - k * PER_WORD;
+        if (left <= 0) w[k] = 0;
+        else if (left < PER_WORD) w[k] &= 0xffffu;
+      }
+    }
+    from_words(w, x);
   }
+}
+// Writes a piece to its place in such a row, in shared memory.
+__device__ __forceinline__ void place_piece(uint8_t* row, int off, int c, const Piece<4>& x) {
+  uint32_t* p = reinterpret_cast<uint32_t*>(row + off + c * 4);
+  float f[4];
+  x.v[0].get(f[0], f[1]);
+  x.v[1].get(f[2], f[3]);
+  if (off & 4) {
+    p[0] = __float_as_uint(f[0]);
+    *reinterpret_cast<F2*>(p + 1) = F2(f[1], f[2]);
+    p[3] = __float_as_uint(f[3]);
+  } else {
+    *reinterpret_cast<F2*>(p) = x.v[0];
+    *reinterpret_cast<F2*>(p + 2) = x.v[1];
+  }
+}
+__device__ __forceinline__ void place_piece(uint8_t* row, int off, int c, const Piece<8>& x) {
+  uint8_t* p = row + off + c * 2;
+  uint32_t w[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) w[k] = x.v[k].bf16();
+  if (off & 2) {
+    *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w[0]);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) *reinterpret_cast<uint32_t*>(p + 2 + 4 * k) = __funnelshift_r(w[k], w[k + 1], 16);
+    *reinterpret_cast<uint16_t*>(p + 14) = static_cast<uint16_t>(w[3] >> 16);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) *reinterpret_cast<uint32_t*>(p + 4 * k) = w[k];
+  }
+}
+// Stores the 16 bytes of a row (F values at `row` in memory, which lies `off` bytes behind a boundary) that start `at` bytes
+// behind that boundary; at the row's ends only what belongs to it.
+template <class T>
+__device__ __forceinline__ void store_between(T* row, int off, int at, int F, uint4 x) {
+  const int from = at - off, end = F * static_cast<int>(sizeof(T));
+  uint8_t* p = reinterpret_cast<uint8_t*>(row) + from;
+  if (from >= 0 && from + 16 <= end) {
+    *reinterpret_cast<uint4*>(p) = x;
+  } else {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int k = 0; k < 16; k += sizeof(T)) {
+      if (from + k < 0 || from + k >= end) continue;
+      if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(p + k) = w[k / 4];
+      else *reinterpret_cast<uint16_t*>(p + k) = static_cast<uint16_t>(w[k / 4] >> (k % 4 * 8));
+    }
+  }
+}
+// The sums of 16 bytes of values, each rounded to T. (Of two bf16 numbers the sum rounded once is the fp32 sum rounded to
+// bf16: where the fp32 sum is not exact, the smaller one is too small to move the larger.)
+template <class T>
+__device__ __forceinline__ uint4 add16(uint4 a, uint4 b) {
+  const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+  uint32_t s[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (sizeof(T) == 4) {
+      s[k] = __float_as_uint(__uint_as_float(x[k]) + __uint_as_float(y[k]));
+    } else {
+      const __nv_bfloat162 t = __hadd2_rn(*reinterpret_cast<const __nv_bfloat162*>(&x[k]), *reinterpret_cast<const __nv_bfloat162*>(&y[k]));
+      s[k] = *reinterpret_cast<const uint32_t*>(&t);
+    }
+  }
+  return make_uint4(s[0], s[1], s[2], s[3]);
 }
 // Gamma in shared memory: as it is, or for pieces of 8 first every piece's first four values, then every piece's last four
 // (neighbouring lanes then read neighbouring 16 bytes instead of every second 16).
 template <int VEC>
 __device__ __forceinline__ int gamma_at(int col, int F) {
-  return VEC == 8 ? ((col >> 2) & 1) * (F >> 1) + (col >> 3) * 4 + (col & 3) : col;
+  return VEC == 8 ? ((col >> 2) & 1) * ((F + 7) / 8 * 4) + (col >> 3) * 4 + (col & 3) : col;
 }
 // the columns' fp32 parameters (1 where there are none)
-template <int VEC, int TEAM>
+template <int VEC>
 __device__ __forceinline__ void load_gamma(const float* gamma, int c, int F, Piece<VEC>& g) {
   if (!gamma) {
 #pragma unroll
     for (int j = 0; j < Piece<VEC>::PAIRS; ++j) g.v[j] = F2(1.f, 1.f);
-  } else if constexpr (VEC == 1) {
-    g.v[0] = F2(gamma[c], c + TEAM < F ? gamma[c + TEAM] : 0.f);
   } else {
 #pragma unroll
     for (int j = 0; j < VEC; j += 4) {
@@ -155,18 +252,12 @@ template <bool ONE>
 __device__ __forceinline__ int8_t round1(float x, RowInverse inv, uint32_t keep) {
   return static_cast<int8_t>(__float_as_uint(ONE ? fmaf(x, inv.hi, MAGIC) : __fadd_rn(fmaf(x, inv.hi, __fmul_rn(x, inv.lo)), MAGIC)) & keep);
 }
-template <int VEC, int TEAM, bool ONE>
-__device__ __forceinline__ void store_q(int8_t* row, int c, int F, const Piece<VEC>& x, const RowInverse2& inv, uint32_t keep) {
-  if constexpr (VEC == 8) {
-    *reinterpret_cast<uint2*>(row + c) = make_uint2(round4<ONE>(x.v[0], x.v[1], inv) & keep, round4<ONE>(x.v[2], x.v[3], inv) & keep);
-  } else if constexpr (VEC == 4) {
-    *reinterpret_cast<uint32_t*>(row + c) = round4<ONE>(x.v[0], x.v[1], inv) & keep;
-  } else {
-    float a, b;
-    quotient2<ONE>(x.v[0], inv).get(a, b);
-    row[c] = static_cast<int8_t>(__float_as_uint(a) & keep);
-    if (c + TEAM < F) row[c + TEAM] = static_cast<int8_t>(__float_as_uint(b) & keep);
-  }
+// (8-bit rows start on 16-byte boundaries and have room for whole pieces)
+template <bool ONE, int VEC>
+__device__ __forceinline__ void store_q(int8_t* row, int c, const Piece<VEC>& x, const RowInverse2& inv, uint32_t keep) {
+  const uint32_t w = round4<ONE>(x.v[0], x.v[1], inv) & keep;
+  if constexpr (VEC == 8) *reinterpret_cast<uint2*>(row + c) = make_uint2(w, round4<ONE>(x.v[2], x.v[3], inv) & keep);
+  else *reinterpret_cast<uint32_t*>(row + c) = w;
 }
 // four signed bytes as floats: byte + 128 below the bits of 2^23, then the offset taken off; exact
 __device__ __forceinline__ void unpack4(uint32_t w, F2& lo, F2& hi) {
@@ -175,16 +266,14 @@ __device__ __forceinline__ void unpack4(uint32_t w, F2& lo, F2& hi) {
   lo = add2(F2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440)), __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7441))), offset);
   hi = add2(F2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7442)), __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7443))), offset);
 }
-template <int VEC, int TEAM>
-__device__ __forceinline__ void load_q(const int8_t* row, int c, int F, Piece<VEC>& x) {
+template <int VEC>
+__device__ __forceinline__ void load_q(const uint8_t* row, int c, Piece<VEC>& x) {
   if constexpr (VEC == 8) {
     const uint2 t = *reinterpret_cast<const uint2*>(row + c);
     unpack4(t.x, x.v[0], x.v[1]);
     unpack4(t.y, x.v[2], x.v[3]);
-  } else if constexpr (VEC == 4) {
-    unpack4(*reinterpret_cast<const uint32_t*>(row + c), x.v[0], x.v[1]);
   } else {
-    x.v[0] = F2(static_cast<float>(row[c]), c + TEAM < F ? static_cast<float>(row[c + TEAM]) : 0.f);
+    unpack4(*reinterpret_cast<const uint32_t*>(row + c), x.v[0], x.v[1]);
   }
 }
 
@@ -254,7 +343,7 @@ struct Team {
     }
     float* gm = reinterpret_cast<float*>(smem + g.gamma_at);
     if (gamma)
-      for (int c = threadIdx.x; c < g.F; c += CTA) gm[gamma_at<VEC>(c, g.F)] = __ldg(gamma + c);
+      for (int c = threadIdx.x; c < (g.F + VEC - 1) / VEC * VEC; c += CTA) gm[gamma_at<VEC>(c, g.F)] = c < g.F ? __ldg(gamma + c) : 0.f;
     __syncthreads();
   }
   // the team's lanes of its warp (a team of 16: half a warp)
@@ -328,15 +417,17 @@ struct Team {
     }
     return ok != 0;
   }
-  // the current row of tensor i: its first value
-  template <class T>
-  __device__ const T* values(int i) const {
-    return reinterpret_cast<const T*>(slot_of(slot) + g.at[i] + static_cast<int>(row * g.pitch[i] & 15));
-  }
-  // everything of the row has been read
+  // the current row of tensor i, from the 16-byte boundary at or before its first value, and that value's distance
+  __device__ uint8_t* bytes(int i) const { return slot_of(slot) + g.at[i]; }
+  __device__ int off(int i) const { return static_cast<int>(row * g.pitch[i] & 15); }
+  // everything of the row has been read. WROTE: its slot was written to as well, before a bulk copy fills it
+  template <bool WROTE>
   __device__ void done() {
     sync();
-    if (tid == 0) fetch(row + g.depth * step, slot);
+    if (tid == 0) {
+      if (WROTE) fence_proxy_async_smem();
+      fetch(row + g.depth * step, slot);
+    }
     row += step;
     if (++slot == g.depth) {
       slot = 0;
@@ -382,8 +473,8 @@ struct Team {
 // The pieces of a row that a thread has: i counts them, c is the first column. Rows shorter than a team's full width leave
 // the loop for all threads at once.
 #define FOR_PIECES(i, c)                                                                       \
-  _Pragma("unroll") for (int i = 0, c = t.tid * VEC; i < NV; ++i, c += TEAM * Piece<VEC>::WIDTH) \
-    if (i * TEAM * Piece<VEC>::WIDTH >= F) break;                                              \
+  _Pragma("unroll") for (int i = 0, c = t.tid * VEC; i < NV; ++i, c += TEAM * VEC) \
+    if (i * TEAM * VEC >= F) break;                                              \
     else if (c < F)
 
 // ---- a row per block of 1024 threads, for what the ring does not take
@@ -402,20 +493,21 @@ __device__ __forceinline__ RowStats block_reduce(RowStats s, RowStats* red) {
 }
 
 // ---------------------------------------------------------------- quantise
-template <class T, int VEC, int TEAM>
+template <class T, int TEAM, bool ODD>
 __global__ void __launch_bounds__(CTA, 1) quantize_rows_kernel(const __grid_constant__ Ring ring, int8_t* q, float* scale, long long ld) {
-  constexpr int NV = PER_THREAD / Piece<VEC>::WIDTH, PAIRS = Piece<VEC>::PAIRS;
+  constexpr int VEC = 16 / sizeof(T), NV = PER_THREAD / VEC, PAIRS = Piece<VEC>::PAIRS;
   extern __shared__ __align__(16) uint8_t smem[];
   Team<TEAM> t(ring, smem);
   t.template start<VEC>(nullptr);
   const int F = ring.F;
-  for (; t.row < ring.rows; t.done()) {
+  for (; t.row < ring.rows; t.template done<false>()) {
     if (!t.next()) break;
-    const T* xp = t.template values<T>(0);
+    const uint8_t* xp = t.bytes(0);
+    const int off = ODD ? t.off(0) : 0;
     Piece<VEC> x[NV];
     float m = 0.f;
     FOR_PIECES(i, c) {
-      load_piece<VEC, TEAM>(xp, c, F, x[i]);
+      load_piece<ODD, VEC, T>(xp, off, c, F, x[i]);
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j) m = max_abs(m, x[i].v[j]);
     }
@@ -424,8 +516,8 @@ __global__ void __launch_bounds__(CTA, 1) quantize_rows_kernel(const __grid_cons
     const RowInverse2 inv(row_inverse<sizeof(T) == 2>(sc, m));
     const uint32_t keep = not_finite(m) ? 0u : FULL;
     int8_t* qp = q + t.row * ld;
-    FOR_PIECES(i, c) store_q<VEC, TEAM, sizeof(T) == 2>(qp, c, F, x[i], inv, keep);
-    for (long long c = F + t.tid; c < ld; c += TEAM) qp[c] = 0;
+    FOR_PIECES(i, c) store_q<sizeof(T) == 2>(qp, c, x[i], inv, keep);
+    for (long long c = (F + VEC - 1) / VEC * VEC + t.tid; c < ld; c += TEAM) qp[c] = 0;
     if (t.tid == 0) scale[t.row] = sc;
   }
   t.end();
@@ -481,7 +573,66 @@ __global__ void __launch_bounds__(256) dequantize_vec_kernel(const int8_t* __res
     }
   }
 }
-// Any row length: one warp per row.
+// Row lengths that are no multiple of 16: the values in the order of memory, 8 to a thread from a 16-byte boundary on,
+// whichever row they belong to. Their bytes are shifted out of the two aligned 8-byte words that hold them; pieces that
+// reach into the next row go value by value. The caller made sure that the values can be counted in 32 bits.
+template <class T>
+__device__ __forceinline__ void store8(T* p, const F2* v) {
+  if constexpr (sizeof(T) == 2) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(v[0].bf16(), v[1].bf16(), v[2].bf16(), v[3].bf16());
+  } else {
+    reinterpret_cast<ulonglong2*>(p)[0] = make_ulonglong2(v[0].v, v[1].v);
+    reinterpret_cast<ulonglong2*>(p)[1] = make_ulonglong2(v[2].v, v[3].v);
+  }
+}
+template <class T>
+__global__ void __launch_bounds__(256) dequantize_odd_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale, T* __restrict__ y,
+                                                             uint32_t values, uint32_t F, long long ld) {
+  constexpr int AT_ONCE = 4;
+  const uint32_t pieces = (values + 7) / 8;
+  for (uint32_t base = blockIdx.x * (256u * AT_ONCE) + threadIdx.x; base < pieces; base += gridDim.x * (256u * AT_ONCE)) {
+    uint2 lo[AT_ONCE], hi[AT_ONCE];
+    float s[AT_ONCE];
+    uint32_t row[AT_ONCE], col[AT_ONCE];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const uint32_t i = min(base + u * 256u, pieces - 1);
+      row[u] = i * 8 / F;
+      col[u] = i * 8 - row[u] * F;
+      const int8_t* p = q + row[u] * ld + (col[u] & ~7u);
+      lo[u] = *reinterpret_cast<const uint2*>(p);
+      hi[u] = (col[u] & 7) && col[u] + 8 <= F ? *reinterpret_cast<const uint2*>(p + 8) : make_uint2(0, 0);
+      s[u] = __ldg(scale + row[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const uint32_t i = base + u * 256u;
+      if (i >= pieces) break;
+      T* yp = y + static_cast<long long>(i) * 8;
+      if (col[u] + 8 <= F) {
+        const bool words = col[u] & 4;
+        const uint32_t bits = (col[u] & 3) * 8, a = words ? lo[u].y : lo[u].x, b = words ? hi[u].x : lo[u].y, c = words ? hi[u].y : hi[u].x;
+        const F2 s2(s[u], s[u]);
+        F2 v[4];
+        unpack4(__funnelshift_r(a, b, bits), v[0], v[1]);
+        unpack4(__funnelshift_r(b, c, bits), v[2], v[3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = mul2(v[j], s2);
+        store8(yp, v);
+      } else {
+        uint32_t r = row[u], c = col[u];
+        for (uint32_t j = 0; j < min(8u, values - i * 8); ++j) {
+          store_one(yp + j, static_cast<float>(q[r * ld + c]) * __ldg(scale + r));
+          if (++c == F) {
+            c = 0;
+            ++r;
+          }
+        }
+      }
+    }
+  }
+}
+// What that does not take: one warp per row.
 template <class T>
 __global__ void __launch_bounds__(256) dequantize_any_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale, T* __restrict__ y,
                                                              long long rows, int F, long long ld) {
@@ -534,32 +685,50 @@ __device__ __forceinline__ void norm_row_done(const NormQ8Args& a, const NormSca
 
 // One reduction serves both outputs: the largest |h gamma| times rstd is the largest |y|, so sum h^2, max |h gamma| and
 // max |h| are taken together and nothing waits for rstd. A row has been read whole before h is written (in place).
-template <class T, int VEC, int TEAM>
+template <class T, int TEAM, bool ODD>
 __global__ void __launch_bounds__(CTA, 1) rmsnorm_q8_kernel(const __grid_constant__ Ring ring, const NormQ8Args a) {
-  constexpr int NV = PER_THREAD / Piece<VEC>::WIDTH, PAIRS = Piece<VEC>::PAIRS;
+  constexpr int VEC = 16 / sizeof(T), NV = PER_THREAD / VEC, PAIRS = Piece<VEC>::PAIRS;
   extern __shared__ __align__(16) uint8_t smem[];
   Team<TEAM> t(ring, smem);
   t.template start<VEC>(a.gamma);
   const float* gamma = a.gamma ? reinterpret_cast<const float*>(smem + ring.gamma_at) : nullptr;
   const int F = ring.F;
   const float inv_f = 1.f / static_cast<float>(F);
-  for (; t.row < ring.rows; t.done()) {
+  for (; t.row < ring.rows; t.template done<ODD && sizeof(T) == 4>()) {
     if (!t.next()) break;
-    const T* xp = t.template values<T>(0);
-    const T* rp = ring.tensors > 1 ? t.template values<T>(1) : nullptr;
+    uint8_t* xp = t.bytes(0);
+    const uint8_t* rp = ring.tensors > 1 ? t.bytes(1) : nullptr;
+    const int off = ODD ? t.off(0) : 0;   // of x, residual and h alike
+    T* hp = a.h ? static_cast<T*>(a.h) + t.row * F : nullptr;
+    // x, residual and h have their own boundaries in common: h is written in their vectors, and where it is fp32 the sum
+    // takes x's place in the ring, so that one tensor is left to be shifted.
+    constexpr bool ADD_FIRST = ODD && sizeof(T) == 4;
+    auto write_h = [&]() {
+      const int end = off + F * static_cast<int>(sizeof(T));
+      for (int at = t.tid * 16; at < end; at += TEAM * 16) {
+        uint4 v = *reinterpret_cast<const uint4*>(xp + at);
+        if (rp) v = add16<T>(v, *reinterpret_cast<const uint4*>(rp + at));
+        if (ADD_FIRST && rp) *reinterpret_cast<uint4*>(xp + at) = v;
+        if (hp) store_between(hp, off, at, F, v);
+      }
+    };
+    if (ADD_FIRST) {
+      write_h();
+      t.sync();
+    }
     Piece<VEC> h[NV];
     F2 sum[2] = {F2(0.f, 0.f), F2(0.f, 0.f)};
     RowStats s{0.f, 0.f, 0.f};
     FOR_PIECES(i, c) {
-      load_piece<VEC, TEAM>(xp, c, F, h[i]);
-      if (rp) {
+      load_piece<ODD, VEC, T>(xp, off, c, F, h[i]);
+      if (!ADD_FIRST && rp) {
         Piece<VEC> r;
-        load_piece<VEC, TEAM>(rp, c, F, r);
+        load_piece<ODD, VEC, T>(rp, off, c, F, r);
 #pragma unroll
         for (int j = 0; j < PAIRS; ++j) h[i].v[j] = add2(h[i].v[j], r.v[j]);
       }
       Piece<VEC> gm;
-      load_gamma<VEC, TEAM>(gamma, c, F, gm);
+      load_gamma(gamma, c, F, gm);
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j) {
         F2& acc = sum[(i * PAIRS + j) & 1];
@@ -575,19 +744,19 @@ __global__ void __launch_bounds__(CTA, 1) rmsnorm_q8_kernel(const __grid_constan
     const NormScales r = norm_scales(s, inv_f, a.eps);
     const F2 rstd(r.rstd, r.rstd);
     const RowInverse2 yi(row_inverse<true>(r.ys, s.my * r.rstd)), hi(row_inverse<false>(r.hs, s.mh));
-    T* hp = a.h ? static_cast<T*>(a.h) + t.row * F : nullptr;
     int8_t* yq = a.yq + t.row * a.ld;
     int8_t* hq = a.hq ? a.hq + t.row * a.ld : nullptr;
     FOR_PIECES(i, c) {
-      if (hp) store_piece<VEC, TEAM>(hp, c, F, h[i]);
-      if (hq) store_q<VEC, TEAM, false>(hq, c, F, h[i], hi, r.keep);
+      if (!ODD && hp) store_vec(hp + c, h[i]);
+      if (hq) store_q<false>(hq, c, h[i], hi, r.keep);
       Piece<VEC> y;
-      load_gamma<VEC, TEAM>(gamma, c, F, y);
+      load_gamma(gamma, c, F, y);
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j) y.v[j] = mul2(mul2(h[i].v[j], rstd), y.v[j]);
-      store_q<VEC, TEAM, true>(yq, c, F, y, yi, r.keep);
+      store_q<true>(yq, c, y, yi, r.keep);
     }
-    for (long long c = F + t.tid; c < a.ld; c += TEAM) {
+    if (ODD && !ADD_FIRST && hp) write_h();
+    for (long long c = (F + VEC - 1) / VEC * VEC + t.tid; c < a.ld; c += TEAM) {
       yq[c] = 0;
       if (hq) hq[c] = 0;
     }
@@ -648,9 +817,10 @@ struct NormBwdQ8Args {
 // A thread keeps the same columns of every row that its team meets, so the gradient of gamma is summed in registers and
 // leaves once per CTA; the CTAs' sums are added by sum_partials_kernel in a fixed order. The row is read from the ring
 // twice (before and after its one sum) instead of being held next to those sums.
-template <class T, int VEC, int TEAM>
+template <class T, int TEAM, bool ODD>
 __global__ void __launch_bounds__(CTA, 1) rmsnorm_bwd_kernel(const __grid_constant__ Ring ring, const NormBwdQ8Args a) {
-  constexpr int NV = PER_THREAD / Piece<VEC>::WIDTH, PAIRS = Piece<VEC>::PAIRS;
+  constexpr int VEC = 16 / sizeof(T), NV = PER_THREAD / VEC, PAIRS = Piece<VEC>::PAIRS;
+  constexpr bool ADD_LAST = ODD && sizeof(T) == 4;   // rstd and the residual's gradient come in as the row leaves the ring
   extern __shared__ __align__(16) uint8_t smem[];
   Team<TEAM> t(ring, smem);
   t.template start<VEC>(a.gamma);
@@ -662,19 +832,20 @@ __global__ void __launch_bounds__(CTA, 1) rmsnorm_bwd_kernel(const __grid_consta
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < PAIRS; ++j) acc[i].v[j] = F2(0.f, 0.f);
-  for (; t.row < ring.rows; t.done()) {
+  for (; t.row < ring.rows; t.template done<ODD>()) {
     const float rstd = __ldg(a.rstd + t.row), s = __ldg(a.hs + t.row) * rstd;
     const F2 s2(s, s), rstd2(rstd, rstd);
     if (!t.next()) break;
-    const int8_t* qp = t.template values<int8_t>(0);
-    const T* gp = t.template values<T>(1);
-    const T* rp = ring.tensors > 2 ? t.template values<T>(2) : nullptr;
+    const uint8_t* qp = t.bytes(0);
+    uint8_t* gp = t.bytes(1);
+    const uint8_t* rp = ring.tensors > 2 ? t.bytes(2) : nullptr;
+    const int off = ODD ? t.off(1) : 0;
     F2 dots[2] = {F2(0.f, 0.f), F2(0.f, 0.f)};
     FOR_PIECES(i, c) {
       Piece<VEC> g, n, gm;
-      load_piece<VEC, TEAM>(gp, c, F, g);
-      load_q<VEC, TEAM>(qp, c, F, n);
-      load_gamma<VEC, TEAM>(gamma, c, F, gm);
+      load_piece<ODD, VEC, T>(gp, off, c, F, g);
+      load_q(qp, c, n);
+      load_gamma(gamma, c, F, gm);
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j) {
         n.v[j] = mul2(n.v[j], s2);
@@ -690,20 +861,39 @@ __global__ void __launch_bounds__(CTA, 1) rmsnorm_bwd_kernel(const __grid_consta
     T* op = static_cast<T*>(a.gh) + t.row * F;
     FOR_PIECES(i, c) {
       Piece<VEC> g, n, r;
-      load_piece<VEC, TEAM>(gp, c, F, g);
-      load_q<VEC, TEAM>(qp, c, F, n);
-      load_gamma<VEC, TEAM>(gamma, c, F, r);
+      load_piece<ODD, VEC, T>(gp, off, c, F, g);
+      load_q(qp, c, n);
+      load_gamma(gamma, c, F, r);
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j) g.v[j] = fma2(n.v[j], back, mul2(g.v[j], r.v[j]));
-      if (rp) {
-        load_piece<VEC, TEAM>(rp, c, F, r);
+      if (ADD_LAST) {
+      } else if (rp) {
+        load_piece<ODD, VEC, T>(rp, off, c, F, r);
 #pragma unroll
         for (int j = 0; j < PAIRS; ++j) g.v[j] = fma2(g.v[j], rstd2, r.v[j]);
       } else {
 #pragma unroll
         for (int j = 0; j < PAIRS; ++j) g.v[j] = mul2(g.v[j], rstd2);
       }
-      store_piece<VEC, TEAM>(op, c, F, g);
+      if (ODD) place_piece(gp, off, c, g);   // its own bytes of grad_out, which nobody reads again
+      else store_vec(op + c, g);
+    }
+    if (ODD) {         // then out of the ring in the vectors that memory has
+      t.sync();
+      const int end = off + F * static_cast<int>(sizeof(T));
+      for (int at = t.tid * 16; at < end; at += TEAM * 16) {
+        uint4 v = *reinterpret_cast<const uint4*>(gp + at);
+        if constexpr (ADD_LAST) {
+          Piece<VEC> g, r;
+          load_vec(reinterpret_cast<const float*>(gp + at), g);
+          r.v[0] = r.v[1] = F2(-0.f, -0.f);
+          if (rp) load_vec(reinterpret_cast<const float*>(rp + at), r);
+#pragma unroll
+          for (int j = 0; j < PAIRS; ++j) g.v[j] = fma2(g.v[j], rstd2, r.v[j]);
+          v = make_uint4(static_cast<uint32_t>(g.v[0].v), static_cast<uint32_t>(g.v[0].v >> 32), static_cast<uint32_t>(g.v[1].v), static_cast<uint32_t>(g.v[1].v >> 32));
+        }
+        store_between(op, off, at, F, v);
+      }
     }
   }
   t.end();
@@ -717,9 +907,8 @@ __global__ void __launch_bounds__(CTA, 1) rmsnorm_bwd_kernel(const __grid_consta
     for (int j = 0; j < PAIRS; ++j) {
       float lo, hi;
       acc[i].v[j].get(lo, hi);
-      mine[c + 2 * j] = lo;
-      if (VEC > 1) mine[c + 2 * j + 1] = hi;
-      else if (c + TEAM < F) mine[c + TEAM] = hi;
+      if (!ODD || c + 2 * j < F) mine[c + 2 * j] = lo;
+      if (!ODD || c + 2 * j + 1 < F) mine[c + 2 * j + 1] = hi;
     }
   }
   __syncthreads();
@@ -774,7 +963,7 @@ bool aligned16(std::initializer_list<const void*> ps) {
 }
 constexpr int RING_BYTES = 216 * 1024;
 
-// The ring's geometry, for rows of up to 512 * 32 values of which two per team fit shared memory, on tensors that start on
+// The ring's geometry, for rows of up to 512 * 32 values that fit shared memory, on tensors that start on
 // 16-byte boundaries. It depends on the row's length alone, so a row's sums have the same order, and its
 // result the same bits, in every batch.
 struct RowTensor {
@@ -805,14 +994,15 @@ int make_ring(grilly_ctx* ctx, Ring& g, long long rows, int F, const RowTensor* 
     g.slot += (tensors[i].bytes + 15) / 16 * 16 + (tensors[i].pitch % 16 ? 16 : 0);
   }
   g.gamma_at = GAMMA_AT;
-  g.slots_at = GAMMA_AT + (gamma ? (4 * F + 15) / 16 * 16 : 0);
+  g.slots_at = GAMMA_AT + (gamma ? (F + 7) / 8 * 32 : 0);
   // the smallest team that holds a row, but few enough of them that each has two rows in shared memory: the threads that
-  // long rows leave without a row of their own join the others
+  // long rows leave without a row of their own join the others. Rows of which only one fits are loaded one after the other
+  // (5000 x 11001 fp32: the norm 189 us, its backward pass 199; read twice from memory instead 413 and 838)
   const int room = RING_BYTES - g.slots_at;
   int team = MIN_TEAM;
   while (team < CTA && (team * PER_THREAD < F || CTA / team * 2 * g.slot > room)) team *= 2;
   const int teams = CTA / team;
-  if (teams * 2 * g.slot > room) return 0;
+  if (teams * g.slot > room) return 0;
   *grid = static_cast<unsigned>(std::min<long long>(rows, ctx->num_sms));
   const long long per_team = (rows + static_cast<long long>(*grid) * teams - 1) / (static_cast<long long>(*grid) * teams);
   g.depth = static_cast<int>(std::min<long long>(std::min(MAX_DEPTH, room / (g.slot * teams)), per_team));
@@ -842,7 +1032,6 @@ unsigned any_grid(long long rows) { return static_cast<unsigned>(std::min<long l
 
 template <class T>
 int launch_quantize(grilly_ctx* ctx, const T* x, int8_t* q, float* scale, long long rows, int F, long long ld) {
-  constexpr int VEC = 16 / sizeof(T);
   Ring ring;
   size_t smem;
   unsigned grid;
@@ -853,7 +1042,7 @@ int launch_quantize(grilly_ctx* ctx, const T* x, int8_t* q, float* scale, long l
     return GRILLY_OK;
   }
   void (*kern)(const Ring, int8_t*, float*, long long) = nullptr;
-#define PICK(TEAM) kern = F % VEC == 0 ? quantize_rows_kernel<T, VEC, TEAM> : quantize_rows_kernel<T, 1, TEAM>
+#define PICK(TEAM) kern = ring.aligned ? quantize_rows_kernel<T, TEAM, false> : quantize_rows_kernel<T, TEAM, true>
   WITH_TEAM(team, PICK)
 #undef PICK
   if (int rc = allow_ring(ctx, kern)) return rc;
@@ -868,6 +1057,10 @@ void launch_dequantize(grilly_ctx* ctx, const int8_t* q, const float* scale, T* 
   if (F % 16 == 0 && aligned16({y}) && vectors < (1ll << 31)) {
     const unsigned grid = static_cast<unsigned>(std::min<long long>((vectors + 511) / 512, ctx->num_sms * 32ll));
     dequantize_vec_kernel<T><<<grid, 256, 0, st>>>(q, scale, y, static_cast<uint32_t>(vectors), static_cast<uint32_t>(F / 16), ld);
+  } else if (aligned16({y}) && rows * F < (1ll << 32) - 4096 && rows * F > 0) {
+    const long long pieces = (rows * F + 7) / 8;
+    const unsigned grid = static_cast<unsigned>(std::min<long long>((pieces + 1023) / 1024, ctx->num_sms * 16ll));
+    dequantize_odd_kernel<T><<<grid, 256, 0, st>>>(q, scale, y, static_cast<uint32_t>(rows * F), static_cast<uint32_t>(F), ld);
   } else {
     dequantize_any_kernel<T><<<any_grid((rows + 7) / 8), 256, 0, st>>>(q, scale, y, rows, F, ld);
   }
@@ -875,7 +1068,6 @@ void launch_dequantize(grilly_ctx* ctx, const int8_t* q, const float* scale, T* 
 
 template <class T>
 int launch_rmsnorm(grilly_ctx* ctx, const NormQ8Args& a) {
-  constexpr int VEC = 16 / sizeof(T);
   Ring ring;
   size_t smem;
   unsigned grid;
@@ -887,7 +1079,7 @@ int launch_rmsnorm(grilly_ctx* ctx, const NormQ8Args& a) {
     return GRILLY_OK;
   }
   void (*kern)(const Ring, const NormQ8Args) = nullptr;
-#define PICK(TEAM) kern = a.F % VEC == 0 ? rmsnorm_q8_kernel<T, VEC, TEAM> : rmsnorm_q8_kernel<T, 1, TEAM>
+#define PICK(TEAM) kern = ring.aligned ? rmsnorm_q8_kernel<T, TEAM, false> : rmsnorm_q8_kernel<T, TEAM, true>
   WITH_TEAM(team, PICK)
 #undef PICK
   if (int rc = allow_ring(ctx, kern)) return rc;
@@ -897,7 +1089,6 @@ int launch_rmsnorm(grilly_ctx* ctx, const NormQ8Args& a) {
 
 template <class T>
 int launch_rmsnorm_bwd(grilly_ctx* ctx, NormBwdQ8Args& a, float* grad_gamma) {
-  constexpr int VEC = 16 / sizeof(T);
   Rows8Scratch scratch(ctx);
   Ring ring;
   size_t smem;
@@ -907,7 +1098,7 @@ int launch_rmsnorm_bwd(grilly_ctx* ctx, NormBwdQ8Args& a, float* grad_gamma) {
   const int team = aligned16({a.gh}) ? make_ring(ctx, ring, a.rows, a.F, in, a.gr ? 3 : 2, a.gamma != nullptr, grad_gamma != nullptr, &smem, &grid) : 0;
   if (team) {
     void (*kern)(const Ring, const NormBwdQ8Args) = nullptr;
-#define PICK(TEAM) kern = a.F % VEC == 0 ? rmsnorm_bwd_kernel<T, VEC, TEAM> : rmsnorm_bwd_kernel<T, 1, TEAM>
+#define PICK(TEAM) kern = ring.aligned ? rmsnorm_bwd_kernel<T, TEAM, false> : rmsnorm_bwd_kernel<T, TEAM, true>
     WITH_TEAM(team, PICK)
 #undef PICK
     if (int rc = allow_ring(ctx, kern)) return rc;

@@ -178,6 +178,10 @@ def test_norm_in_place_and_into_given_tensors(backend):
     rng = rng_for(5)
     for features in (384, 1001, 20000):
         x, r = acts(rng, 50, features), acts(rng, 50, features)
+        xb, rb = R.bf16(x), R.bf16(r * np.exp2(rng.integers(-20, 20, r.shape)).astype(np.float32))
+        xd = backend.device.upload(xb, "bf16")
+        got = backend.fnn.rmsnorm_residual_q8(xd, backend.device.upload(rb, "bf16"), out=(None, xd, None, None)).h
+        assert got is xd and np.array_equal(xd.numpy(), R.bf16(xb + rb))
         want = backend.fnn.rmsnorm_residual_q8(backend.device.upload(x), backend.device.upload(r), keep=True)
         for which in (0, 1):
             xd, rd = backend.device.upload(x), backend.device.upload(r)
@@ -356,6 +360,23 @@ def test_rmsnorm_backward_q8(backend, rows, features, dtype):
     assert all(np.array_equal(s.numpy(), t.numpy()) for s, t in zip(a, b))
     if rows == 3:
         norm_backward_case(backend, rows, features, dtype, gamma=False, residual=False)
+
+
+@pytest.mark.parametrize("features,dtype", [(11001, "f32"), (16384, "f32"), (16001, "f32"), (12000, "f32"), (16383, "bf16"), (16384, "bf16")])
+def test_rows_that_fill_shared_memory(backend, features, dtype):
+    """More rows than the GPU holds at once, few or one of them in each block's shared memory."""
+    norm_backward_case(backend, 450, features, dtype)
+    test_rmsnorm_residual_q8(backend, 450, features, True, True, True, dtype)
+    test_quantize_and_read_back(backend, 450, features, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_rows_on_every_distance_from_a_boundary(backend, dtype):
+    """Row lengths of every remainder: rows start on every distance from a 16-byte boundary that there is."""
+    for features in range(1, 34):
+        norm_backward_case(backend, 900, features, dtype)
+        test_rmsnorm_residual_q8(backend, 900, features, True, True, True, dtype)
+        test_quantize_and_read_back(backend, 900, features, dtype)
 
 
 def test_norm_backward_against_differences(backend):
