@@ -205,29 +205,30 @@ __device__ __forceinline__ void gemm8_stage(uint8_t* stage, int lane, int p, uin
 }
 // The 16 columns from `first` on go to the warp's 2 KB of shared memory, rows of 64 bytes: 16 columns of 32 bits, or a half
 // (h) of 32 columns of bf16. A full row leaves by one TMA store, cut off at the edges of C; where C's rows are not on
-// 16-byte boundaries the lanes store 16 columns themselves.
+// 16-byte boundaries the lanes store the 64 bytes of a row themselves (16 bf16 columns at a time, 32 bytes, took 52 us
+// instead of 40 for 16384 x 385 x 1537).
 __device__ __forceinline__ void gemm8_write(const Gemm8Args& a, const CUtensorMap* tmap_out, const uint32_t (&r)[16], uint8_t* stage, long long row0,
                                             int out_row, int first, int h, int lane) {
   const bool half = a.out_bf16 && !a.raw;
-  if (!(a.wide_store && half && h == 1)) {
+  if (!(half && h == 1)) {
     // the warp's last store has left the staging rows (it may have been of the launch's other product, stored otherwise)
     if (lane == 0) tma_store_wait_read<0>();
     __syncwarp();
   }
+  if (half) {
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = F2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])).bf16();
+    gemm8_stage(stage, lane, 2 * h, w[0], w[1], w[2], w[3]);
+    gemm8_stage(stage, lane, 2 * h + 1, w[4], w[5], w[6], w[7]);
+    if (h == 0) return;
+    first -= 16;
+  } else {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) gemm8_stage(stage, lane, p, r[4 * p], r[4 * p + 1], r[4 * p + 2], r[4 * p + 3]);
+    if (first >= a.N) return;                                // the block's second half lies past C
+  }
   if (a.wide_store) {
-    if (half) {
-      uint32_t w[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = F2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])).bf16();
-      gemm8_stage(stage, lane, 2 * h, w[0], w[1], w[2], w[3]);
-      gemm8_stage(stage, lane, 2 * h + 1, w[4], w[5], w[6], w[7]);
-      if (h == 0) return;
-      first -= 16;
-    } else {
-#pragma unroll
-      for (int p = 0; p < 4; ++p) gemm8_stage(stage, lane, p, r[4 * p], r[4 * p + 1], r[4 * p + 2], r[4 * p + 3]);
-      if (first >= a.N) return;                              // the block's second half lies past C
-    }
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
@@ -236,17 +237,22 @@ __device__ __forceinline__ void gemm8_write(const Gemm8Args& a, const CUtensorMa
     }
     return;
   }
-#pragma unroll
-  for (int p = 0; p < 4; ++p) gemm8_stage(stage, lane, p, r[4 * p], r[4 * p + 1], r[4 * p + 2], r[4 * p + 3]);
   __syncwarp();
-  const int c = lane & 15, rows = static_cast<int>(a.M - row0 < 32 ? a.M - row0 : 32);
-  if (first + c < a.N) {
+  const int rows = static_cast<int>(a.M - row0 < 32 ? a.M - row0 : 32);
+  if (half) {
+    if (first + lane < a.N) {
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + row0 * a.ld_out + first + lane;
 #pragma unroll 8
-    for (int q = lane >> 4; q < rows; q += 2) {
-      const float v = *reinterpret_cast<const float*>(stage + q * 64 + (((c >> 2) ^ ((q >> 1) & 3)) << 4) + (c & 3) * 4);
-      const long long at = (row0 + q) * a.ld_out + first + c;
-      if (half) static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16(v);
-      else static_cast<float*>(a.out)[at] = v;
+      for (int q = 0; q < rows; ++q, out += a.ld_out)
+        *out = *reinterpret_cast<const __nv_bfloat16*>(stage + q * 64 + (((lane >> 3) ^ ((q >> 1) & 3)) << 4) + (lane & 7) * 2);
+    }
+  } else {
+    const int c = lane & 15;
+    if (first + c < a.N) {
+      float* out = static_cast<float*>(a.out) + (row0 + (lane >> 4)) * a.ld_out + first + c;
+#pragma unroll 8
+      for (int q = lane >> 4; q < rows; q += 2, out += 2 * a.ld_out)
+        *out = *reinterpret_cast<const float*>(stage + q * 64 + (((c >> 2) ^ ((q >> 1) & 3)) << 4) + (c & 3) * 4);
     }
   }
 }
