@@ -119,49 +119,76 @@ __device__ __forceinline__ void expand_piece(const uint4 w, float s, __nv_bfloat
   yp[0] = make_uint4(out[0], out[1], out[2], out[3]);
   yp[1] = make_uint4(out[4], out[5], out[6], out[7]);
 }
-// partial[block][n] = sum over the block's rows: 32 threads across with V columns each, 8 threads per column over every 8th
-// row, added in turn
-template <int V>
-__device__ __forceinline__ void sum_columns(const __nv_bfloat16* g, float* partial, long long M, int N, int across, int block, long long rows_per_block,
-                                            float (&part)[8][256]) {
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int n = (across * 32 + tx) * V;
-  const long long r0 = block * rows_per_block, r1 = min(M, r0 + rows_per_block);
-  const __nv_bfloat16* p = g + (r0 + ty) * N + n;
-  const long long step = 8ll * N;
-  if constexpr (V == 8) {
-    F2 acc[4] = {F2(0.f, 0.f), F2(0.f, 0.f), F2(0.f, 0.f), F2(0.f, 0.f)};
-    if (n < N) {
-#pragma unroll 8
-      for (long long r = r0 + ty; r < r1; r += 8, p += step) {
-        const uint4 t = __ldg(reinterpret_cast<const uint4*>(p));
-        const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+// 16 bytes from a 16-byte boundary on, 0 for values outside the tensor [first, last)
+__device__ __forceinline__ uint4 load16_inside(const uint8_t* p, const uint8_t* first, const uint8_t* last) {
+  if (p >= first && p + 16 <= last) return __ldg(reinterpret_cast<const uint4*>(p));
+  uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j] = add2(acc[j], F2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u)));
-      }
-    }
+  for (int j = 0; j < 8; ++j)
+    if (p + 2 * j >= first && p + 2 * j < last) w[j / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + 2 * j)) << (j % 2 * 16);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// 8 bf16 values wherever they start, those from `left` on as 0. ANY = false: on a 16-byte boundary, all inside.
+template <bool ANY>
+__device__ __forceinline__ uint4 load_8(const __nv_bfloat16* x, const uint8_t* first, const uint8_t* last, int left) {
+  const uint8_t* p = reinterpret_cast<const uint8_t*>(x);
+  if constexpr (!ANY) return __ldg(reinterpret_cast<const uint4*>(p));
+  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);
+  const uint4 a = load16_inside(p - off, first, last);
+  const uint4 b = 2 * left + off > 16 && off ? load16_inside(p - off + 16, first, last) : make_uint4(0, 0, 0, 0);
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[j].get(part[ty][(2 * j) * 32 + tx], part[ty][(2 * j + 1) * 32 + tx]);
-  } else {
-    float acc = 0.f;
-    if (n < N) {
-#pragma unroll 8
-      for (long long r = r0 + ty; r < r1; r += 8, p += step) acc += __bfloat162float(*p);
+  for (int k = 0; k < 6; ++k) w[k] = off & 8 ? w[k + 2] : w[k];
+#pragma unroll
+  for (int k = 0; k < 5; ++k) w[k] = off & 4 ? w[k + 1] : w[k];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], (off & 2) * 8);
+  if (left < 8) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (left <= 2 * k) w[k] = 0;
+      else if (left == 2 * k + 1) w[k] &= 0xffffu;
     }
-    part[ty][tx] = acc;
   }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// A block's rows of g, 256 columns of them: their sums to partial[block][n] (or null), and the rows themselves to a copy
+// whose rows are ld apart (or null). 32 threads across with 8 columns each, 8 threads per column over every 8th row, added
+// in turn. ANY: rows start anywhere (the 8 rows of a step have their own distances from a boundary, every step the same).
+template <bool ANY>
+__device__ __forceinline__ void sum_columns(const __nv_bfloat16* g, float* partial, __nv_bfloat16* copy, int ld, long long M, int N, int across, int block,
+                                            long long rows_per_block, float (&part)[8][256]) {
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int n = (across * 32 + tx) * 8;
+  const long long r0 = block * rows_per_block, r1 = min(M, r0 + rows_per_block);
+  const uint8_t *first = reinterpret_cast<const uint8_t*>(g), *last = reinterpret_cast<const uint8_t*>(g + M * N);
+  F2 acc[4] = {F2(0.f, 0.f), F2(0.f, 0.f), F2(0.f, 0.f), F2(0.f, 0.f)};
+  if (n < N) {
+#pragma unroll 8
+    for (long long r = r0 + ty; r < r1; r += 8) {
+      const uint4 t = load_8<ANY>(g + r * N + n, first, last, N - n);
+      if (ANY && copy) *reinterpret_cast<uint4*>(copy + r * ld + n) = t;
+      const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] = add2(acc[j], F2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u)));
+    }
+  }
+  if (!partial) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) acc[j].get(part[ty][(2 * j) * 32 + tx], part[ty][(2 * j + 1) * 32 + tx]);
   __syncthreads();
-  const int c = threadIdx.x;               // column c of the block's 32 V: thread c / V's value c % V
-  if (c < 32 * V && across * 32 * V + c < N) {
-    const int at = (c % V) * 32 + c / V;
+  const int c = threadIdx.x;               // column c of the block's 256: thread c / 8's value c % 8
+  if (across * 256 + c < N) {
+    const int at = (c % 8) * 32 + c / 8;
     float sum = part[0][at];
 #pragma unroll
     for (int i = 1; i < 8; ++i) sum += part[i][at];
-    partial[static_cast<long long>(block) * N + across * 32 * V + c] = sum;
+    partial[static_cast<long long>(block) * N + across * 256 + c] = sum;
   }
 }
-// What the tensor-core launch reads, and the column sums beside it (16384 x 4096, 4096 columns: 335 MB in 60 us): the first sum_blocks * across blocks sum columns of
-// grad_out, the others expand the 8-bit rows.
+// What the tensor-core launch reads, and the column sums beside it (16384 x 4096, 4096 columns: 335 MB in 60 us): the first
+// sum_blocks * across blocks sum columns of grad_out and, where TMA cannot read its rows, copy them; the next w_blocks copy
+// such weights (COPIES), the others expand the 8-bit rows.
 struct PrepareArgs {
   const int8_t* q;
   const float* scale;
@@ -170,21 +197,35 @@ struct PrepareArgs {
   Divisor per_row;
   const __nv_bfloat16* g;
   float* partial;
+  __nv_bfloat16* g_copy;
   long long M, rows_per_block;
-  int N, across, sum_blocks, wide;
+  int N, ld_g, across, sum_blocks;
+  const __nv_bfloat16* w;
+  __nv_bfloat16* w_copy;
+  int K, ld_w, w_blocks;
 };
+template <bool COPIES>
 __global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ PrepareArgs a) {
   __shared__ float part[8][256];
   const unsigned sums = a.sum_blocks * a.across;
   if (blockIdx.x < sums) {
     const int block = blockIdx.x / a.across, across = blockIdx.x - block * a.across;
-    if (a.wide) sum_columns<8>(a.g, a.partial, a.M, a.N, across, block, a.rows_per_block, part);
-    else sum_columns<1>(a.g, a.partial, a.M, a.N, across, block, a.rows_per_block, part);
+    sum_columns<COPIES>(a.g, a.partial, a.g_copy, a.ld_g, a.M, a.N, across, block, a.rows_per_block, part);
+    return;
+  }
+  if (COPIES && blockIdx.x < sums + a.w_blocks) {   // a warp per row
+    const uint8_t *first = reinterpret_cast<const uint8_t*>(a.w), *last = reinterpret_cast<const uint8_t*>(a.w + static_cast<long long>(a.N) * a.K);
+    for (long long row = (blockIdx.x - sums) * 8ll + (threadIdx.x >> 5); row < a.N; row += a.w_blocks * 8ll) {
+#pragma unroll 4
+      for (int k = (threadIdx.x & 31) * 8; k < a.K; k += 256)
+        *reinterpret_cast<uint4*>(a.w_copy + row * a.ld_w + k) = load_8<true>(a.w + row * a.K + k, first, last, a.K - k);
+    }
     return;
   }
   // 4 pieces per thread and turn, their loads together
-  const long long step = (gridDim.x - sums) * 1024ll;
-  for (long long base = (blockIdx.x - sums) * 1024ll + threadIdx.x; base < a.pieces; base += step) {
+  const unsigned before = sums + (COPIES ? a.w_blocks : 0);
+  const long long step = (gridDim.x - before) * 1024ll;
+  for (long long base = (blockIdx.x - before) * 1024ll + threadIdx.x; base < a.pieces; base += step) {
     uint4 w[4];
     float scale[4];
 #pragma unroll
@@ -198,15 +239,6 @@ __global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ Pr
       if (base + u * 256 < a.pieces) expand_piece(w[u], scale[u], a.x, base + u * 256);
   }
 }
-// rows of n bf16 values to rows of ld values, for TMA, which wants rows on 16-byte boundaries
-__global__ void __launch_bounds__(256) pitch_rows_kernel(const __nv_bfloat16* __restrict__ x, __nv_bfloat16* __restrict__ y, long long rows, int n, int ld) {
-  const int lane = threadIdx.x & 31;
-  for (long long row = blockIdx.x * 8ll + (threadIdx.x >> 5); row < rows; row += gridDim.x * 8ll) {
-#pragma unroll 8
-    for (int c = lane; c < n; c += 32) y[row * ld + c] = x[row * n + c];
-  }
-}
-
 // ---------------------------------------------------------------- launches
 struct Operand {
   const void* p;
@@ -356,22 +388,10 @@ void launch_few(grilly_ctx* ctx, const FewArgs& a) {
   else linear_q8_few_kernel<NT, NT == 4 ? 8 : 16><<<blocks, NT == 4 ? 256 : 512, 0, ctx->stream>>>(a);
 }
 
-// bf16 rows that TMA can read: the tensor itself, or a copy with rows of a multiple of 8 values
+// bf16 rows that TMA can read as they are; others are copied to rows of a multiple of 8 values
 bool tma_reads(const void* x, int n) { return n % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
-int pitch_rows(grilly_ctx* ctx, const void* x, long long rows, int n, __nv_bfloat16* copy, Operand* out) {
-  if (tma_reads(x, n)) {
-    *out = {x, n};
-    return GRILLY_OK;
-  }
-  const int ld = (n + 7) / 8 * 8;
-  pitch_rows_kernel<<<static_cast<unsigned>(std::min<long long>((rows + 7) / 8, ctx->num_sms * 16ll)), 256, 0, ctx->stream>>>(
-      static_cast<const __nv_bfloat16*>(x), copy, rows, n, ld);
-  ctx->launches++;
-  GB_CUDA_CHECK(ctx, cudaGetLastError());
-  *out = {copy, ld};
-  return GRILLY_OK;
-}
-size_t pitch_bytes(const void* x, long long rows, int n) { return tma_reads(x, n) ? 0 : static_cast<size_t>(rows) * ((n + 7) / 8 * 8) * 2; }
+int pitch_of(int n) { return (n + 7) / 8 * 8; }
+size_t pitch_bytes(const void* x, long long rows, int n) { return tma_reads(x, n) ? 0 : static_cast<size_t>(rows) * pitch_of(n) * 2; }
 
 }  // namespace
 }  // namespace gb
@@ -466,26 +486,38 @@ int grilly_linear_backward_q8(grilly_ctx* ctx, const void* go, const void* xq, c
     }
     PrepareArgs p{};
     p.per_row = Divisor(1);
-    if (gbias) {
-      p.wide = tma_reads(go, N);
-      p.across = p.wide ? (N + 255) / 256 : (N + 31) / 32;
+    const bool copy_g = jobs.count && !tma_reads(go, N), copy_w = gx && !tma_reads(w, K);
+    if (gbias || copy_g) {
+      p.across = (N + 255) / 256;
       p.sum_blocks = static_cast<int>(std::max<long long>(1, std::min<long long>((M + 63) / 64, ctx->num_sms * 4ll / p.across)));
     }
     Rows8Scratch scratch(ctx);
-    const size_t at_g = scratch.reserve(jobs.count ? pitch_bytes(go, M, N) : 0), at_w = scratch.reserve(gx ? pitch_bytes(w, N, K) : 0);
-    const size_t at_x = scratch.reserve(gw ? static_cast<size_t>(M) * ldx * 2 : 0), at_sums = scratch.reserve(sizeof(float) * static_cast<size_t>(p.sum_blocks) * N);
+    const size_t at_g = scratch.reserve(copy_g ? pitch_bytes(go, M, N) : 0), at_w = scratch.reserve(copy_w ? pitch_bytes(w, N, K) : 0);
+    const size_t at_x = scratch.reserve(gw ? static_cast<size_t>(M) * ldx * 2 : 0), at_sums = scratch.reserve(gbias ? sizeof(float) * static_cast<size_t>(p.sum_blocks) * N : 0);
     const size_t at_parts[2] = {scratch.reserve(part_bytes(jobs.job[0])), scratch.reserve(part_bytes(jobs.job[1]))};
     if ((rc = scratch.take())) return rc;
     Gemm8Finish finish{};
-    // the checkpoint as bf16 rows, and the column sums of grad_out by blocks of rows
+    // the checkpoint as bf16 rows, the column sums of grad_out by blocks of rows, copies
     unsigned blocks = 0;
-    if (gbias) {
+    p.N = N;
+    if (gbias || copy_g) {
       p.g = static_cast<const __nv_bfloat16*>(go);
       p.M = M;
-      p.N = N;
       p.rows_per_block = (M + p.sum_blocks - 1) / p.sum_blocks;
-      p.partial = scratch.at<float>(at_sums);
       blocks = p.across * p.sum_blocks;
+      if (copy_g) p.g_copy = scratch.at<__nv_bfloat16>(at_g);
+      p.ld_g = pitch_of(N);
+    }
+    if (copy_w) {
+      p.w = static_cast<const __nv_bfloat16*>(w);
+      p.w_copy = scratch.at<__nv_bfloat16>(at_w);
+      p.K = K;
+      p.ld_w = pitch_of(K);
+      p.w_blocks = static_cast<int>(std::min<long long>((N + 7) / 8, ctx->num_sms * 4ll));
+      blocks += p.w_blocks;
+    }
+    if (gbias) {
+      p.partial = scratch.at<float>(at_sums);
       finish.partial = p.partial;
       finish.sums = gbias;
       finish.blocks = p.sum_blocks;
@@ -500,16 +532,15 @@ int grilly_linear_backward_q8(grilly_ctx* ctx, const void* go, const void* xq, c
       blocks += static_cast<unsigned>(std::min<long long>((p.pieces + 1023) / 1024, ctx->num_sms * 4ll));
     }
     if (blocks) {
-      const int pi = prof_begin(ctx, PROF_OTHER, 0.0, (gw ? 3.0 * M * K : 0.0) + (gbias ? 2.0 * M * N : 0.0));
-      prepare_kernel<<<blocks, 256, 0, ctx->stream>>>(p);
+      const int pi = prof_begin(ctx, PROF_OTHER, 0.0, (gw ? 3.0 * M * K : 0.0) + (gbias || copy_g ? 2.0 * M * N : 0.0) + (copy_g ? 2.0 * M * N : 0.0) + (copy_w ? 4.0 * N * K : 0.0));
+      if (copy_w || !tma_reads(go, N)) prepare_kernel<true><<<blocks, 256, 0, ctx->stream>>>(p);
+      else prepare_kernel<false><<<blocks, 256, 0, ctx->stream>>>(p);
       prof_end(ctx, pi);
       ctx->launches++;
       GB_CUDA_CHECK(ctx, cudaGetLastError());
     }
     if (jobs.count) {
-      Operand g{}, weights{};
-      if ((rc = pitch_rows(ctx, go, M, N, scratch.at<__nv_bfloat16>(at_g), &g))) return rc;
-      if (gx && (rc = pitch_rows(ctx, w, N, K, scratch.at<__nv_bfloat16>(at_w), &weights))) return rc;
+      const Operand g = copy_g ? Operand{p.g_copy, p.ld_g} : Operand{go, N}, weights = copy_w ? Operand{p.w_copy, p.ld_w} : Operand{w, K};
       Gemm8Maps maps[2];
       for (int j = 0; j < jobs.count; ++j) {
         const Operand b = is_w[j] ? Operand{scratch.at<void>(at_x), ldx} : weights;

@@ -465,6 +465,38 @@ def test_tensors_on_any_boundary_and_what_lies_around_them(backend, rows, featur
     assert np.all(np.abs(gg.numpy() - wg.numpy()) <= 2 * (2 * rows + 8) * U * (np.abs(x) * n).sum(0) + 1e-30)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (7, 5, 3), (70, 37, 41), (70, 40, 41), (70, 37, 48), (530, 263, 130), (600, 1026, 77)])
+@pytest.mark.parametrize("by", [0, 1, 2, 3, 5, 7])
+def test_gradients_whose_rows_are_copied(backend, M, N, K, by):
+    """grad_out and weights that TMA cannot read, amid NaN that belongs to others; every choice of results gives the same."""
+    b, lib, d = backend, backend.device.lib, backend.device
+    rng = rng_for(29, M, N, K)
+    xq, xs = R.quantize(acts(rng, M, K))
+    g, w = R.bf16((0.01 * rng.standard_normal((M, N))).astype(np.float32)), R.bf16(rng.standard_normal((N, K)).astype(np.float32))
+    x8 = put_rows8(b, xq, xs)
+
+    def among_nans(x):
+        flat = np.full(x.size + 64, np.nan, np.float32)
+        flat[32 + by: 32 + by + x.size] = x.reshape(-1)
+        buf = d.upload(flat, "bf16")
+        return buf, DeviceTensor(d, buf.ptr + (32 + by) * 2, x.shape, "bf16", owned=False)
+
+    gbuf, gd = among_nans(g)
+    wbuf, wd = among_nans(w)
+    want = b.fnn.linear_backward_q8(d.upload(g, "bf16"), x8, d.upload(w, "bf16"), dtype="f32")
+    wants = R.linear_backward(g, xq * xs[:, None].astype(np.float64), w)
+    for choice in range(1, 8):
+        outs = [d.upload(np.full(t.shape, 7.0, np.float32)) for t in wants]
+        d.check(lib.grilly_linear_backward_q8(d.ctx, gd.ptr, x8.q.ptr, x8.scale.ptr, wd.ptr if choice & 1 else None,
+                                              *(o.ptr if choice >> i & 1 else None for i, o in enumerate(outs)), M, N, K, x8.ld, 0))
+        for i, (o, t, e) in enumerate(zip(outs, want, wants)):
+            if not choice >> i & 1:
+                assert np.all(o.numpy() == 7)
+                continue
+            assert np.array_equal(o.numpy(), t.numpy())
+            assert np.linalg.norm(o.numpy() - e) <= 4e-3 * np.linalg.norm(e)
+
+
 @pytest.mark.parametrize("by", [1, 4])
 def test_products_on_any_boundary(backend, by):
     """Scales, bias, gradients, weights and results that start off a 16-byte boundary; results keep to themselves."""
