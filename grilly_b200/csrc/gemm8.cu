@@ -337,7 +337,7 @@ int pairs_that_fit(grilly_ctx* ctx, cudaLaunchConfig_t& cfg, cudaLaunchAttribute
 }
 
 template <bool kInt8>
-int launch_gemm8(grilly_ctx* ctx, cudaLaunchConfig_t& cfg, int pairs, const Gemm8Maps* maps, Gemm8Jobs& jobs) {
+int launch_gemm8(grilly_ctx* ctx, cudaLaunchConfig_t& cfg, int pairs, const Gemm8Maps* maps, Gemm8Jobs& jobs, bool follows) {
   int items = 0;
   double flops = 0, bytes = 0;
   for (int j = 0; j < jobs.count; ++j) {
@@ -357,6 +357,7 @@ int launch_gemm8(grilly_ctx* ctx, cudaLaunchConfig_t& cfg, int pairs, const Gemm
   }
   jobs.err = ctx->err_dev;
   cfg.gridDim = dim3(2 * P, 1, 1);
+  if (follows) cfg.attrs[cfg.numAttrs++] = early_launch();
   const int pi = prof_begin(ctx, PROF_GEMM, flops, bytes);
   GB_CUDA_CHECK(ctx, cudaLaunchKernelEx(&cfg, gemm8_pair_kernel<kInt8>, maps[0], maps[jobs.count - 1], jobs));
   prof_end(ctx, pi);
@@ -371,9 +372,8 @@ int launch_finish(grilly_ctx* ctx, Gemm8Finish& f) {
   f.sum_at = static_cast<unsigned>(std::min<long long>((pieces + 511) / 512, ctx->num_sms * 4ll));
   const unsigned grid = f.sum_at + (f.sums ? (f.F + 31) / 32 : 0);
   if (!grid) return GRILLY_OK;
-  gemm8_finish_kernel<kInt8><<<grid, 512, 0, ctx->stream>>>(f);
+  GB_CUDA_CHECK(ctx, launch_following(ctx->stream, gemm8_finish_kernel<kInt8>, grid, 512, f));
   ctx->launches++;
-  GB_CUDA_CHECK(ctx, cudaGetLastError());
   return GRILLY_OK;
 }
 
@@ -427,9 +427,9 @@ int grilly_linear_q8(grilly_ctx* ctx, const void* xq, const float* xs, const voi
       return GRILLY_OK;
     }
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
+    cudaLaunchAttribute attr[2];
     int pairs = 0, rc;
-    if ((rc = pairs_that_fit<true>(ctx, cfg, &attr, &pairs))) return rc;
+    if ((rc = pairs_that_fit<true>(ctx, cfg, attr, &pairs))) return rc;
     Gemm8Jobs jobs{};
     Gemm8Maps maps;
     Gemm8Finish finish{};
@@ -442,7 +442,7 @@ int grilly_linear_q8(grilly_ctx* ctx, const void* xq, const float* xs, const voi
     const size_t at = parts.reserve(part_bytes(g));
     if ((rc = parts.take())) return rc;
     if ((rc = map_gemm8(ctx, true, {xq, ldx}, {wq, ldw}, K, g, maps, parts.at<uint32_t>(at), finish, 0))) return rc;
-    if ((rc = launch_gemm8<true>(ctx, cfg, pairs, &maps, jobs))) return rc;
+    if ((rc = launch_gemm8<true>(ctx, cfg, pairs, &maps, jobs, false))) return rc;
     return launch_finish<true>(ctx, finish);
   });
 }
@@ -467,8 +467,8 @@ int grilly_linear_backward_q8(grilly_ctx* ctx, const void* go, const void* xq, c
     }
     int rc, pairs = 0;
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
-    if ((rc = pairs_that_fit<false>(ctx, cfg, &attr, &pairs))) return rc;
+    cudaLaunchAttribute attr[2];
+    if ((rc = pairs_that_fit<false>(ctx, cfg, attr, &pairs))) return rc;
     // the products, the one with the longer sums first
     Gemm8Jobs jobs{};
     bool is_w[2] = {};
@@ -546,7 +546,7 @@ int grilly_linear_backward_q8(grilly_ctx* ctx, const void* go, const void* xq, c
         const Operand b = is_w[j] ? Operand{scratch.at<void>(at_x), ldx} : weights;
         if ((rc = map_gemm8(ctx, false, g, b, is_w[j] ? M : N, jobs.job[j], maps[j], scratch.at<uint32_t>(at_parts[j]), finish, j))) return rc;
       }
-      if ((rc = launch_gemm8<false>(ctx, cfg, pairs, maps, jobs))) return rc;
+      if ((rc = launch_gemm8<false>(ctx, cfg, pairs, maps, jobs, blocks > 0))) return rc;
     }
     return launch_finish<false>(ctx, finish);
   });

@@ -327,6 +327,7 @@ gemm8_pair_kernel(const __grid_constant__ Gemm8Maps maps0, const __grid_constant
   cluster_sync();                                              // the peer's barriers exist before anything signals them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
+  wait_for_previous_kernel();                                  // what it writes is read from here on
 
   // a failed wait stops both CTAs: the peer's waits poll its own flag
   auto fail = [&](int code) {
@@ -548,7 +549,7 @@ __device__ __forceinline__ void gemm8_join(const Gemm8Args& a, const uint32_t* w
     int s[4] = {0, 0, 0, 0};
 #pragma unroll 4
     for (int p = 0; p < a.splits; ++p) {
-      const uint4 t = __ldg(src + p * (plane / 4));
+      const uint4 t = src[p * (plane / 4)];
       s[0] += static_cast<int>(t.x); s[1] += static_cast<int>(t.y); s[2] += static_cast<int>(t.z); s[3] += static_cast<int>(t.w);
     }
     const float rs = __ldg(a.row_scale + row);
@@ -561,7 +562,7 @@ __device__ __forceinline__ void gemm8_join(const Gemm8Args& a, const uint32_t* w
     v[0] = v[1] = v[2] = v[3] = 0.f;
 #pragma unroll 4
     for (int p = 0; p < a.splits; ++p) {
-      const uint4 t = __ldg(src + p * (plane / 4));
+      const uint4 t = src[p * (plane / 4)];
       v[0] += __uint_as_float(t.x); v[1] += __uint_as_float(t.y); v[2] += __uint_as_float(t.z); v[3] += __uint_as_float(t.w);
     }
   }
@@ -594,6 +595,7 @@ struct Gemm8Finish {
 template <bool kInt8>
 __global__ void __launch_bounds__(512) gemm8_finish_kernel(const __grid_constant__ Gemm8Finish f) {
   __shared__ float part[16][33];
+  wait_for_previous_kernel();
   if (blockIdx.x >= f.sum_at) {
     column_total(f.partial, f.sums, f.blocks, f.F, static_cast<int>(blockIdx.x - f.sum_at), part);
     return;

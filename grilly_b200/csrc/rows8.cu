@@ -950,8 +950,9 @@ __global__ void __launch_bounds__(256) rmsnorm_bwd_long_columns_kernel(const Nor
     a.partial[static_cast<long long>(blockIdx.x) * a.F + f] = acc;
   }
 }
-__global__ void __launch_bounds__(512) sum_partials_kernel(const float* __restrict__ partial, float* __restrict__ out, int blocks, int F) {
+__global__ void __launch_bounds__(512) sum_partials_kernel(const float* partial, float* out, int blocks, int F) {
   __shared__ float part[16][33];
+  wait_for_previous_kernel();
   column_total(partial, out, blocks, F, static_cast<int>(blockIdx.x), part);
 }
 
@@ -1110,7 +1111,7 @@ int launch_rmsnorm_bwd(grilly_ctx* ctx, NormBwdQ8Args& a, float* grad_gamma) {
     kern<<<grid, CTA, smem, ctx->stream>>>(ring, a);
     ctx->launches++;
     if (grad_gamma) {
-      sum_partials_kernel<<<(a.F + 31) / 32, 512, 0, ctx->stream>>>(a.partial, grad_gamma, static_cast<int>(grid), a.F);
+      GB_CUDA_CHECK(ctx, launch_following(ctx->stream, sum_partials_kernel, (a.F + 31) / 32, 512, a.partial, grad_gamma, static_cast<int>(grid), a.F));
       ctx->launches++;
     }
     GB_CUDA_CHECK(ctx, cudaGetLastError());
@@ -1123,7 +1124,7 @@ int launch_rmsnorm_bwd(grilly_ctx* ctx, NormBwdQ8Args& a, float* grad_gamma) {
     if (int rc = scratch.take()) return rc;
     a.partial = scratch.at<float>(at);
     rmsnorm_bwd_long_columns_kernel<T><<<blocks, 256, 0, ctx->stream>>>(a, per);
-    sum_partials_kernel<<<(a.F + 31) / 32, 512, 0, ctx->stream>>>(a.partial, grad_gamma, blocks, a.F);
+    GB_CUDA_CHECK(ctx, launch_following(ctx->stream, sum_partials_kernel, (a.F + 31) / 32, 512, a.partial, grad_gamma, blocks, a.F));
     ctx->launches += 2;
   }
   rmsnorm_bwd_long_rows_kernel<T><<<any_grid(a.rows), 1024, 0, ctx->stream>>>(a);
