@@ -128,14 +128,19 @@ __device__ __forceinline__ uint4 load16_inside(const uint8_t* p, const uint8_t* 
     if (p + 2 * j >= first && p + 2 * j < last) w[j / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + 2 * j)) << (j % 2 * 16);
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-// 8 bf16 values wherever they start, those from `left` on as 0. ANY = false: on a 16-byte boundary, all inside.
-template <bool ANY>
+// 8 bf16 values wherever they start, those from `left` on as 0. INSIDE: the aligned vectors that hold them are.
+template <bool INSIDE>
 __device__ __forceinline__ uint4 load_8(const __nv_bfloat16* x, const uint8_t* first, const uint8_t* last, int left) {
   const uint8_t* p = reinterpret_cast<const uint8_t*>(x);
-  if constexpr (!ANY) return __ldg(reinterpret_cast<const uint4*>(p));
   const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);
-  const uint4 a = load16_inside(p - off, first, last);
-  const uint4 b = 2 * left + off > 16 && off ? load16_inside(p - off + 16, first, last) : make_uint4(0, 0, 0, 0);
+  uint4 a, b;
+  if constexpr (INSIDE) {
+    a = __ldg(reinterpret_cast<const uint4*>(p - off));
+    b = __ldg(reinterpret_cast<const uint4*>(p - off) + (off ? 1 : 0));
+  } else {
+    a = load16_inside(p - off, first, last);
+    b = 2 * left + off > 16 && off ? load16_inside(p - off + 16, first, last) : make_uint4(0, 0, 0, 0);
+  }
   uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
   for (int k = 0; k < 6; ++k) w[k] = off & 8 ? w[k + 2] : w[k];
@@ -163,14 +168,24 @@ __device__ __forceinline__ void sum_columns(const __nv_bfloat16* g, float* parti
   const long long r0 = block * rows_per_block, r1 = min(M, r0 + rows_per_block);
   const uint8_t *first = reinterpret_cast<const uint8_t*>(g), *last = reinterpret_cast<const uint8_t*>(g + M * N);
   F2 acc[4] = {F2(0.f, 0.f), F2(0.f, 0.f), F2(0.f, 0.f), F2(0.f, 0.f)};
-  if (n < N) {
-#pragma unroll 8
-    for (long long r = r0 + ty; r < r1; r += 8) {
-      const uint4 t = load_8<ANY>(g + r * N + n, first, last, N - n);
-      if (ANY && copy) *reinterpret_cast<uint4*>(copy + r * ld + n) = t;
-      const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+  auto take = [&](long long r, uint4 t) {
+    if (ANY && copy) *reinterpret_cast<uint4*>(copy + r * ld + n) = t;
+    const uint32_t w[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] = add2(acc[j], F2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u)));
+    for (int j = 0; j < 4; ++j) acc[j] = add2(acc[j], F2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u)));
+  };
+  if (n < N) {
+    long long r = r0 + ty;
+    if constexpr (ANY) {
+      // rows 28 bytes away from both ends of the tensor go without checks: a row's last vector ends at most that far behind it
+      const long long edge = (13 + N) / N, to = min(r1, M - edge);
+      for (; r < r1 && r < edge; r += 8) take(r, load_8<false>(g + r * N + n, first, last, N - n));
+#pragma unroll 8
+      for (; r < to; r += 8) take(r, load_8<true>(g + r * N + n, first, last, N - n));
+      for (; r < r1; r += 8) take(r, load_8<false>(g + r * N + n, first, last, N - n));
+    } else {
+#pragma unroll 8
+      for (; r < r1; r += 8) take(r, __ldg(reinterpret_cast<const uint4*>(g + r * N + n)));
     }
   }
   if (!partial) return;
@@ -218,7 +233,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ Pr
     for (long long row = (blockIdx.x - sums) * 8ll + (threadIdx.x >> 5); row < a.N; row += a.w_blocks * 8ll) {
 #pragma unroll 4
       for (int k = (threadIdx.x & 31) * 8; k < a.K; k += 256)
-        *reinterpret_cast<uint4*>(a.w_copy + row * a.ld_w + k) = load_8<true>(a.w + row * a.K + k, first, last, a.K - k);
+        *reinterpret_cast<uint4*>(a.w_copy + row * a.ld_w + k) = load_8<false>(a.w + row * a.K + k, first, last, a.K - k);
     }
     return;
   }
