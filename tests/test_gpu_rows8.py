@@ -675,6 +675,51 @@ def test_offsets_past_32_bits(backend):
     assert np.array_equal(tail_out, f.linear_q8(last(got.y8), w8, dtype="bf16").numpy())
 
 
+@pytest.mark.parametrize("values", [1 << 31, 1 << 32])
+def test_offsets_past_32_bits_in_odd_rows(backend, values):
+    """The same where rows start anywhere, and with more elements than 32 bits count."""
+    d, f = backend.device, backend.fnn
+    features = 4097
+    rows = values // features // 8 * 8 + 72
+    x = d.empty((rows, features), "bf16")
+    d.check(d.lib.grilly_memset(d.ctx, x.ptr, 0, x.nbytes))
+    td, _ = put(backend, acts(rng_for(30), 64, features), "bf16")
+    at = (rows - 64) * features * 2
+    d.check(d.lib.grilly_copy_2d(d.ctx, x.ptr + at, td.nbytes, td.ptr, td.nbytes, td.nbytes, 1))
+    tail = lambda t: DeviceTensor(d, t.ptr + at, (64, features), "bf16", owned=False).numpy()  # noqa: E731
+    got, want = f.rmsnorm_residual_q8(x, x, keep=True, out=(None, x, None, None)), f.rmsnorm_residual_q8(td, td, keep=True)
+    assert np.array_equal(tail(x), want.h.numpy())
+    for a, w in ((got.y8, want.y8), (got.h8, want.h8), (f.quantize_rows(x), f.quantize_rows(want.h))):
+        end = DeviceTensor(d, a.q.ptr + (rows - 64) * a.ld, (64, a.ld), "i8", owned=False)
+        assert np.array_equal(end.numpy(), w.q.numpy())
+    gh, _ = f.rmsnorm_backward_q8(x, got.h8, got.rstd, None, x, out=(x, None))
+    assert np.array_equal(tail(gh), f.rmsnorm_backward_q8(want.h, want.h8, want.rstd, None, want.h)[0].numpy())
+    f.dequantize_rows(got.h8, out=x)
+    assert np.array_equal(tail(x), f.dequantize_rows(want.h8, "bf16").numpy())
+
+
+def test_gradients_past_32_bits_in_odd_rows(backend):
+    """grad_out with more than 2^31 elements that TMA cannot read; all but the last rows are zero."""
+    d, f = backend.device, backend.fnn
+    rng = rng_for(31)
+    N, K, last = 1077, 40, 600
+    rows = (1 << 31) // N // 8 * 8 + last
+    xq, xs = R.quantize(acts(rng, last, K))
+    x8, end8 = Rows8.empty(d, (rows, K)), put_rows8(backend, xq, xs)
+    go = d.empty((rows, N), "bf16")
+    for t in (x8.q, x8.scale, go):
+        d.check(d.lib.grilly_memset(d.ctx, t.ptr, 0, t.nbytes))
+    ge, g = put(backend, (0.01 * rng.standard_normal((last, N))).astype(np.float32), "bf16")
+    wd, w = put(backend, rng.standard_normal((N, K)).astype(np.float32), "bf16")
+    for to, end in ((go.ptr + (rows - last) * N * 2, ge), (x8.q.ptr + (rows - last) * x8.ld, end8.q), (x8.scale.ptr + (rows - last) * 4, end8.scale)):
+        d.check(d.lib.grilly_copy_2d(d.ctx, to, end.nbytes, end.ptr, end.nbytes, end.nbytes, 1))
+    gx, gw, gb = f.linear_backward_q8(go, x8, wd, dtype="f32")
+    wants = R.linear_backward(g, xq * xs[:, None].astype(np.float64), w)
+    end = DeviceTensor(d, gx.ptr + (rows - last) * K * 4, (last, K), "f32", owned=False)
+    for t, e in zip((end, gw, gb), wants):
+        assert np.linalg.norm(t.numpy() - e) <= 4e-3 * np.linalg.norm(e)
+
+
 def layer(b, x, r, gm, w8, wd, bias, target):
     """One training step's part: norm into 8 bits, product in 8 bits, gradient of sum(y * target) back to x."""
     f = b.fnn
