@@ -832,10 +832,19 @@ __global__ void __launch_bounds__(CTA, 1) rmsnorm_bwd_kernel(const __grid_consta
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < PAIRS; ++j) acc[i].v[j] = F2(0.f, 0.f);
+  float row_rstd = 0.f, row_scale8 = 0.f;   // of the next row: they come from memory while this one is worked on
+  if (t.row < ring.rows) {
+    row_rstd = __ldg(a.rstd + t.row);
+    row_scale8 = __ldg(a.hs + t.row);
+  }
   for (; t.row < ring.rows; t.template done<ODD>()) {
-    const float rstd = __ldg(a.rstd + t.row), s = __ldg(a.hs + t.row) * rstd;
+    const float rstd = row_rstd, s = row_scale8 * rstd;
     const F2 s2(s, s), rstd2(rstd, rstd);
     if (!t.next()) break;
+    if (t.row + t.step < ring.rows) {
+      row_rstd = __ldg(a.rstd + t.row + t.step);
+      row_scale8 = __ldg(a.hs + t.row + t.step);
+    }
     const uint8_t* qp = t.bytes(0);
     uint8_t* gp = t.bytes(1);
     const uint8_t* rp = ring.tensors > 2 ? t.bytes(2) : nullptr;
