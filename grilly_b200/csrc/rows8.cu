@@ -7,10 +7,11 @@
 // reduce and store a row reached half the bandwidth). A row goes from there into registers, is reduced once and written once.
 // Rows that start off 16-byte boundaries (odd lengths) are copied from the boundary below and shifted into place as they are
 // read (load_piece); 16-bit and 32-bit results leave in the vectors that memory has, 8-bit rows start on boundaries always.
-// 16384 x 4096 bf16: the norm with both outputs 91 us (5.9 TB/s), its backward pass with the residual's gradient 86 us
+// 16384 x 4096 bf16: the norm with both outputs 91 us (5.9 TB/s), its backward pass with the residual's gradient 85 us
 // (5.5 TB/s), quantise 40 us (5.0 TB/s), read back 35 us (5.8 TB/s); a plain copy runs at 6.5 TB/s.
 // 16384 x 4001 bf16: 129 us (4.1 TB/s), 133 (3.5), 55 (3.6) and 36 (5.5); fp32: 191 us (4.8), 185 (4.6), 69 (4.8). The
-// shifts are the difference: half of the issue slots are used, by 66 % more instructions than for aligned rows. Read and
+// shifts are the difference: half of the issue slots are used, by 36 % (norm) and 58 % (backward) more
+// instructions than for aligned rows. Read and
 // stored value by value the same took 177, 146, 79 and 59 us in bf16; only fp32's backward pass was faster, 171.
 #include "rows8.h"
 #include "rows8_sum.cuh"
