@@ -8,7 +8,7 @@
 // Rows that start off 16-byte boundaries (odd lengths) are copied from the boundary below and shifted into place as they are
 // read (load_piece); 16-bit and 32-bit results leave in the vectors that memory has, 8-bit rows start on boundaries always.
 // 16384 x 4096 bf16: the norm with both outputs 91 us (5.9 TB/s), its backward pass with the residual's gradient 85 us
-// (5.5 TB/s), quantise 40 us (5.0 TB/s), read back 35 us (5.8 TB/s); a plain copy runs at 6.5 TB/s.
+// (5.5 TB/s), quantise 39 us (5.1 TB/s), read back 35 us (5.8 TB/s); a plain copy runs at 6.5 TB/s.
 // 16384 x 4001 bf16: 129 us (4.1 TB/s), 133 (3.5), 55 (3.6) and 36 (5.5); fp32: 191 us (4.8), 185 (4.6), 69 (4.8). The
 // shifts are the difference: half of the issue slots are used, by 36 % (norm) and 58 % (backward) more
 // instructions than for aligned rows. Read and
@@ -317,6 +317,7 @@ struct Team {
   uint64_t* bars;
   volatile int* abort_flag;
   int team, tid, slot, parity;   // parity: of the slot's barrier
+  int ok;                        // whether the row's wait ended; the team's word on it after agree()
   uint32_t flip;                 // which half of the reduction scratch
   long long row, step;
 
@@ -385,9 +386,11 @@ struct Team {
     if constexpr (TEAM <= 32) __syncwarp(lanes());
     else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(TEAM) : "memory");
   }
-  // waits for the current row; false: the wait ran out (reported) and the team stops
+  // Waits for the current row. Whether the wait ended (else it is reported and the team stops) is agreed on at once and
+  // returned, or, LATER, by the reduction that follows: one barrier less.
+  template <bool LATER>
   __device__ bool next() {
-    int ok = mbar_wait(&bars[slot], static_cast<uint32_t>(parity), abort_flag) ? 1 : 0;
+    ok = mbar_wait(&bars[slot], static_cast<uint32_t>(parity), abort_flag) ? 1 : 0;
     if (!ok) {
       if (!*abort_flag) atomicCAS(g.err, 0, ERR_WAIT_FULL);
       *abort_flag = 1;
@@ -404,6 +407,12 @@ struct Team {
         }
       }
     }
+    if (row >= g.first_tail) sync();
+    if (!LATER) agree();
+    return LATER || ok != 0;
+  }
+  // a barrier of the team at which ok becomes that of all
+  __device__ void agree() {
     if constexpr (TEAM <= 32) {
       ok = __all_sync(lanes(), ok);
     } else {
@@ -416,7 +425,6 @@ struct Team {
           "}\n"
           : "=r"(ok) : "r"(ok), "r"(team + 1), "n"(TEAM) : "memory");
     }
-    return ok != 0;
   }
   // the current row of tensor i, from the 16-byte boundary at or before its first value, and that value's distance
   __device__ uint8_t* bytes(int i) const { return slot_of(slot) + g.at[i]; }
@@ -441,9 +449,10 @@ struct Team {
     if (*abort_flag)
       for (int i = 0; i < 100; ++i) __nanosleep(10000);
   }
-  // over the team, in an order that its size alone decides
+  // over the team, in an order that its size alone decides; a point where the team agrees on ok
   template <bool kSum, bool kMax, bool kTwo>
   __device__ RowStats reduce(RowStats s) {
+    if constexpr (TEAM <= 32) agree();
     if constexpr (TEAM == 16) {
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) {
@@ -462,7 +471,7 @@ struct Team {
       RowStats* red = reinterpret_cast<RowStats*>(smem + RED_AT) + flip * (CTA / 32);
       flip ^= 1;             // the other half is free again once every thread has passed this row's barriers
       if (lane == 0) red[threadIdx.x >> 5] = s;
-      sync();
+      agree();
       s = lane < WARPS ? red[team * WARPS + lane] : RowStats{0.f, 0.f, 0.f};
       if constexpr (kSum) s.sq = warp_sum(s.sq);
       if constexpr (kMax) s.mh = warp_max(s.mh);
@@ -502,7 +511,7 @@ __global__ void __launch_bounds__(CTA, 1) quantize_rows_kernel(const __grid_cons
   t.template start<VEC>(nullptr);
   const int F = ring.F;
   for (; t.row < ring.rows; t.template done<false>()) {
-    if (!t.next()) break;
+    t.template next<true>();
     const uint8_t* xp = t.bytes(0);
     const int off = ODD ? t.off(0) : 0;
     Piece<VEC> x[NV];
@@ -513,6 +522,7 @@ __global__ void __launch_bounds__(CTA, 1) quantize_rows_kernel(const __grid_cons
       for (int j = 0; j < PAIRS; ++j) m = max_abs(m, x[i].v[j]);
     }
     m = t.template reduce<false, true, false>(RowStats{0.f, 0.f, m}).mh;
+    if (!t.ok) break;
     const float sc = row_scale(m);
     const RowInverse2 inv(row_inverse<sizeof(T) == 2>(sc, m));
     const uint32_t keep = not_finite(m) ? 0u : FULL;
@@ -696,7 +706,7 @@ __global__ void __launch_bounds__(CTA, 1) rmsnorm_q8_kernel(const __grid_constan
   const int F = ring.F;
   const float inv_f = 1.f / static_cast<float>(F);
   for (; t.row < ring.rows; t.template done<ODD && sizeof(T) == 4>()) {
-    if (!t.next()) break;
+    if (!t.template next<!(ODD && sizeof(T) == 4)>()) break;
     uint8_t* xp = t.bytes(0);
     const uint8_t* rp = ring.tensors > 1 ? t.bytes(1) : nullptr;
     const int off = ODD ? t.off(0) : 0;   // of x, residual and h alike
@@ -742,6 +752,7 @@ __global__ void __launch_bounds__(CTA, 1) rmsnorm_q8_kernel(const __grid_constan
     add2(sum[0], sum[1]).get(even, odd);
     s.sq = even + odd;
     s = t.template reduce<true, true, true>(s);
+    if (!t.ok) break;
     const NormScales r = norm_scales(s, inv_f, a.eps);
     const F2 rstd(r.rstd, r.rstd);
     const RowInverse2 yi(row_inverse<true>(r.ys, s.my * r.rstd)), hi(row_inverse<false>(r.hs, s.mh));
@@ -841,7 +852,7 @@ __global__ void __launch_bounds__(CTA, 1) rmsnorm_bwd_kernel(const __grid_consta
   for (; t.row < ring.rows; t.template done<ODD>()) {
     const float rstd = row_rstd, s = row_scale8 * rstd;
     const F2 s2(s, s), rstd2(rstd, rstd);
-    if (!t.next()) break;
+    t.template next<true>();
     if (t.row + t.step < ring.rows) {
       row_rstd = __ldg(a.rstd + t.row + t.step);
       row_scale8 = __ldg(a.hs + t.row + t.step);
@@ -867,6 +878,7 @@ __global__ void __launch_bounds__(CTA, 1) rmsnorm_bwd_kernel(const __grid_consta
     float even, odd;
     add2(dots[0], dots[1]).get(even, odd);
     const float dot = t.template reduce<true, false, false>(RowStats{even + odd, 0.f, 0.f}).sq * inv_f;
+    if (!t.ok) break;
     const F2 back(-s * dot, -s * dot);       // the row's part along n, for the bytes of n
     T* op = static_cast<T*>(a.gh) + t.row * F;
     FOR_PIECES(i, c) {
