@@ -674,12 +674,14 @@ struct NormQ8Args {
 };
 struct NormScales {
   float rstd, ys, hs;
-  uint32_t keep;
+  uint32_t keep_y, keep_h;   // all ones, or zero for a row that is not finite
 };
+// h, its 8-bit rows and rstd follow from the sum of squares alone: a gamma that is not finite is y's affair.
 __device__ __forceinline__ NormScales norm_scales(const RowStats& s, float inv_f, float eps) {
   NormScales r;
-  const bool bad = not_finite(s.sq) || not_finite(s.my);   // a sum of squares: never negative
-  r.keep = bad ? 0u : FULL;
+  const bool bad = not_finite(s.sq);           // a sum of squares: never negative; where it is finite, max |h| is
+  r.keep_h = bad ? 0u : FULL;
+  r.keep_y = bad || not_finite(s.my) ? 0u : FULL;
   const float var = s.sq * inv_f + eps;
   float t = rsqrtf(var);                       // within 2 ulp; one Newton step brings it to the rounding of 1 / sqrt
   t = fmaf(t, fmaf(-0.5f * var * t, t, 0.5f), t);
@@ -760,12 +762,12 @@ __global__ void __launch_bounds__(CTA, 1) rmsnorm_q8_kernel(const __grid_constan
     int8_t* hq = a.hq ? a.hq + t.row * a.ld : nullptr;
     FOR_PIECES(i, c) {
       if (!ODD && hp) store_vec(hp + c, h[i]);
-      if (hq) store_q<false>(hq, c, h[i], hi, r.keep);
+      if (hq) store_q<false>(hq, c, h[i], hi, r.keep_h);
       Piece<VEC> y;
       load_gamma(gamma, c, F, y);
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j) y.v[j] = mul2(mul2(h[i].v[j], rstd), y.v[j]);
-      store_q<true>(yq, c, y, yi, r.keep);
+      store_q<true>(yq, c, y, yi, r.keep_y);
     }
     if (ODD && !ADD_FIRST && hp) write_h();
     for (long long c = (F + VEC - 1) / VEC * VEC + t.tid; c < a.ld; c += TEAM) {
@@ -804,8 +806,8 @@ __global__ void __launch_bounds__(1024) rmsnorm_q8_long_kernel(const NormQ8Args 
         in(c);
         if (a.h) store_one(static_cast<T*>(a.h) + row * a.F + c, h);
       }
-      if (a.hq) a.hq[row * a.ld + c] = round1<false>(h, hi, n.keep);
-      a.yq[row * a.ld + c] = round1<true>(h * n.rstd * gm, yi, n.keep);
+      if (a.hq) a.hq[row * a.ld + c] = round1<false>(h, hi, n.keep_h);
+      a.yq[row * a.ld + c] = round1<true>(h * n.rstd * gm, yi, n.keep_y);
     }
     if (threadIdx.x == 0) norm_row_done(a, n, row);
     __syncthreads();
