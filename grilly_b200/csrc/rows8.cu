@@ -673,21 +673,22 @@ struct NormQ8Args {
   float eps;
 };
 struct NormScales {
-  float rstd, ys, hs;
+  float rstd, ymax, ys, hs;    // ymax: the largest |y|
   uint32_t keep_y, keep_h;   // all ones, or zero for a row that is not finite
 };
 // h, its 8-bit rows and rstd follow from the sum of squares alone: a gamma that is not finite is y's affair.
 __device__ __forceinline__ NormScales norm_scales(const RowStats& s, float inv_f, float eps) {
   NormScales r;
   const bool bad = not_finite(s.sq);           // a sum of squares: never negative; where it is finite, max |h| is
-  r.keep_h = bad ? 0u : FULL;
-  r.keep_y = bad || not_finite(s.my) ? 0u : FULL;
   const float var = s.sq * inv_f + eps;
   float t = rsqrtf(var);                       // within 2 ulp; one Newton step brings it to the rounding of 1 / sqrt
   t = fmaf(t, fmaf(-0.5f * var * t, t, 0.5f), t);
   r.rstd = bad ? ROWS8_NAN : t;
-  r.ys = bad ? ROWS8_NAN : row_scale(s.my * r.rstd);
   r.hs = bad ? ROWS8_NAN : row_scale(s.mh);
+  r.keep_h = bad ? 0u : FULL;
+  r.ymax = s.my * r.rstd;
+  r.ys = row_scale(r.ymax);
+  r.keep_y = not_finite(r.ymax) ? 0u : FULL;
   return r;
 }
 __device__ __forceinline__ void norm_row_done(const NormQ8Args& a, const NormScales& r, long long row) {
@@ -757,7 +758,7 @@ __global__ void __launch_bounds__(CTA, 1) rmsnorm_q8_kernel(const __grid_constan
     if (!t.ok) break;
     const NormScales r = norm_scales(s, inv_f, a.eps);
     const F2 rstd(r.rstd, r.rstd);
-    const RowInverse2 yi(row_inverse<true>(r.ys, s.my * r.rstd)), hi(row_inverse<false>(r.hs, s.mh));
+    const RowInverse2 yi(row_inverse<true>(r.ys, r.ymax)), hi(row_inverse<false>(r.hs, s.mh));
     int8_t* yq = a.yq + t.row * a.ld;
     int8_t* hq = a.hq ? a.hq + t.row * a.ld : nullptr;
     FOR_PIECES(i, c) {
@@ -799,7 +800,7 @@ __global__ void __launch_bounds__(1024) rmsnorm_q8_long_kernel(const NormQ8Args 
     }
     s = block_reduce(s, red);
     const NormScales n = norm_scales(s, 1.f / static_cast<float>(a.F), a.eps);
-    const RowInverse yi = row_inverse<true>(n.ys, s.my * n.rstd), hi = row_inverse<false>(n.hs, s.mh);
+    const RowInverse yi = row_inverse<true>(n.ys, n.ymax), hi = row_inverse<false>(n.hs, s.mh);
     for (long long c = threadIdx.x; c < a.ld; c += blockDim.x) {
       h = gm = 0.f;
       if (c < a.F) {

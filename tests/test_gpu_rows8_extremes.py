@@ -5,7 +5,9 @@ is inside it is no reason for a larger one."""
 import numpy as np
 import pytest
 
-from test_gpu_rows8 import acts, put, rng_for
+from oracle import rows8 as R
+
+from test_gpu_rows8 import U, acts, check_quantised, put, rng_for
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +32,22 @@ def test_a_gamma_that_is_not_finite_leaves_the_checkpoint_alone(backend, feature
         assert np.array_equal(a.numpy(), w.numpy())
     assert np.isfinite(want.rstd.numpy()).all()
     assert np.isnan(got.y8.scale.numpy()).all() and np.all(got.y8.q.numpy() == 0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("features", FEATURES)
+def test_a_norm_that_overflows_has_no_bytes(backend, features, dtype):
+    """y = h rstd gamma above fp32's range although h gamma is inside it: scale NaN, q = 0, the row's checkpoint as ever."""
+    b, f = backend, backend.fnn
+    x = acts(rng_for(41, features), 20, features)
+    x[:, 3] = 2 * np.abs(x).max(-1)          # the row's largest: its normalised value is above 1
+    x *= 0.01 / np.abs(x).max(-1, keepdims=True)
+    xd, x = put(b, x, dtype)
+    gamma = np.ones(features, np.float32)
+    gamma[3] = 3.4e38
+    got = f.rmsnorm_residual_q8(xd, None, gamma, eps=1e-12, keep=True)
+    h, rstd, y = R.rmsnorm(x, None, gamma, 1e-12)
+    assert np.all(y[:, 3] > 3.5e38) and np.abs(h * gamma).max() < 1e37
+    assert np.isnan(got.y8.scale.numpy()).all() and np.all(got.y8.q.numpy() == 0)
+    check_quantised(got.h8, h, U)
+    assert np.all(np.abs(got.rstd.numpy() - rstd) <= (features / 4 + 16) * U * rstd)
