@@ -674,7 +674,12 @@ struct NormQ8Args {
 };
 struct NormScales {
   float rstd, ymax, ys, hs;    // ymax: the largest |y|
-  uint32_t keep_y, keep_h;   // all ones, or zero for a row that is not finite
+  uint32_t keep_y, keep_h;     // all ones, or zero for a row that is not finite
+  __device__ __forceinline__ void set_ymax(float m) {
+    ymax = m;
+    ys = row_scale(m);
+    keep_y = not_finite(m) ? 0u : FULL;
+  }
 };
 // h, its 8-bit rows and rstd follow from the sum of squares alone: a gamma that is not finite is y's affair.
 __device__ __forceinline__ NormScales norm_scales(const RowStats& s, float inv_f, float eps) {
@@ -686,10 +691,15 @@ __device__ __forceinline__ NormScales norm_scales(const RowStats& s, float inv_f
   r.rstd = bad ? ROWS8_NAN : t;
   r.hs = bad ? ROWS8_NAN : row_scale(s.mh);
   r.keep_h = bad ? 0u : FULL;
-  r.ymax = s.my * r.rstd;
-  r.ys = row_scale(r.ymax);
-  r.keep_y = not_finite(r.ymax) ? 0u : FULL;
+  r.set_ymax(s.my * r.rstd);
   return r;
+}
+// rstd max |h gamma| stands for max |y|, but not where a product h gamma has left fp32's range and y = h rstd gamma need not
+// have: above the range, or below its normal numbers with an rstd that brings it back (up to 1024, what is lost is less than
+// 2^-13 of the smallest scale; with an eps of 1e-6 or more rstd is never larger, and a gamma of zeros costs nothing).
+// Then the row's largest |y| is looked for once more, in the values that are quantised.
+__device__ __forceinline__ bool ymax_is_lost(const RowStats& s, float rstd) {
+  return s.mh > 0.f && !not_finite(s.sq) && (not_finite(s.my) || (s.my < ROWS8_TINY && rstd > 1024.f));
 }
 __device__ __forceinline__ void norm_row_done(const NormQ8Args& a, const NormScales& r, long long row) {
   a.ys[row] = r.ys;
@@ -697,8 +707,9 @@ __device__ __forceinline__ void norm_row_done(const NormQ8Args& a, const NormSca
   if (a.rstd) a.rstd[row] = r.rstd;
 }
 
-// One reduction serves both outputs: the largest |h gamma| times rstd is the largest |y|, so sum h^2, max |h gamma| and
-// max |h| are taken together and nothing waits for rstd. A row has been read whole before h is written (in place).
+// One reduction serves both outputs: the largest |h gamma| times rstd is the largest |y| (but see ymax_is_lost), so sum h^2,
+// max |h gamma| and max |h| are taken together and nothing waits for rstd. A row has been read whole before h is written (in
+// place).
 template <class T, int TEAM, bool ODD>
 __global__ void __launch_bounds__(CTA, 1) rmsnorm_q8_kernel(const __grid_constant__ Ring ring, const NormQ8Args a) {
   constexpr int VEC = 16 / sizeof(T), NV = PER_THREAD / VEC, PAIRS = Piece<VEC>::PAIRS;
@@ -756,8 +767,18 @@ __global__ void __launch_bounds__(CTA, 1) rmsnorm_q8_kernel(const __grid_constan
     s.sq = even + odd;
     s = t.template reduce<true, true, true>(s);
     if (!t.ok) break;
-    const NormScales r = norm_scales(s, inv_f, a.eps);
+    NormScales r = norm_scales(s, inv_f, a.eps);
     const F2 rstd(r.rstd, r.rstd);
+    if (ymax_is_lost(s, r.rstd)) {         // the same for all of the team
+      float m = 0.f;
+      FOR_PIECES(i, c) {
+        Piece<VEC> gm;
+        load_gamma(gamma, c, F, gm);
+#pragma unroll
+        for (int j = 0; j < PAIRS; ++j) m = max_abs(m, mul2(mul2(h[i].v[j], rstd), gm.v[j]));
+      }
+      r.set_ymax(t.template reduce<false, false, true>(RowStats{0.f, m, 0.f}).my);
+    }
     const RowInverse2 yi(row_inverse<true>(r.ys, r.ymax)), hi(row_inverse<false>(r.hs, s.mh));
     int8_t* yq = a.yq + t.row * a.ld;
     int8_t* hq = a.hq ? a.hq + t.row * a.ld : nullptr;
@@ -799,7 +820,16 @@ __global__ void __launch_bounds__(1024) rmsnorm_q8_long_kernel(const NormQ8Args 
       s.mh = max_abs(s.mh, h, 0.f);
     }
     s = block_reduce(s, red);
-    const NormScales n = norm_scales(s, 1.f / static_cast<float>(a.F), a.eps);
+    NormScales n = norm_scales(s, 1.f / static_cast<float>(a.F), a.eps);
+    if (ymax_is_lost(s, n.rstd)) {         // the same for the whole block
+      RowStats y{0.f, 0.f, 0.f};
+      for (int c = threadIdx.x; c < a.F; c += blockDim.x) {
+        in(c);
+        y.my = max_abs(y.my, h * n.rstd * gm, 0.f);
+      }
+      __syncthreads();                     // red has been read
+      n.set_ymax(block_reduce(y, red).my);
+    }
     const RowInverse yi = row_inverse<true>(n.ys, n.ymax), hi = row_inverse<false>(n.hs, s.mh);
     for (long long c = threadIdx.x; c < a.ld; c += blockDim.x) {
       h = gm = 0.f;

@@ -7,7 +7,7 @@ import pytest
 
 from oracle import rows8 as R
 
-from test_gpu_rows8 import U, acts, check_quantised, put, rng_for
+from test_gpu_rows8 import EPS, U, acts, check_quantised, put, rng_for
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +51,26 @@ def test_a_norm_that_overflows_has_no_bytes(backend, features, dtype):
     assert np.isnan(got.y8.scale.numpy()).all() and np.all(got.y8.q.numpy() == 0)
     check_quantised(got.h8, h, U)
     assert np.all(np.abs(got.rstd.numpy() - rstd) <= (features / 4 + 16) * U * rstd)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("features", FEATURES)
+@pytest.mark.parametrize("size,scale,eps", [(1e4, 1e36, EPS), (1e-25, 1e-20, 1e-30), (1e-30, 1e-15, 1e-34)])
+def test_products_with_gamma_outside_the_range_of_fp32(backend, features, dtype, size, scale, eps):
+    """h gamma overflows, or is a number of a few bits or 0, while y = h rstd gamma is an ordinary number. Every second row
+    is an ordinary one."""
+    b, f = backend, backend.fnn
+    rng = rng_for(42, features)
+    rows = 41
+    x = acts(rng, rows, features)
+    x[::2] *= np.float32(size)
+    xd, x = put(b, x, dtype)
+    gamma = (scale * (1 + 0.3 * rng.standard_normal(features))).astype(np.float32)
+    got = f.rmsnorm_residual_q8(xd, None, gamma, eps=eps, keep=True)
+    h, rstd, y = R.rmsnorm(x, None, gamma, float(np.float32(eps)))
+    assert np.abs(y).max() < 3e38
+    # the tolerances of test_rmsnorm_residual_q8
+    rel = (features / 4 + 16) * U
+    check_quantised(got.y8, y, rel + 4 * U)
+    check_quantised(got.h8, h, U)
+    assert np.all(np.abs(got.rstd.numpy() - rstd) <= rel * rstd)
