@@ -687,7 +687,7 @@ __device__ __forceinline__ NormScales norm_scales(const RowStats& s, float inv_f
   const bool bad = not_finite(s.sq);           // a sum of squares: never negative; where it is finite, max |h| is
   const float var = s.sq * inv_f + eps;
   float t = rsqrtf(var);                       // within 2 ulp; one Newton step brings it to the rounding of 1 / sqrt
-  t = fmaf(t, fmaf(-0.5f * var * t, t, 0.5f), t);
+  t = fmaf(t, fmaf(var * t, -0.5f * t, 0.5f), t);   // var * t, a normal number, before the half: var need not be normal
   r.rstd = bad ? ROWS8_NAN : t;
   r.hs = bad ? ROWS8_NAN : row_scale(s.mh);
   r.keep_h = bad ? 0u : FULL;

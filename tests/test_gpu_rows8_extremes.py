@@ -74,3 +74,17 @@ def test_products_with_gamma_outside_the_range_of_fp32(backend, features, dtype,
     check_quantised(got.y8, y, rel + 4 * U)
     check_quantised(got.h8, h, U)
     assert np.all(np.abs(got.rstd.numpy() - rstd) <= rel * rstd)
+
+
+@pytest.mark.parametrize("features", FEATURES)
+@pytest.mark.parametrize("eps", [1e-38, 1e-40, 4e-45])
+def test_a_zero_row_with_the_smallest_eps(backend, features, eps):
+    """rstd = 1 / sqrt(eps) where eps is below the smallest normal number; gamma of zeros gives zeros."""
+    got = backend.fnn.rmsnorm_residual_q8(backend.device.upload(np.zeros((3, features), np.float32)), eps=eps, keep=True)
+    want = 1 / np.sqrt(float(np.float32(eps)))
+    # the inverse root to 2 ulp, improved by a step whose own roundings are below an ulp
+    assert np.all(np.abs(got.rstd.numpy() - want) <= 4 * U * want)
+    assert np.all(got.y8.scale.numpy() == R.TINY) and np.all(got.y8.q.numpy() == 0)
+    x = backend.device.upload(acts(rng_for(43), 3, features))
+    y8 = backend.fnn.rmsnorm_residual_q8(x, None, np.zeros(features, np.float32), eps=eps).y8
+    assert np.all(y8.scale.numpy() == R.TINY) and np.all(y8.q.numpy() == 0)
