@@ -408,7 +408,7 @@ gemm8_pair_kernel(const __grid_constant__ Gemm8Maps maps0, const __grid_constant
         const uint64_t a_hi = a0 & 0xffffffff00000000ull, b_hi = b0 & 0xffffffff00000000ull;
         const uint32_t idesc = kInt8 ? make_idesc_i8(256, width) : make_idesc(true, 256, width, a_across, true);
         const int acc = it & 1;
-        if (!mbar_wait(&tmem_empty[acc], ((it >> 1) & 1u) ^ 1u, abort_flag)) { fail(ERR_WAIT_TMEM_EMPTY); break; }
+        if (!mbar_wait_cluster(&tmem_empty[acc], ((it >> 1) & 1u) ^ 1u, abort_flag)) { fail(ERR_WAIT_TMEM_EMPTY); break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * Cfg::TILE;
         for (int kb = k0; kb < k1; ++kb) {

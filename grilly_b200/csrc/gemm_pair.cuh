@@ -146,7 +146,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
       for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++it) {
         const int acc = it & 1;
         const uint32_t acc_phase = (it >> 1) & 1u;
-        if (!mbar_wait(&tmem_empty[acc], acc_phase ^ 1u, abort_flag)) { fail(ERR_WAIT_TMEM_EMPTY); break; }
+        if (!mbar_wait_cluster(&tmem_empty[acc], acc_phase ^ 1u, abort_flag)) { fail(ERR_WAIT_TMEM_EMPTY); break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * Cfg::TILE;
         for (int kb = 0; kb < args.num_k_blocks; ++kb) {

@@ -182,3 +182,22 @@ def test_oracle_gradients_against_differences():
         e = np.zeros(7)
         e[j] = d
         assert abs((loss(h, gamma + e) - loss(h, gamma - e)) / (2 * d) - gg[j]) < 1e-6
+
+
+def test_waits_for_the_other_cta_acquire_at_cluster_scope():
+    """In the kernels of CTA pairs, a barrier on which threads of the other CTA arrive is waited for by mbar_wait_cluster."""
+    import re
+    from pathlib import Path
+
+    import grilly_b200
+
+    found = 0
+    for path in sorted((Path(grilly_b200.__file__).parent / "csrc").glob("*.cu*")):
+        text = path.read_text()
+        remote = dict(re.findall(r"const uint32_t (\w+) = map_to_cta\(&(\w+)\[", text))
+        for address in re.findall(r"mbar_arrive(?:_release)?_cluster\((\w+) [+]", text):
+            barrier = remote[address]
+            waits = re.findall(r"\b(mbar_wait\w*)\(&" + barrier + r"\[", text)
+            assert waits and set(waits) == {"mbar_wait_cluster"}, (path.name, barrier, waits)
+            found += 1
+    assert found >= 3
