@@ -40,16 +40,28 @@ class _Block:
 class DeviceTensor:
     """A contiguous array in device memory. dtype is 'f32', 'bf16', 'i32' or 'i8'."""
 
-    __slots__ = ("dev", "ptr", "shape", "dtype", "_owned", "__weakref__")
+    __slots__ = ("dev", "_ptr", "shape", "dtype", "_owned", "__weakref__")
     _ITEMSIZE = {"f32": 4, "bf16": 2, "i32": 4, "i8": 1}
 
     def __init__(self, dev: "Device", ptr: int, shape, dtype: str, owned: bool = True):
         # a view is made for every operand of a call: this is kept short, and only memory of its own has a finaliser
         self.dev = dev
-        self.ptr = ptr
+        self._ptr = ptr
         self.shape = tuple(map(int, shape))
         self.dtype = dtype
         self._owned = _Block(dev, ptr) if owned is True else owned
+
+    @property
+    def ptr(self) -> int:
+        """Device address. Where the tensor owns its memory, that is whatever address stands here: one that is set later is
+        given back with the tensor, and 0 lets go of the memory without giving it back."""
+        return self._ptr
+
+    @ptr.setter
+    def ptr(self, value: int) -> None:
+        self._ptr = value
+        if type(self._owned) is _Block:
+            self._owned.ptr = value
 
     @property
     def size(self) -> int:
@@ -81,7 +93,7 @@ class DeviceTensor:
     def free(self) -> None:
         if type(self._owned) is _Block:
             self._owned.free()
-            self.ptr = 0
+            self._ptr = 0
 
 
 class Device:

@@ -247,3 +247,45 @@ def test_clock_sampler_without_nvidia_smi(monkeypatch):
               ["0", "210", "1965", "90.0", "Not Active", "Not Active", "Not Active", "Not Active"]]
     out = s.stop()
     assert out["samples"] == 3 and out["sm_mhz"] == 1882.5 and out["sm_max_mhz"] == 1965.0 and out["reasons"] == ["sw_power_cap"]
+
+
+def test_a_tensor_frees_the_address_that_it_holds():
+    """An owning DeviceTensor gives back what its ``ptr`` says when it goes away: set after construction, taken away by 0, once
+    after free(), and not while a view of it lives."""
+    from grilly_b200.device import DeviceTensor
+
+    class Dev:
+        def __init__(self):
+            self.freed = []
+
+        def free_ptr(self, p):
+            self.freed.append(p)
+
+    dev = Dev()
+    t = DeviceTensor(dev, 0, (4,), "f32")
+    t.ptr = 4096
+    assert t.ptr == 4096
+    del t
+    assert dev.freed == [4096]
+    t = DeviceTensor(dev, 8192, (4,), "f32")
+    t.ptr = 0                                   # handed over to somebody else
+    del t
+    assert dev.freed == [4096]
+    t = DeviceTensor(dev, 8192, (4,), "f32")
+    view = t.reshape(2, 2).reshape(4)
+    del t
+    assert dev.freed == [4096] and view.ptr == 8192
+    view.ptr = 0                                # a view's address is its own
+    del view
+    assert dev.freed == [4096, 8192]
+    t = DeviceTensor(dev, 12288, (4,), "f32")
+    t.free()
+    assert t.ptr == 0
+    t.free()
+    del t
+    assert dev.freed == [4096, 8192, 12288]
+    t = DeviceTensor(dev, 16384, (4,), "f32", owned=False)
+    t.ptr = 20480
+    t.free()
+    del t
+    assert dev.freed == [4096, 8192, 12288]
