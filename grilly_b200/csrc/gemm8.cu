@@ -427,9 +427,9 @@ int grilly_linear_q8(grilly_ctx* ctx, const void* xq, const float* xs, const voi
     if (M == 0) return GRILLY_OK;
     if (!y) return set_error(ctx, GRILLY_ERR_INVALID_ARG, "linear_q8: null output");
     const int out_bf16 = (flags & GRILLY_FLAG_OUT_BF16) ? 1 : 0;
-    const Rows8Span outs[] = {{y, M * N * (out_bf16 ? 2 : 4)}};
+    const Rows8Span outs[] = {{y, M * N * (out_bf16 ? 2 : 4), 0, out_bf16 ? 2 : 4}};
     const Rows8Span ins[] = {{xq, M * ldx}, {xs, 4 * M}, {wq, N * ldw}, {ws, 4ll * N}, {bias, 4ll * N}};
-    if (int rc = rows8_apart(ctx, "linear_q8", outs, ins)) return rc;
+    if (int rc = rows8_memory(ctx, "linear_q8", outs, ins)) return rc;
     if (M <= FEW_TOKENS) {
       const FewArgs a{static_cast<const int8_t*>(xq), xs, static_cast<const int8_t*>(wq), ws, bias, y, static_cast<int>(M), N, K, ldx, ldw, act, out_bf16};
       const int pi = prof_begin(ctx, PROF_GEMM, 2.0 * M * N * K, static_cast<double>(N) * K + M * (K + (out_bf16 ? 2.0 : 4.0) * N));
@@ -472,9 +472,9 @@ int grilly_linear_backward_q8(grilly_ctx* ctx, const void* go, const void* xq, c
     if (M > 0 && !go) return set_error(ctx, GRILLY_ERR_INVALID_ARG, "linear_backward_q8: null gradient");
     if (gx && !w) return set_error(ctx, GRILLY_ERR_INVALID_ARG, "linear_backward_q8: grad_x needs the weights");
     const int elt = bf16 ? 2 : 4;
-    const Rows8Span outs[] = {{gx, M * K * elt}, {gw, static_cast<long long>(N) * K * elt}, {gbias, 4ll * N}};
-    const Rows8Span ins[] = {{go, M * N * 2}, {xq, M * ldx}, {xs, 4 * M}, {w, static_cast<long long>(N) * K * 2}};
-    if (int rc = rows8_apart(ctx, "linear_backward_q8", outs, ins)) return rc;
+    const Rows8Span outs[] = {{gx, M * K * elt, 0, elt}, {gw, static_cast<long long>(N) * K * elt, 0, elt}, {gbias, 4ll * N}};
+    const Rows8Span ins[] = {{go, M * N * 2, 0, 2}, {xq, M * ldx}, {xs, 4 * M}, {w, static_cast<long long>(N) * K * 2, 0, 2}};
+    if (int rc = rows8_memory(ctx, "linear_backward_q8", outs, ins)) return rc;
     if (M == 0) {
       if (gw) GB_CUDA_CHECK(ctx, cudaMemsetAsync(gw, 0, static_cast<size_t>(N) * K * (bf16 ? 2 : 4), ctx->stream));
       if (gbias) GB_CUDA_CHECK(ctx, cudaMemsetAsync(gbias, 0, sizeof(float) * N, ctx->stream));

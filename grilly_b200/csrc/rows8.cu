@@ -1208,8 +1208,9 @@ int grilly_quantize_rows(grilly_ctx* ctx, const void* x, void* q, float* scale, 
     if (rows == 0) return GRILLY_OK;
     if (!x) return set_error(ctx, GRILLY_ERR_INVALID_ARG, "quantize_rows: null input");
     const bool bf16 = flags & GRILLY_FLAG_IN_BF16;
-    const Rows8Span outs[] = {{q, rows * ld}, {scale, 4 * rows}}, ins[] = {{x, rows * features * (bf16 ? 2 : 4)}};
-    if (int rc = rows8_apart(ctx, "quantize_rows", outs, ins)) return rc;
+    const int elt = bf16 ? 2 : 4;
+    const Rows8Span outs[] = {{q, rows * ld}, {scale, 4 * rows}}, ins[] = {{x, rows * features * elt, 0, elt}};
+    if (int rc = rows8_memory(ctx, "quantize_rows", outs, ins)) return rc;
     const int pi = prof_begin(ctx, PROF_NORM, 2.0 * rows * features, static_cast<double>(rows) * features * (bf16 ? 3 : 5) + 4.0 * rows);
     const int rc = bf16 ? launch_quantize(ctx, static_cast<const __nv_bfloat16*>(x), static_cast<int8_t*>(q), scale, rows, features, ld)
                         : launch_quantize(ctx, static_cast<const float*>(x), static_cast<int8_t*>(q), scale, rows, features, ld);
@@ -1223,8 +1224,9 @@ int grilly_dequantize_rows(grilly_ctx* ctx, const void* q, const float* scale, v
     if (rows == 0) return GRILLY_OK;
     if (!y) return set_error(ctx, GRILLY_ERR_INVALID_ARG, "dequantize_rows: null output");
     const bool bf16 = flags & GRILLY_FLAG_OUT_BF16;
-    const Rows8Span outs[] = {{y, rows * features * (bf16 ? 2 : 4)}}, ins[] = {{q, rows * ld}, {scale, 4 * rows}};
-    if (int rc = rows8_apart(ctx, "dequantize_rows", outs, ins)) return rc;
+    const int elt = bf16 ? 2 : 4;
+    const Rows8Span outs[] = {{y, rows * features * elt, 0, elt}}, ins[] = {{q, rows * ld}, {scale, 4 * rows}};
+    if (int rc = rows8_memory(ctx, "dequantize_rows", outs, ins)) return rc;
     const int pi = prof_begin(ctx, PROF_NORM, 1.0 * rows * features, static_cast<double>(rows) * features * (bf16 ? 3 : 5) + 4.0 * rows);
     if (bf16) launch_dequantize(ctx, static_cast<const int8_t*>(q), scale, static_cast<__nv_bfloat16*>(y), rows, features, ld);
     else launch_dequantize(ctx, static_cast<const int8_t*>(q), scale, static_cast<float*>(y), rows, features, ld);
@@ -1242,10 +1244,11 @@ int grilly_rmsnorm_residual_q8(grilly_ctx* ctx, const void* x, const void* resid
     if (rows == 0) return GRILLY_OK;
     if (!x) return set_error(ctx, GRILLY_ERR_INVALID_ARG, "rmsnorm_residual_q8: null input");
     const bool bf16 = flags & GRILLY_FLAG_IN_BF16;
-    const long long size = rows * features * (bf16 ? 2 : 4);
-    const Rows8Span outs[] = {{h, size}, {y_q, rows * ld}, {y_scale, 4 * rows}, {h_q, rows * ld}, {h_scale, 4 * rows}, {rstd, 4 * rows}};
-    const Rows8Span ins[] = {{x, size, 1}, {residual, size, 1}, {gamma, 4ll * features}};
-    if (int rc = rows8_apart(ctx, "rmsnorm_residual_q8", outs, ins)) return rc;
+    const int elt = bf16 ? 2 : 4;
+    const long long size = rows * features * elt;
+    const Rows8Span outs[] = {{h, size, 0, elt}, {y_q, rows * ld}, {y_scale, 4 * rows}, {h_q, rows * ld}, {h_scale, 4 * rows}, {rstd, 4 * rows}};
+    const Rows8Span ins[] = {{x, size, 1, elt}, {residual, size, 1, elt}, {gamma, 4ll * features}};
+    if (int rc = rows8_memory(ctx, "rmsnorm_residual_q8", outs, ins)) return rc;
     NormQ8Args a{x, residual, gamma, h, static_cast<int8_t*>(y_q), y_scale, static_cast<int8_t*>(h_q), h_scale, rstd, rows, ld, features, eps};
     const double e = bf16 ? 2 : 4, n = static_cast<double>(rows) * features;
     const int pi = prof_begin(ctx, PROF_NORM, 8.0 * n, n * (e * (1 + (residual ? 1 : 0) + (h ? 1 : 0)) + 1 + (h_q ? 1 : 0)) + 4.0 * features + 12.0 * rows);
@@ -1264,10 +1267,11 @@ int grilly_rmsnorm_backward_q8(grilly_ctx* ctx, const void* go, const void* h_q,
     }
     if (!go || !rstd || !grad_h) return set_error(ctx, GRILLY_ERR_INVALID_ARG, "rmsnorm_backward_q8: null operand");
     const bool bf16 = flags & GRILLY_FLAG_IN_BF16;
-    const long long size = rows * features * (bf16 ? 2 : 4);
-    const Rows8Span outs[] = {{grad_h, size}, {grad_gamma, 4ll * features}};
-    const Rows8Span ins[] = {{go, size, 1}, {grad_residual, size, 1}, {h_q, rows * ld}, {h_scale, 4 * rows}, {rstd, 4 * rows}, {gamma, 4ll * features}};
-    if (int rc = rows8_apart(ctx, "rmsnorm_backward_q8", outs, ins)) return rc;
+    const int elt = bf16 ? 2 : 4;
+    const long long size = rows * features * elt;
+    const Rows8Span outs[] = {{grad_h, size, 0, elt}, {grad_gamma, 4ll * features}};
+    const Rows8Span ins[] = {{go, size, 1, elt}, {grad_residual, size, 1, elt}, {h_q, rows * ld}, {h_scale, 4 * rows}, {rstd, 4 * rows}, {gamma, 4ll * features}};
+    if (int rc = rows8_memory(ctx, "rmsnorm_backward_q8", outs, ins)) return rc;
     NormBwdQ8Args a{go, static_cast<const int8_t*>(h_q), h_scale, rstd, gamma, grad_residual, grad_h, nullptr, rows, ld, features};
     const double e = bf16 ? 2 : 4, n = static_cast<double>(rows) * features;
     const int pi = prof_begin(ctx, PROF_NORM, 10.0 * n, n * (e * (2 + (grad_residual ? 1 : 0)) + 1) + 8.0 * features + 8.0 * rows);

@@ -72,21 +72,27 @@ inline int rows8_check(grilly_ctx* ctx, const char* who, const void* q, const vo
   return GRILLY_OK;
 }
 
-// An operand's memory. `in_place`: number (from 1) of the output that may be this very memory.
+// An operand's memory. `in_place`: number (from 1) of the output that may be this very memory. `align`: bytes of an element.
 struct Rows8Span {
   const void* p;
   long long bytes;
   int in_place = 0;
+  int align = 4;
 };
-// Outputs may overlap neither each other nor an input, but for an input that is an output's very memory where that is
-// offered: the kernels read inputs while other blocks write.
+// Every tensor starts on a boundary of its own type: the kernels load whole elements. Outputs may overlap neither each other
+// nor an input, but for an input that is an output's very memory where that is offered: the kernels read inputs while other
+// blocks write.
 template <int OUTS, int INS>
-int rows8_apart(grilly_ctx* ctx, const char* who, const Rows8Span (&outs)[OUTS], const Rows8Span (&ins)[INS]) {
+int rows8_memory(grilly_ctx* ctx, const char* who, const Rows8Span (&outs)[OUTS], const Rows8Span (&ins)[INS]) {
+  auto off = [](const Rows8Span& a) { return reinterpret_cast<uintptr_t>(a.p) % a.align != 0; };
   auto overlap = [](const Rows8Span& a, const Rows8Span& b) {
     const auto x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
     return a.p && b.p && x < y + static_cast<uintptr_t>(b.bytes) && y < x + static_cast<uintptr_t>(a.bytes);
   };
+  for (const Rows8Span& in : ins)
+    if (off(in)) return set_error(ctx, GRILLY_ERR_INVALID_ARG, std::string(who) + ": an operand does not start on a boundary of its type");
   for (int i = 0; i < OUTS; ++i) {
+    if (off(outs[i])) return set_error(ctx, GRILLY_ERR_INVALID_ARG, std::string(who) + ": a result does not start on a boundary of its type");
     for (int j = 0; j < i; ++j)
       if (overlap(outs[i], outs[j])) return set_error(ctx, GRILLY_ERR_INVALID_ARG, std::string(who) + ": two results share memory");
     for (const Rows8Span& in : ins)

@@ -286,7 +286,8 @@ int grilly_transpose_2d(grilly_ctx* ctx, const float* in_dev, float* out_dev, in
  * stand beside its linear, RMSNorm and backward entry points. All are asynchronous on the context's stream, keep no
  * state between calls and can be captured into a CUDA graph; scratch comes from the pool in stream order. rows = 0 is
  * allowed (gradients summed over rows are then zero). Results share no memory with each other or with operands, but for
- * the in-place forms that are named (else GRILLY_ERR_INVALID_ARG). Sums have a fixed order: results repeat bit for bit, and a row
+ * the in-place forms that are named, and floating tensors start on a boundary of their own type, 4 or 2 bytes (else
+ * GRILLY_ERR_INVALID_ARG). Sums have a fixed order: results repeat bit for bit, and a row
  * quantised, normed or multiplied on tensors that start on 16-byte boundaries has the same bits in every batch. A row that
  * stands for NaN makes its own results NaN, and with them every sum over rows that it is part of. */
 /* x [rows][features] fp32, or bf16 with GRILLY_FLAG_IN_BF16, -> q, scale. A weight matrix (out, in) quantised this way

@@ -856,3 +856,48 @@ def test_two_contexts_at_the_same_time(lib):
     for runs in out.values():
         for r in runs[1:]:
             assert all(np.array_equal(a, c) for a, c in zip(runs[0], r))
+
+
+def test_library_refuses_tensors_off_their_own_boundary(backend):
+    """An fp32 tensor off a 4-byte boundary, a bf16 one off a 2-byte boundary: refused by every entry point, nothing launched."""
+    d, lib = backend.device, backend.device.lib
+    q, q2, s, s2, s3 = d.empty((4, 64), "i8"), d.empty((4, 64), "i8"), d.empty((8,)), d.empty((8,)), d.empty((8,))
+    x, y, z, g, w = (d.empty((8, 64)) for _ in range(5))
+    before = d.launch_count()
+
+    def quantize(a=0, b=0, flags=0):
+        return lib.grilly_quantize_rows(d.ctx, x.ptr + a, q.ptr, s.ptr + b, 4, 64, 64, flags)
+
+    def dequantize(a=0, b=0, flags=0):
+        return lib.grilly_dequantize_rows(d.ctx, q.ptr, s.ptr + a, x.ptr + b, 4, 64, 64, flags)
+
+    def norm(by=(0,) * 7, flags=0):
+        return lib.grilly_rmsnorm_residual_q8(d.ctx, x.ptr + by[0], y.ptr + by[1], g.ptr + by[2], z.ptr + by[3], q.ptr, s.ptr + by[4],
+                                              q2.ptr, s2.ptr + by[5], s3.ptr + by[6], 4, 64, 64, 1e-5, flags)
+
+    def linear(by=(0,) * 4, flags=0):
+        return lib.grilly_linear_q8(d.ctx, q.ptr, s.ptr + by[0], q2.ptr, s2.ptr + by[1], s3.ptr + by[2], x.ptr + by[3], 4, 4, 64, 64, 64, 0, flags)
+
+    def linear_backward(by=(0,) * 6, flags=0):
+        return lib.grilly_linear_backward_q8(d.ctx, x.ptr + by[0], q.ptr, s.ptr + by[1], w.ptr + by[2], y.ptr + by[3], z.ptr + by[4], s3.ptr + by[5],
+                                             4, 4, 64, 64, flags)
+
+    def norm_backward(by=(0,) * 7, flags=0):
+        return lib.grilly_rmsnorm_backward_q8(d.ctx, x.ptr + by[0], q.ptr, s.ptr + by[1], s2.ptr + by[2], g.ptr + by[3], y.ptr + by[4],
+                                              z.ptr + by[5], w.ptr + by[6], 4, 64, 64, flags)
+
+    bad = [quantize(1), quantize(2), quantize(0, 2), quantize(1, 0, L.FLAG_IN_BF16), dequantize(1), dequantize(0, 2), dequantize(0, 3, L.FLAG_OUT_BF16)]
+    for call, n in ((norm, 7), (linear, 4), (linear_backward, 6), (norm_backward, 7)):
+        for i in range(n):
+            for flags in (0, L.FLAG_IN_BF16 | L.FLAG_OUT_BF16):
+                bad += [call(tuple(by if j == i else 0 for j in range(n)), flags) for by in (1, 3)]
+    bad += [norm((2, 0, 0, 0, 0, 0, 0)), norm((0, 0, 0, 2, 0, 0, 0)), linear((0, 0, 0, 2)), linear_backward((0, 0, 0, 2, 0, 0)),
+            norm_backward((2, 0, 0, 0, 0, 0, 0)), norm_backward((0, 0, 0, 0, 0, 2, 0))]
+    assert bad == [L.ERR_INVALID_ARG] * len(bad) and d.launch_count() == before
+    # bf16 tensors on any 2-byte boundary are taken
+    both = L.FLAG_IN_BF16 | L.FLAG_OUT_BF16
+    for t in (x, y, z, g, w, s, s2, s3, q, q2):
+        d.check(lib.grilly_memset(d.ctx, t.ptr, 0, t.nbytes))
+    assert [quantize(2, 0, both), dequantize(0, 2, both), norm((2, 6, 0, 2, 0, 0, 0), both), linear((0, 0, 0, 2), both),
+            linear_backward((2, 0, 2, 2, 2, 0), both), norm_backward((2, 0, 0, 0, 2, 2, 0), both)] == [L.OK] * 6
+    d.sync()
