@@ -21,7 +21,6 @@ struct FewArgs {
   long long ldx, ldw;
   int act, out_bf16;
 };
-constexpr int FEW_TOKENS = 32;
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -392,15 +391,31 @@ int launch_finish(grilly_ctx* ctx, Gemm8Finish& f) {
   return GRILLY_OK;
 }
 
+// Which products go to linear_q8_few_kernel, which to the tensor-core tiles; the results are the same. Up to 16 tokens cost
+// about as much as one, the weights' bytes (us here | tiles at 16 tokens: 1536 x 384 2.3 | 6.1, 4096 x 4096 7.0 | 15.2,
+// 16384 x 4096 17.2 | 20.3, 65536 x 512 13.7 | 14.2, 100000 x 768 24.0 | 24.5), but where few blocks share a long row, which
+// tiles split along k (1024 x 16384 14.1 | 14.1, 2048 x 32768 28.1 | 21.8, 512 x 65536 48.9 | 18.3, 4096 x 32768 33.2 | 35.7).
+// With more tokens their bytes, read again for every 16 features, and the mma.sync pipe count. At 32 tokens: 4096 x 4096
+// 10.9 | 15.2, 6144 x 4096 12.9 | 15.6, 6144 x 384 6.5 | 6.9, 8192 x 384 8.3 | 6.9, 8192 x 4096 19.9 | 16.1, 2048 x 8192
+// 15.2 | 13.7, 16384 x 4096 21.9 | 19.0, 4096 x 16384 30.4 | 21.5.
+bool few_tokens(long long M, int N, int K) {
+  if (M <= 16) return K <= 16384 || N > 2048;
+  return M <= 32 && N <= 6144 && K <= 4096;
+}
+
 template <int NT>
 void launch_few(grilly_ctx* ctx, const FewArgs& a) {
   // about 4096 warps on the GPU, whatever N: many blocks of 4 warps, or few of 16 that share a longer row (for a single
   // token 4096 x 4096 takes 6.7, 4.2 and 3.9 us with 4, 8 and 16 warps, 16384 x 4096 15.7, 16.6 and 18.6 us). 32 tokens
-  // make the warps' join dearer: at most 8 (22, 33 and 49 us at 16384 x 4096, 50, 30 and 36 us at 4096 x 16384).
+  // make the warps' join dearer: 8 (4096 x 4096 takes 14.8, 10.9 and 14.5 us, 6144 x 1024 6.7, 7.7 and 13.5).
   const unsigned blocks = (a.N + 15) / 16;
-  if (blocks > 512) linear_q8_few_kernel<NT, 4><<<blocks, 128, 0, ctx->stream>>>(a);
-  else if (blocks > 256 || NT == 4) linear_q8_few_kernel<NT, 8><<<blocks, 256, 0, ctx->stream>>>(a);
-  else linear_q8_few_kernel<NT, NT == 4 ? 8 : 16><<<blocks, NT == 4 ? 256 : 512, 0, ctx->stream>>>(a);
+  if constexpr (NT == 4) {
+    linear_q8_few_kernel<NT, 8><<<blocks, 256, 0, ctx->stream>>>(a);
+  } else {
+    if (blocks > 512) linear_q8_few_kernel<NT, 4><<<blocks, 128, 0, ctx->stream>>>(a);
+    else if (blocks > 256) linear_q8_few_kernel<NT, 8><<<blocks, 256, 0, ctx->stream>>>(a);
+    else linear_q8_few_kernel<NT, 16><<<blocks, 512, 0, ctx->stream>>>(a);
+  }
 }
 
 // bf16 rows that TMA can read as they are; others are copied to rows of a multiple of 8 values
@@ -430,7 +445,7 @@ int grilly_linear_q8(grilly_ctx* ctx, const void* xq, const float* xs, const voi
     const Rows8Span outs[] = {{y, M * N * (out_bf16 ? 2 : 4), 0, out_bf16 ? 2 : 4}};
     const Rows8Span ins[] = {{xq, M * ldx}, {xs, 4 * M}, {wq, N * ldw}, {ws, 4ll * N}, {bias, 4ll * N}};
     if (int rc = rows8_memory(ctx, "linear_q8", outs, ins)) return rc;
-    if (M <= FEW_TOKENS) {
+    if (few_tokens(M, N, K)) {
       const FewArgs a{static_cast<const int8_t*>(xq), xs, static_cast<const int8_t*>(wq), ws, bias, y, static_cast<int>(M), N, K, ldx, ldw, act, out_bf16};
       const int pi = prof_begin(ctx, PROF_GEMM, 2.0 * M * N * K, static_cast<double>(N) * K + M * (K + (out_bf16 ? 2.0 : 4.0) * N));
       if (M <= 8) launch_few<1>(ctx, a);

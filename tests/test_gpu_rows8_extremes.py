@@ -1,13 +1,14 @@
-"""The 8-bit row operators at the ends of fp32's range, against the formulas in 64 bits.
+"""The 8-bit row operators at the ends of fp32's range and at the borders between kernels, against the formulas in 64 bits.
 
 Tolerances are those of the ordinary sizes (U is half a step of fp32): a value beyond fp32's range on the way to a result that
 is inside it is no reason for a larger one."""
 import numpy as np
 import pytest
 
+from grilly_b200 import Rows8
 from oracle import rows8 as R
 
-from test_gpu_rows8 import EPS, U, acts, check_quantised, put, rng_for
+from test_gpu_rows8 import EPS, U, acts, check_quantised, linear_case, put, rng_for
 
 pytestmark = pytest.mark.gpu
 
@@ -88,3 +89,21 @@ def test_a_zero_row_with_the_smallest_eps(backend, features, eps):
     x = backend.device.upload(acts(rng_for(43), 3, features))
     y8 = backend.fnn.rmsnorm_residual_q8(x, None, np.zeros(features, np.float32), eps=eps).y8
     assert np.all(y8.scale.numpy() == R.TINY) and np.all(y8.q.numpy() == 0)
+
+
+@pytest.mark.parametrize("N,K", [(6144, 4096), (6160, 4096), (6144, 4112), (4096, 8192), (100, 4112), (2048, 16400), (2064, 16400)])
+@pytest.mark.parametrize("M", [16, 17, 32, 33])
+def test_linear_q8_where_one_kernel_gives_way_to_the_other(backend, M, N, K):
+    """Few tokens under large weights, on both sides of the rule that chooses the kernel: right, and a token has the same bits."""
+    got, _ = linear_case(backend, M, N, K, "silu", True, "f32", seed=1)
+    b, f = backend, backend.fnn
+    rng = rng_for(6, M, N, K, 1)            # the operands of linear_case
+    xq, xs = R.quantize(acts(rng, M, K))
+    wq, ws = R.quantize((rng.standard_normal((N, K)) * K ** -0.5).astype(np.float32))
+    bias = (0.1 * rng.standard_normal(N)).astype(np.float32)
+    def rows8(q, s):
+        buf = np.zeros((len(q), (K + 15) // 16 * 16), np.int8)
+        buf[:, :K] = q
+        return Rows8(b.device.upload(buf, "i8"), b.device.upload(np.asarray(s, np.float32)), (len(q), K))
+    one = f.linear_q8(rows8(xq[M - 1:], xs[M - 1:]), rows8(wq, ws), bias, act="silu").numpy()
+    assert np.array_equal(got.numpy()[M - 1:], one)
