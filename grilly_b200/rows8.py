@@ -157,8 +157,9 @@ class Rows8Ops:
     # ---- operators --------------------------------------------------------------------------
     def quantize_rows(self, x, out=None) -> Rows8:
         """``x`` (..., features) in 8-bit rows: per row scale = max|x| / 127 (at least 2^-126) and x / scale rounded to the
-        nearest integer, ties to even (a tie is one of x / (max|x| / 127) in exact arithmetic), so a value is off by at most scale / 2. A row with a NaN or an infinity reads back
-        as NaN. An activation's checkpoint, or a weight (out, in) with one scale per output channel for ``linear_q8``."""
+        nearest integer, ties to even (a tie is one of x / (max|x| / 127) in exact arithmetic), so q * scale is off by at most
+        half a step and the scale's own rounding, (1/2 + 2^-17) scale. A row with a NaN or an infinity reads back as NaN. An
+        activation's checkpoint, or a weight (out, in) with one scale per output channel for ``linear_q8``."""
         shape = self._shape(x, "x")
         y8 = self._rows8_out(out, shape)
         xd, _ = self._float_in(x, "x")
@@ -167,7 +168,8 @@ class Rows8Ops:
         return y8
 
     def dequantize_rows(self, x8: Rows8, dtype="f32", out=None) -> DeviceTensor:
-        """The values of 8-bit rows as an 'f32' or 'bf16' DeviceTensor of their shape."""
+        """The values of 8-bit rows as an 'f32' or 'bf16' DeviceTensor of their shape: the fp32 product q * scale, for bf16
+        rounded to that."""
         self._rows8_in(x8, "x8")
         if dtype not in _FLOAT:
             raise ValueError("dtype must be 'f32' or 'bf16'")
@@ -179,7 +181,8 @@ class Rows8Ops:
     def rmsnorm_residual_q8(self, x, residual=None, gamma=None, eps=1e-5, keep=False, out=None) -> NormQ8:
         """h = x + residual and RMSNorm(h) * gamma in 8-bit rows, in one pass over the rows (``residual`` then ``rmsnorm``,
         with 8 bits written instead of 32). ``keep`` also gives what ``rmsnorm_backward_q8`` needs: h in 8-bit rows and
-        the rows' 1 / sqrt(mean(h^2) + eps). The statistics and y come from the unrounded fp32 sum.
+        the rows' 1 / sqrt(mean(h^2) + eps). The statistics and y come from the unrounded fp32 sum. A row of y with a value
+        that is not finite (by gamma, say) reads back as NaN; h, h8 and rstd depend on h alone.
 
         x and residual share shape and type; h has that type too. ``out`` = (y8, h, h8, rstd), each None for a new
         tensor; h may be x or residual (in place), h8 and rstd belong to ``keep``."""
@@ -214,10 +217,11 @@ class Rows8Ops:
 
     def linear_q8(self, x, weights, bias=None, act=None, dtype="f32", out=None):
         """act(x @ W.T + b) on 8-bit rows: int8 products, exact 32-bit sums, then the token's and the channel's scale, the
-        bias and the activation (None, 'gelu', 'silu', 'relu'), rounded once to ``dtype`` ('f32' or 'bf16').
+        bias and the activation (None, 'gelu', 'silu', 'relu') in fp32, rounded to ``dtype`` ('f32' or 'bf16') at the end.
 
         ``x`` and ``weights`` (out, in) are Rows8; an array or a floating DeviceTensor is quantised in this call (keep
-        ``quantize_rows(weights)`` to do that once). At most 131071 input features."""
+        ``quantize_rows(weights)`` to do that once). At most 131071 input features; rows of |x| above 2^104 may leave fp32's
+        range before the channel's scale brings them back."""
         if act not in _ACT:
             raise ValueError("act must be None, 'gelu', 'silu' or 'relu'")
         if dtype not in _FLOAT:

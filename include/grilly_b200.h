@@ -280,21 +280,24 @@ int grilly_transpose_2d(grilly_ctx* ctx, const float* in_dev, float* out_dev, in
  * A tensor in 8-bit rows is an int8 matrix q [rows][ld] (ld >= features, a multiple of 16; the base 16-byte aligned;
  * the buffer holds rows * ld bytes) and one fp32 scale per row; element (r, c) stands for q[r][c] * scale[r].
  * Written here: scale = max(max|row| / 127, 2^-126), q = x / scale rounded to the nearest integer (ties to even; the
- * quotient by the scale before its own rounding to fp32, so max|row| / 2 is a tie and gives 64), so |q| <= 127 and a value is off by at most scale / 2; a zero row is exact. A row that holds a NaN or an infinity gets
- * scale NaN and q = 0: every value read back from it is NaN. Bytes between features and ld are written as 0 and never
- * change a result when read. The reference has no 8-bit type (its layers store fp32, backend/fnn.py:1437-1489); these
- * stand beside its linear, RMSNorm and backward entry points. All are asynchronous on the context's stream, keep no
- * state between calls and can be captured into a CUDA graph; scratch comes from the pool in stream order. rows = 0 is
- * allowed (gradients summed over rows are then zero). Results share no memory with each other or with operands, but for
- * the in-place forms that are named, and floating tensors start on a boundary of their own type, 4 or 2 bytes (else
- * GRILLY_ERR_INVALID_ARG). Sums have a fixed order: results repeat bit for bit, and a row
- * quantised, normed or multiplied on tensors that start on 16-byte boundaries has the same bits in every batch. A row that
- * stands for NaN makes its own results NaN, and with them every sum over rows that it is part of. */
+ * quotient by the scale before its own rounding to fp32, so max|row| / 2 is a tie and gives 64). So |q| <= 127, and
+ * q * scale is off by at most (1/2 + 2^-17) scale: half a step, and 127 times the scale's rounding; a zero row is exact. A
+ * row that holds a NaN or an infinity gets scale NaN and q = 0: every value read back from it is NaN. Bytes between
+ * features and ld are written as 0 and never change a result when read. The reference has no 8-bit type (its layers store
+ * fp32, backend/fnn.py:1437-1489); these stand beside its linear, RMSNorm and backward entry points. All are asynchronous
+ * on the context's stream, keep no state between calls and can be captured into a CUDA graph; scratch comes from the pool
+ * in stream order. rows = 0 is allowed (gradients summed over rows are then zero). Results share no memory with each other
+ * or with operands, but for the in-place forms that are named, and floating tensors start on a boundary of their own type,
+ * 4 or 2 bytes (else GRILLY_ERR_INVALID_ARG). Sums have a fixed order: results repeat bit for bit, and a row quantised,
+ * normed or multiplied (grilly_quantize_rows, grilly_rmsnorm_residual_q8, grilly_linear_q8) on tensors that start on
+ * 16-byte boundaries has the same bits in every batch. A row that stands for NaN makes its own results NaN, and with them
+ * every sum over rows that it is part of. */
 /* x [rows][features] fp32, or bf16 with GRILLY_FLAG_IN_BF16, -> q, scale. A weight matrix (out, in) quantised this way
  * carries one scale per output channel. */
 int grilly_quantize_rows(grilly_ctx* ctx, const void* x_dev, void* q_dev, float* scale_dev, long long rows, int features,
                          long long ld, int flags);
-/* q, scale -> y [rows][features] fp32, or bf16 with GRILLY_FLAG_OUT_BF16 (the product, rounded once). */
+/* q, scale -> y [rows][features] fp32, or bf16 with GRILLY_FLAG_OUT_BF16 (the fp32 product,
+ * rounded to bf16). */
 int grilly_dequantize_rows(grilly_ctx* ctx, const void* q_dev, const float* scale_dev, void* y_dev, long long rows, int features,
                            long long ld, int flags);
 /* h = x + residual (residual NULL: h = x); rstd = 1 / sqrt(mean(h^2) + eps); y = h * rstd * gamma (gamma NULL: 1), written
@@ -302,13 +305,15 @@ int grilly_dequantize_rows(grilly_ctx* ctx, const void* q_dev, const float* scal
  * h. Optional outputs (NULL: not written): h_dev [rows][features] in the inputs' type; h_q with h_scale, h in 8-bit rows
  * (the checkpoint that grilly_rmsnorm_backward_q8 reads), and rstd_dev [rows]. h_dev may be x_dev or residual_dev (in
  * place). x, residual and h are fp32, or bf16 with GRILLY_FLAG_IN_BF16. eps > 0. A row whose sum of squares is not a
- * finite fp32 number counts as a row with an infinity. */
+ * finite fp32 number counts as a row with an infinity. What gamma makes of a row shows in y alone: where a value of y is
+ * not finite, y_scale is NaN and the row of y_q 0, and h, its 8-bit rows and rstd are as with any other gamma. */
 int grilly_rmsnorm_residual_q8(grilly_ctx* ctx, const void* x_dev, const void* residual_dev, const float* gamma_dev, void* h_dev,
                                void* y_q_dev, float* y_scale_dev, void* h_q_dev, float* h_scale_dev, float* rstd_dev,
                                long long rows, int features, long long ld, float eps, int flags);
 /* y[m][n] = act(x_scale[m] * w_scale[n] * sum_k x_q[m][k] * w_q[n][k] + bias[n]), y [M][N] fp32 or bf16
  * (GRILLY_FLAG_OUT_BF16): fnn-linear.glsl:33-58 and its fused activations on 8-bit rows. The sum is exact (int32):
- * K <= 131071. bias fp32 or NULL; act in GRILLY_ACT_*. */
+ * K <= 131071. It is multiplied by x_scale[m] first, in fp32: rows of |x| up to 2^104 stay inside fp32's range there, whatever
+ * K is. bias fp32 or NULL; act in GRILLY_ACT_*. */
 int grilly_linear_q8(grilly_ctx* ctx, const void* x_q_dev, const float* x_scale_dev, const void* w_q_dev, const float* w_scale_dev,
                      const float* bias_dev, void* y_dev, long long M, int N, int K, long long ld_x, long long ld_w, int act, int flags);
 /* Backward pass of y = x W^T + b (backend/fnn.py:1501-1573) from the 8-bit checkpoint of x [M][K]:

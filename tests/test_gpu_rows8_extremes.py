@@ -107,3 +107,15 @@ def test_linear_q8_where_one_kernel_gives_way_to_the_other(backend, M, N, K):
         return Rows8(b.device.upload(buf, "i8"), b.device.upload(np.asarray(s, np.float32)), (len(q), K))
     one = f.linear_q8(rows8(xq[M - 1:], xs[M - 1:]), rows8(wq, ws), bias, act="silu").numpy()
     assert np.array_equal(got.numpy()[M - 1:], one)
+
+
+@pytest.mark.parametrize("M", [1, 20, 40, 200, 2000])
+def test_linear_q8_of_the_largest_rows_that_stay_in_range(backend, M):
+    """|x| = 2^104 in every one of 131071 columns: the sum times the row's scale is just inside fp32's range."""
+    K, N = 131071, 70
+    xs, ws = np.full(M, np.float32(2.0 ** 104 / 127)), np.full(N, np.float32(1e-30))
+    def rows8(n, s):
+        return Rows8(backend.device.upload(np.full((n, K + 1), 127, np.int8), "i8"), backend.device.upload(s), (n, K))
+    got = backend.fnn.linear_q8(rows8(M, xs), rows8(N, ws)).numpy()
+    want = K * 127.0 * 127.0 * float(xs[0]) * float(ws[0])
+    assert np.all(np.abs(got - want) <= 4 * U * want)     # the sum, two products and the result round once each

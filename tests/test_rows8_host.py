@@ -201,3 +201,17 @@ def test_waits_for_the_other_cta_acquire_at_cluster_scope():
             assert waits and set(waits) == {"mbar_wait_cluster"}, (path.name, barrier, waits)
             found += 1
     assert found >= 3
+
+
+def test_half_a_step_and_the_rounding_of_the_scale():
+    """|q scale - x| <= (1/2 + 2^-17) scale: x is at most half a step from q max / 127, and the scale at most 2^-24 of itself
+    from max / 127, up to 127 times. Half a step alone is not a bound."""
+    rng = np.random.default_rng(2)
+    x = R.bf16((rng.standard_normal((300, 4000)) * np.exp(rng.uniform(-3, 3, (300, 1)))).astype(np.float32))
+    # next to a tie at 126.5 steps, on the side that the rounded scale is worse for
+    a = np.abs(x).max(-1).astype(np.float64)
+    x[:, 0] = np.float32(a * 126.5 / 127)
+    x[:, 1] = np.float32(a)
+    q, s = R.quantize(x)
+    steps = np.abs(q * s[:, None].astype(np.float64) - x) / s[:, None].astype(np.float64)
+    assert 0.5 < steps.max() <= 0.5 + 2.0 ** -17
