@@ -9,10 +9,10 @@
 // read (load_piece); 16-bit and 32-bit results leave in the vectors that memory has, 8-bit rows start on boundaries always.
 // 16384 x 4096 bf16: the norm with both outputs 91 us (5.9 TB/s), its backward pass with the residual's gradient 85 us
 // (5.5 TB/s), quantise 39 us (5.1 TB/s), read back 35 us (5.8 TB/s); a plain copy runs at 6.5 TB/s.
-// 16384 x 4001 bf16: 129 us (4.1 TB/s), 133 (3.5), 55 (3.6) and 36 (5.5); fp32: 191 us (4.8), 185 (4.6), 69 (4.8). The
-// shifts are the difference: half of the issue slots are used, by 36 % (norm) and 58 % (backward) more
-// instructions than for aligned rows. Read and
-// stored value by value the same took 177, 146, 79 and 59 us in bf16; only fp32's backward pass was faster, 171.
+// 16384 x 4001 bf16: 131 us (4.0 TB/s), 132 (3.5), 52 (3.8) and 36 (5.5); fp32: 196 us (4.7), 185 (4.6), 68 (4.8). The
+// shifts are the difference: half of the issue slots are used, by 36 % (norm) and 55 % (backward) more
+// instructions than for aligned rows. Read and stored value by value the same took 177, 146, 79 and 59 us in bf16; only
+// fp32's backward pass was faster, 171.
 #include "rows8.h"
 #include "rows8_sum.cuh"
 #include "ptx.cuh"
@@ -1053,7 +1053,7 @@ int make_ring(grilly_ctx* ctx, Ring& g, long long rows, int F, const RowTensor* 
   g.slots_at = GAMMA_AT + (gamma ? (F + 7) / 8 * 32 : 0);
   // the smallest team that holds a row, but few enough of them that each has two rows in shared memory: the threads that
   // long rows leave without a row of their own join the others. Rows of which only one fits are loaded one after the other
-  // (5000 x 11001 fp32: the norm 189 us, its backward pass 199; read twice from memory instead 413 and 838)
+  // (5000 x 11001 fp32: the norm 196 us, its backward pass 200; read twice from memory instead 413 and 838)
   const int room = RING_BYTES - g.slots_at;
   int team = MIN_TEAM;
   while (team < CTA && (team * PER_THREAD < F || CTA / team * 2 * g.slot > room)) team *= 2;
