@@ -1024,8 +1024,7 @@ constexpr int RING_BYTES = 216 * 1024;
 // result the same bits, in every batch.
 struct RowTensor {
   const void* p;
-  long long pitch;   // bytes
-  int bytes;
+  long long pitch, bytes;   // from row to row, and of a row (more than an int holds where the ring does not take them)
 };
 // Returns the threads per row, or 0.
 int make_ring(grilly_ctx* ctx, Ring& g, long long rows, int F, const RowTensor* tensors, int count, bool gamma, bool gamma_sums, size_t* smem, unsigned* grid) {
@@ -1041,13 +1040,13 @@ int make_ring(grilly_ctx* ctx, Ring& g, long long rows, int F, const RowTensor* 
     if (reinterpret_cast<uintptr_t>(tensors[i].p) & 15) return 0;
     g.src[i] = tensors[i].p;
     g.pitch[i] = tensors[i].pitch;
-    g.bytes[i] = tensors[i].bytes;
+    g.bytes[i] = static_cast<int>(tensors[i].bytes);
     g.total[i] = tensors[i].pitch * (rows - 1) + tensors[i].bytes;
     const long long whole = g.total[i] & ~15ll;
     g.first_tail = std::min(g.first_tail, whole < g.bytes[i] ? 0 : (whole - g.bytes[i]) / g.pitch[i] + 1);
     g.at[i] = g.slot;
     if (g.pitch[i] % 16 || g.bytes[i] % 16) g.aligned = 0;
-    g.slot += (tensors[i].bytes + 15) / 16 * 16 + (tensors[i].pitch % 16 ? 16 : 0);
+    g.slot += (g.bytes[i] + 15) / 16 * 16 + (tensors[i].pitch % 16 ? 16 : 0);
   }
   g.gamma_at = GAMMA_AT;
   g.slots_at = GAMMA_AT + (gamma ? (F + 7) / 8 * 32 : 0);
@@ -1091,7 +1090,8 @@ int launch_quantize(grilly_ctx* ctx, const T* x, int8_t* q, float* scale, long l
   Ring ring;
   size_t smem;
   unsigned grid;
-  const RowTensor in[1] = {{x, static_cast<long long>(sizeof(T)) * F, static_cast<int>(sizeof(T)) * F}};
+  const long long pitch = static_cast<long long>(sizeof(T)) * F;
+  const RowTensor in[1] = {{x, pitch, pitch}};
   const int team = make_ring(ctx, ring, rows, F, in, 1, false, false, &smem, &grid);
   if (!team) {
     quantize_long_rows_kernel<<<any_grid(rows), 1024, 0, ctx->stream>>>(x, q, scale, rows, F, ld);
@@ -1128,7 +1128,7 @@ int launch_rmsnorm(grilly_ctx* ctx, const NormQ8Args& a) {
   size_t smem;
   unsigned grid;
   const long long pitch = static_cast<long long>(sizeof(T)) * a.F;
-  const RowTensor in[2] = {{a.x, pitch, static_cast<int>(pitch)}, {a.residual, pitch, static_cast<int>(pitch)}};
+  const RowTensor in[2] = {{a.x, pitch, pitch}, {a.residual, pitch, pitch}};
   const int team = aligned16({a.h}) ? make_ring(ctx, ring, a.rows, a.F, in, a.residual ? 2 : 1, a.gamma != nullptr, false, &smem, &grid) : 0;
   if (!team) {
     rmsnorm_q8_long_kernel<T><<<any_grid(a.rows), 1024, 0, ctx->stream>>>(a);
@@ -1150,7 +1150,7 @@ int launch_rmsnorm_bwd(grilly_ctx* ctx, NormBwdQ8Args& a, float* grad_gamma) {
   size_t smem;
   unsigned grid;
   const long long pitch = static_cast<long long>(sizeof(T)) * a.F;
-  const RowTensor in[3] = {{a.hq, a.ld, (a.F + 15) / 16 * 16}, {a.go, pitch, static_cast<int>(pitch)}, {a.gr, pitch, static_cast<int>(pitch)}};
+  const RowTensor in[3] = {{a.hq, a.ld, (a.F + 15) / 16 * 16}, {a.go, pitch, pitch}, {a.gr, pitch, pitch}};
   const int team = aligned16({a.gh}) ? make_ring(ctx, ring, a.rows, a.F, in, a.gr ? 3 : 2, a.gamma != nullptr, grad_gamma != nullptr, &smem, &grid) : 0;
   if (team) {
     void (*kern)(const Ring, const NormBwdQ8Args) = nullptr;

@@ -5,7 +5,7 @@ is inside it is no reason for a larger one."""
 import numpy as np
 import pytest
 
-from grilly_b200 import Rows8
+from grilly_b200 import DeviceTensor, Rows8
 from oracle import rows8 as R
 
 from test_gpu_rows8 import EPS, U, acts, check_quantised, linear_case, put, rng_for
@@ -119,3 +119,35 @@ def test_linear_q8_of_the_largest_rows_that_stay_in_range(backend, M):
     got = backend.fnn.linear_q8(rows8(M, xs), rows8(N, ws)).numpy()
     want = K * 127.0 * 127.0 * float(xs[0]) * float(ws[0])
     assert np.all(np.abs(got - want) <= 4 * U * want)     # the sum, two products and the result round once each
+
+
+def test_the_longest_row(backend):
+    """2^30 features, the most there may be: the row's ends are where they should be, the zeros between them are zeros."""
+    d, f, rng = backend.device, backend.fnn, rng_for(44)
+    F = 1 << 30
+    x = d.empty((1, F), "bf16")
+    d.check(d.lib.grilly_memset(d.ctx, x.ptr, 0, x.nbytes))
+    ends = R.bf16(rng.standard_normal((1, 128)).astype(np.float32))
+    for at, part in ((0, ends[:, :64]), ((F - 64) * 2, ends[:, 64:])):
+        t = d.upload(part, "bf16")
+        d.check(d.lib.grilly_copy_2d(d.ctx, x.ptr + at, t.nbytes, t.ptr, t.nbytes, t.nbytes, 1))
+    q, s = R.quantize(ends)
+
+    def view(t, first, n):
+        item = {"i8": 1, "bf16": 2}[t.dtype]
+        return DeviceTensor(d, t.ptr + first * item, (n,), t.dtype, owned=False).numpy()
+
+    def check(r8):
+        assert np.array_equal(view(r8.q, 0, 64), q[0, :64]) and np.array_equal(view(r8.q, F - 64, 64), q[0, 64:])
+        assert not view(r8.q, 64, 4096).any() and not view(r8.q, F - 4160, 4096).any()
+
+    r8 = f.quantize_rows(x)
+    check(r8)
+    assert np.array_equal(r8.scale.numpy(), s)
+    got = f.rmsnorm_residual_q8(x, eps=1e-12, keep=True, out=(None, x, None, None))
+    check(got.y8)
+    check(got.h8)
+    rstd = R.rmsnorm(ends, None, None, 0.0)[1] * np.sqrt(F / 128)       # eps is 8e-6 of the mean square
+    assert abs(got.rstd.numpy()[0] - rstd[0]) <= (128 * U + 1e-5) * rstd[0]
+    back = f.dequantize_rows(r8, out=x)
+    assert np.array_equal(view(back, F - 64, 64), R.bf16((q[0, 64:] * s[0].astype(np.float64)).astype(np.float32)))
