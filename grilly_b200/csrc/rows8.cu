@@ -219,7 +219,8 @@ struct RowInverse2 {
   __device__ __forceinline__ explicit RowInverse2(RowInverse r) : hi(r.hi, r.hi), lo(r.lo, r.lo) {}
 };
 // ONE = false: 127 / a as a sum of two floats. A product and a fused multiply-add give the quotient right to 2^-47 before
-// its rounding to fp32, so that a tie comes out as that tie.
+// its rounding to fp32, so that a tie comes out as that tie (and what is nearer to one than 2^-18, half a step of an fp32
+// number of 64 to 127, becomes one).
 // ONE: for bf16 values one float rounded up and one fused multiply-add do. 254 x and a (2 k + 1) have 16 bits each and are
 // equal or 2^-16 apart, equal only where a is 127 * 2^j (the inverse is a power of two then, the product exact) or
 // x = a / 2, and that tie goes up, to 64.

@@ -157,9 +157,10 @@ class Rows8Ops:
     # ---- operators --------------------------------------------------------------------------
     def quantize_rows(self, x, out=None) -> Rows8:
         """``x`` (..., features) in 8-bit rows: per row scale = max|x| / 127 (at least 2^-126) and x / scale rounded to the
-        nearest integer, ties to even (a tie is one of x / (max|x| / 127) in exact arithmetic), so q * scale is off by at most
-        half a step and the scale's own rounding, (1/2 + 2^-17) scale. A row with a NaN or an infinity reads back as NaN. An
-        activation's checkpoint, or a weight (out, in) with one scale per output channel for ``linear_q8``."""
+        nearest integer, ties to even (a tie is one of x / (max|x| / 127); of fp32 values also what lies within 2^-18 of one),
+        so q * scale is off by at most half a step and the scale's own rounding, (1/2 + 2^-16) scale. A row with a NaN or an
+        infinity reads back as NaN. An activation's checkpoint, or a weight (out, in) with one scale per output channel for
+        ``linear_q8``."""
         shape = self._shape(x, "x")
         y8 = self._rows8_out(out, shape)
         xd, _ = self._float_in(x, "x")

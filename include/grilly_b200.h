@@ -280,8 +280,9 @@ int grilly_transpose_2d(grilly_ctx* ctx, const float* in_dev, float* out_dev, in
  * A tensor in 8-bit rows is an int8 matrix q [rows][ld] (ld >= features, a multiple of 16; the base 16-byte aligned;
  * the buffer holds rows * ld bytes) and one fp32 scale per row; element (r, c) stands for q[r][c] * scale[r].
  * Written here: scale = max(max|row| / 127, 2^-126), q = x / scale rounded to the nearest integer (ties to even; the
- * quotient by the scale before its own rounding to fp32, so max|row| / 2 is a tie and gives 64). So |q| <= 127, and
- * q * scale is off by at most (1/2 + 2^-17) scale: half a step, and 127 times the scale's rounding; a zero row is exact. A
+ * quotient by the scale before its own rounding to fp32, so max|row| / 2 is a tie and gives 64; of fp32 values the quotient
+ * is rounded to fp32 first, so what lies within 2^-18 of a tie counts as one). So |q| <= 127, and q * scale is off by at
+ * most (1/2 + 2^-16) scale: half a step, 2^-18 of one, and up to 127 times the scale's rounding; a zero row is exact. A
  * row that holds a NaN or an infinity gets scale NaN and q = 0: every value read back from it is NaN. Bytes between
  * features and ld are written as 0 and never change a result when read. The reference has no 8-bit type (its layers store
  * fp32, backend/fnn.py:1437-1489); these stand beside its linear, RMSNorm and backward entry points. All are asynchronous
@@ -306,7 +307,8 @@ int grilly_dequantize_rows(grilly_ctx* ctx, const void* q_dev, const float* scal
  * (the checkpoint that grilly_rmsnorm_backward_q8 reads), and rstd_dev [rows]. h_dev may be x_dev or residual_dev (in
  * place). x, residual and h are fp32, or bf16 with GRILLY_FLAG_IN_BF16. eps > 0. A row whose sum of squares is not a
  * finite fp32 number counts as a row with an infinity. What gamma makes of a row shows in y alone: where a value of y is
- * not finite, y_scale is NaN and the row of y_q 0, and h, its 8-bit rows and rstd are as with any other gamma. */
+ * not finite, y_scale is NaN and the row of y_q 0, and h, its 8-bit rows and rstd are as with any other gamma. y and the
+ * quotient that y_q is rounded from are fp32 numbers with a few roundings each, which comes on top of the half step. */
 int grilly_rmsnorm_residual_q8(grilly_ctx* ctx, const void* x_dev, const void* residual_dev, const float* gamma_dev, void* h_dev,
                                void* y_q_dev, float* y_scale_dev, void* h_q_dev, float* h_scale_dev, float* rstd_dev,
                                long long rows, int features, long long ld, float eps, int flags);

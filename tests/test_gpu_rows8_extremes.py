@@ -151,3 +151,24 @@ def test_the_longest_row(backend):
     assert abs(got.rstd.numpy()[0] - rstd[0]) <= (128 * U + 1e-5) * rstd[0]
     back = f.dequantize_rows(r8, out=x)
     assert np.array_equal(view(back, F - 64, 64), R.bf16((q[0, 64:] * s[0].astype(np.float64)).astype(np.float32)))
+
+
+@pytest.mark.parametrize("features", [384, 1001, 4096, 17000])
+def test_next_to_ties(backend, features):
+    """fp32 values a few roundings away from ties: the nearest integer but for what is closer to a tie than half a step of the
+    fp32 quotient (2^-18 at 64 to 127), and the documented distance from x."""
+    rng = rng_for(45, features)
+    a = rng.uniform(1, 2, (64, 1)) * 2.0 ** rng.integers(-60, 60, (64, 1))
+    x = a * (rng.integers(-127, 127, (64, features)) + 0.5 + rng.uniform(-1, 1, (64, features)) * 2.0 ** rng.uniform(-26, -12, (64, features))) / 127
+    x[:, 5] = a[:, 0]
+    x = x.astype(np.float32)
+    a = np.abs(x).max(-1, keepdims=True).astype(np.float64)
+    steps = 127 * x.astype(np.float64) / a
+    xd = backend.device.upload(x)
+    in_range = (x.astype(np.float64) ** 2).sum(-1) < 3e38          # the others are infinite rows to the norm
+    for r8, rows in ((backend.fnn.quantize_rows(xd), slice(None)), (backend.fnn.rmsnorm_residual_q8(xd, keep=True).h8, in_range)):
+        q, s = r8.q.numpy()[rows, :features].astype(np.float64), r8.scale.numpy()[rows, None].astype(np.float64)
+        assert np.all(np.abs(q - steps[rows]) <= 0.5 + 2.0 ** -18)
+        clear = np.abs(steps[rows] - np.floor(steps[rows]) - 0.5) > 2.0 ** -18
+        assert clear.mean() > 0.3 and np.array_equal(q[clear], np.rint(steps[rows][clear]))
+        assert np.all(np.abs(q * s - x[rows]) <= (0.5 + 2.0 ** -16) * s)
